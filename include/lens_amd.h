@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define LENS_AMD_ABI_VERSION 11
+#define LENS_AMD_ABI_VERSION 12
 
 /* Rows of slack behind the currents buffer of lens_feature_currents / lens_feature_fire. */
 #define LENS_FIRE_SLACK_ROWS 32
@@ -55,8 +55,18 @@ enum {
     LENS_ERR_SIZE = -2,        /* a size / stride argument is out of range */
     LENS_ERR_UNSUPPORTED = -3, /* valid request outside what the kernels implement (see each function) */
     LENS_ERR_ALIGN = -4,       /* a pointer / leading dimension violates the stated alignment */
-    LENS_ERR_SCRATCH = -5      /* lens_forward_counts_static: the batch does not fit the static scratch array */
+    LENS_ERR_SCRATCH = -5      /* lens_forward_counts_static: the batch does not fit the static scratch array;
+                                  event-stream operators: scratch_bytes is less than the call needs */
 };
+
+/* Element types of the event-stream operators. */
+enum { LENS_F32 = 0, LENS_BF16 = 1, LENS_F16 = 2 };
+
+#define LENS_EMBED_MAX_TOKENS 2147000000ll   /* events of one call */
+#define LENS_EMBED_MAX_ROWS 2147483000ll     /* rows of a table */
+#define LENS_EMBED_MAX_DIM 2048              /* channels of a row */
+#define LENS_SCAN_MAX_ROWS 2147000000ll      /* rows (events) of one scan, all sequences together */
+#define LENS_SCAN_MAX_DIM 4096               /* channels of a state */
 
 /* ABI version of the loaded library (== LENS_AMD_ABI_VERSION it was built with). */
 int lens_amd_abi_version(void);
@@ -349,6 +359,100 @@ int lens_sad_matrix(const uint8_t *d_query, int Q, const uint8_t *d_reference, i
  */
 int lens_output_counts_dense(const float *d_featspk, int Q, int T, int F, int ld_f, const float *d_w2t, int P, int ldw2,
                              float *d_counts, int ldo, void *stream);
+
+
+/* ---------------------------------------------------------------------------------------------
+ * Event streams, event by event.  The reference bins events into frames before its network sees them
+ * (lens/collect_data.py:193-199) and its layers are never differentiated; these operators have no counterpart there.
+ * An event's address (polarity, y, x) is a token, a row of a learned table is its input current, and leaky states integrate
+ * the currents; all three have their gradients.
+ *
+ * Types: LENS_F32, LENS_BF16 or LENS_F16 where a `type` is passed, float elsewhere.  All arithmetic is 32-bit; a 16-bit
+ * output is rounded once.  Leading dimensions count elements; rows are contiguous in their last index and aligned to their
+ * elements.  Results do not depend on timing: the same inputs give the same bits.
+ * Scratch is the caller's, 16-byte aligned, contents irrelevant; two calls that may overlap need scratch of their own.
+ * ------------------------------------------------------------------------------------------- */
+
+/*
+ * Lookup with scaling:  out[i] = scale * weight[i] * table[tokens[i]]          (weight NULL: 1)
+ * d_table  type [n_rows][ld_table], d_tokens int32 or int64 [T] (token_bytes 4 or 8), d_out type [T][ld_out]
+ * Token -1 is padding: its row is zeros whatever its weight is.  Any other token outside [0, n_rows) gives zeros too and
+ * lowers *d_first_bad (int64, optional; the caller sets it to INT64_MAX) to its position.
+ * D <= LENS_EMBED_MAX_DIM.  d_out must not overlap the inputs.
+ */
+int lens_embed_events(const void *d_table, int type, int64_t n_rows, int64_t ld_table, const void *d_tokens, int token_bytes,
+                      const float *d_weight, float scale, int64_t T, int D, void *d_out, int64_t ld_out,
+                      int64_t *d_first_bad, void *stream);
+
+/*
+ * Tokens in ascending order:  d_keys int32 [T] the sorted tokens, d_index int32 [T] where each stood; equal tokens keep their
+ * order.  Tokens outside [0, n_rows), padding among them, get the key n_rows and stand behind the others.
+ * Scratch: lens_sort_tokens_scratch_bytes(T, n_rows).
+ */
+size_t lens_sort_tokens_scratch_bytes(int64_t T, int64_t n_rows);
+int lens_sort_tokens(const void *d_tokens, int token_bytes, int64_t T, int64_t n_rows, int32_t *d_keys, int32_t *d_index,
+                     void *d_scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * Gradients of lens_embed_events, from the sorted tokens (d_keys, d_index as lens_sort_tokens wrote them):
+ *   grad_table[v] = scale * sum_{i : tokens[i] = v} weight[i] * grad[i]          float [n_rows][D], every row written
+ *   grad_weight[i] = scale * <grad[i], table[tokens[i]]>                         float [T], optional; 0 for tokens without a row
+ * d_grad type [T][ld_grad] (ld_grad 0: one row for all events); d_table is read for grad_weight only.
+ * Sums are 32-bit, in an order that the tokens alone fix.  Scratch: lens_embed_events_grad_scratch_bytes(type, T, n_rows, D).
+ */
+size_t lens_embed_events_grad_scratch_bytes(int type, int64_t T, int64_t n_rows, int D);
+int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const int32_t *d_keys, const int32_t *d_index,
+                           const float *d_weight, float scale, int64_t T, int64_t n_rows, int D, const void *d_table,
+                           int64_t ld_table, float *d_grad_table, float *d_grad_weight, void *d_scratch, size_t scratch_bytes,
+                           void *stream);
+
+/*
+ * Gated linear recurrence:  h_t = a_t h_{t-1} + x_t   for every channel, over the rows of every sequence.
+ * The gates a_t are d_gate [T][ldg] (gate_type: x_type or LENS_F32), or, with d_gate NULL, the decays
+ * a = exp(-dt_t * rate_d) of d_dt float [T] (time since the previous event) and d_rate float [D].
+ * d_x       x_type [T][ldx]; a leading dimension of 0 (x, gate) is one row for all events
+ * d_seq_off int64 [n_seq + 1] or NULL (n_seq = 1: all rows are one sequence).  Non-decreasing, the last at most T; rows of
+ *           sequence s are [off[s], off[s+1]), none is allowed.  The kernels stay inside their buffers whatever it holds.
+ * d_h0      float [n_seq][D], the state before the first row of every sequence; NULL: zeros
+ * d_h       x_type [T][ldh], the states.  Rows of no sequence: zeros where `fill` is not 0, else left as they were.
+ * d_last    float [n_seq][D], the last state of every sequence (h0 for one without rows), in 32 bits
+ * d_marks   float [ceil(T / lens_scan_mark_rows(D))][D], optional: what lens_gated_scan_grad needs of the states
+ * d_h must not overlap the inputs.  |a| <= 1 is assumed to the extent that the product of the gates over some hundred rows
+ * must not overflow.  Scratch: lens_gated_scan_scratch_bytes(T, D, 0).
+ */
+int lens_scan_mark_rows(int D);
+size_t lens_gated_scan_scratch_bytes(int64_t T, int D, int backward);
+int lens_gated_scan(const void *d_x, int x_type, int64_t ldx, const void *d_gate, int gate_type, int64_t ldg,
+                    const float *d_dt, const float *d_rate, const int64_t *d_seq_off, int n_seq, const float *d_h0,
+                    int64_t T, int D, void *d_h, int64_t ldh, int fill, float *d_last, float *d_marks,
+                    void *d_scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * Gradients of lens_gated_scan for the gradients of its states and last states (inputs and d_marks as there):
+ *   g_t = grad_h_t + a_{t+1} g_{t+1} (behind a sequence's last row: grad_last);  grad_x = g,  grad_gate = g_t h_{t-1},
+ *   grad_rate_d = -sum_t dt_t a_t g_t h_{t-1},  grad_h0 = a g at a sequence's first row (grad_last for one without rows)
+ * The states are computed again from the marks, in 32 bits.
+ * d_grad_h x_type [T][ld_grad] or NULL (zeros; ld_grad 0: one row for all), d_grad_last float [n_seq][D] or NULL (zeros)
+ * d_grad_x x_type [T][ld_gx], d_grad_gate gate_type [T][ld_gg] (gates), d_grad_rate float [D] (decays), d_grad_h0 float
+ * [n_seq][D] or NULL.  Rows of no sequence get zeros.  Outputs must not overlap the inputs.
+ * Scratch: lens_gated_scan_scratch_bytes(T, D, 1).
+ */
+int lens_gated_scan_grad(const void *d_grad_h, int64_t ld_grad, const float *d_grad_last, const void *d_x, int x_type, int64_t ldx,
+                         const void *d_gate, int gate_type, int64_t ldg, const float *d_dt, const float *d_rate,
+                         const int64_t *d_seq_off, int n_seq, const float *d_h0, const float *d_marks, int64_t T, int D,
+                         void *d_grad_x, int64_t ld_gx, void *d_grad_gate, int64_t ld_gg, float *d_grad_rate, float *d_grad_h0,
+                         void *d_scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * One step of n carried states:  out[b] = a_b state[b] + x[b],  with x rows of their own (d_tokens NULL, d_x x_type [n][ldx]),
+ * or looked up in the same pass: x[b] = scale * weight[b] * table[tokens[b]] with d_x the table [n_rows][ldx] (tokens as for
+ * lens_embed_events).  Gates as for lens_gated_scan, one row a state.  d_state float [n][lds] and d_out float [n][ldo] may be
+ * the same memory.
+ */
+int lens_gated_step(const float *d_state, int64_t lds, const void *d_x, int x_type, int64_t ldx,
+                    const void *d_tokens, int token_bytes, int64_t n_rows, const float *d_weight, float scale,
+                    const void *d_gate, int gate_type, int64_t ldg, const float *d_dt, const float *d_rate,
+                    int n, int D, float *d_out, int64_t ldo, int64_t *d_first_bad, void *stream);
 
 #ifdef __cplusplus
 }

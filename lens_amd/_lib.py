@@ -6,12 +6,14 @@ GPU the call raises.  `build()` compiles the library in-tree with hipcc for gfx9
 import ctypes
 import os
 import subprocess
+import tempfile
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(_PKG)
 # LENS_AMD_SO selects another in-tree build of the same sources (kernel experiments); the default is the product.
 SO_PATH = os.environ.get("LENS_AMD_SO") or os.path.join(_PKG, "liblens_amd.so")
 SRC = os.path.join(_PKG, "csrc", "lens_kernels.hip")
+SOURCES = [SRC] + [os.path.join(_PKG, "csrc", n) for n in ("event_embed.hip", "event_scan.hip")]
 INCLUDES = [os.path.join(_PKG, "csrc", n)                            # textually included by SRC
             for n in ("feature_loop_n2f4.inc", "fire_loop.inc", "carry_l2_loop.inc", "output_loop_p1.inc", "output_loop_p2.inc", "output_loop_p3.inc",
                       "output_loop_p4.inc")]
@@ -28,6 +30,9 @@ HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off"
 
 _c_p = ctypes.c_void_p
 _i = ctypes.c_int
+_l = ctypes.c_int64
+_z = ctypes.c_size_t
+_f = ctypes.c_float
 
 # name -> (restype, argtypes); must list every symbol include/lens_amd.h declares
 SIGNATURES = {
@@ -59,10 +64,23 @@ SIGNATURES = {
     "lens_layer_forward_clamped": (_i, [_c_p, _i, _i, _c_p, _i, _c_p, _i, _i, _c_p, _i, _c_p]),
     "lens_train_layer": (_i, [_c_p, _i, _c_p, _c_p, _c_p, _i, _c_p, _i, _c_p, _c_p, _i, _c_p, _c_p, _c_p, _c_p,
                               _i, _i, _i, _c_p]),
+    "lens_embed_events": (_i, [_c_p, _i, _l, _l, _c_p, _i, _c_p, _f, _l, _i, _c_p, _l, _c_p, _c_p]),
+    "lens_sort_tokens_scratch_bytes": (_z, [_l, _l]),
+    "lens_sort_tokens": (_i, [_c_p, _i, _l, _l, _c_p, _c_p, _c_p, _z, _c_p]),
+    "lens_embed_events_grad_scratch_bytes": (_z, [_i, _l, _l, _i]),
+    "lens_embed_events_grad": (_i, [_c_p, _i, _l, _c_p, _c_p, _c_p, _f, _l, _l, _i, _c_p, _l, _c_p, _c_p, _c_p, _z, _c_p]),
+    "lens_scan_mark_rows": (_i, [_i]),
+    "lens_gated_scan_scratch_bytes": (_z, [_l, _i, _i]),
+    "lens_gated_scan": (_i, [_c_p, _i, _l, _c_p, _i, _l, _c_p, _c_p, _c_p, _i, _c_p, _l, _i, _c_p, _l, _i, _c_p, _c_p,
+                             _c_p, _z, _c_p]),
+    "lens_gated_scan_grad": (_i, [_c_p, _l, _c_p, _c_p, _i, _l, _c_p, _i, _l, _c_p, _c_p, _c_p, _i, _c_p, _c_p, _l, _i,
+                                  _c_p, _l, _c_p, _l, _c_p, _c_p, _c_p, _z, _c_p]),
+    "lens_gated_step": (_i, [_c_p, _l, _c_p, _i, _l, _c_p, _i, _l, _c_p, _f, _c_p, _i, _l, _c_p, _c_p, _i, _i, _c_p, _l,
+                             _c_p, _c_p]),
 }
 
 _lib = None
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 
 class LensAmdError(RuntimeError):
@@ -70,15 +88,22 @@ class LensAmdError(RuntimeError):
 
 
 def build(force=False, verbose=False):
-    """Compile lens_amd/csrc/lens_kernels.hip -> lens_amd/liblens_amd.so (gfx950)."""
-    newest = max(os.path.getmtime(f) for f in [SRC, HEADER] + INCLUDES)
+    """Compile lens_amd/csrc/*.hip -> lens_amd/liblens_amd.so (gfx950), the sources side by side."""
+    newest = max(os.path.getmtime(f) for f in SOURCES + [HEADER] + INCLUDES)
     if not force and os.path.exists(SO_PATH) and os.path.getmtime(SO_PATH) >= newest:
         return SO_PATH
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc] + HIPCC_FLAGS + ["-o", SO_PATH, SRC]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, os.path.basename(f) + ".o") for f in SOURCES]
+        cmds = [[hipcc] + HIPCC_FLAGS + ["-c", "-o", o, f] for f, o in zip(SOURCES, objects)]
+        link = [hipcc] + HIPCC_FLAGS + ["-o", SO_PATH] + objects
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds + [link]))
+        running = [(subprocess.Popen(c), c) for c in cmds]
+        for status, c in [(p.wait(), c) for p, c in running]:
+            if status:
+                raise subprocess.CalledProcessError(status, c)
+        subprocess.check_call(link)
     return SO_PATH
 
 

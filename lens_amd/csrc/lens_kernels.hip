@@ -1966,7 +1966,7 @@ const char *lens_amd_strerror(int status)
     case LENS_ERR_SIZE: return "a size or stride argument is out of range";
     case LENS_ERR_UNSUPPORTED: return "request is outside what the kernels implement";
     case LENS_ERR_ALIGN: return "a pointer or leading dimension violates the required alignment";
-    case LENS_ERR_SCRATCH: return "the batch needs more spike-stream workspace than the library's static scratch array holds";
+    case LENS_ERR_SCRATCH: return "the call needs more scratch memory than it was given, or than the library's static scratch array holds";
     default: return "";
     }
 }

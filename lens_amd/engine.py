@@ -482,3 +482,255 @@ def sad_matrix(query, reference):
     st = _lib.lib().lens_sad_matrix(_ptr(q), q.shape[0], _ptr(r), r.shape[0], q.shape[1], _ptr(out), r.shape[0], _stream())
     _lib.check(st, "lens_sad_matrix")
     return out
+
+
+# --------------------------------------------------------------------------------------------
+# event streams, event by event: token lookup, gated recurrence, their gradients
+# --------------------------------------------------------------------------------------------
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # LENS_F32, LENS_BF16, LENS_F16
+
+
+def _call(name, t, *args):
+    """One entry point on the current stream of t's device (which need not be the current one)."""
+    fn = getattr(_lib.lib(), name)
+    if t.device.index == torch.cuda.current_device():
+        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(t.device):
+            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if st:
+        _lib.check(st, name)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t, name, n, D, dtype, device, spread=False):
+    """The leading dimension of a [n, D] operand, checked; spread: rows may be one row, expanded."""
+    assert t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}"
+    assert t.dim() == 2 and t.shape[0] == n and t.shape[1] == D, f"{name} must be [{n}, {D}], got {list(t.shape)}"
+    assert t.device == device, f"{name} is on {t.device}, expected {device}"
+    ld, last = t.stride()
+    assert last == 1 or D <= 1, f"{name}: the last index must be contiguous"
+    if n <= 1:
+        return D
+    assert ld >= D or (spread and ld == 0), f"{name}: rows overlap (stride {ld}, {D} channels)"
+    return ld
+
+
+def _flat(t, name, n, dtype, device):
+    assert t.dtype == dtype and t.is_contiguous() and t.numel() == n, f"{name} must be {n} contiguous {dtype}, got {list(t.shape)} {t.dtype}"
+    assert t.device == device, f"{name} is on {t.device}, expected {device}"
+    return t.data_ptr()
+
+
+def _tokens(tokens, device=None):
+    _need_cuda(tokens, "tokens")
+    assert tokens.dtype in (torch.int32, torch.int64) and tokens.dim() == 1 and tokens.is_contiguous(), \
+        "tokens must be a contiguous int32 or int64 vector"
+    assert device is None or tokens.device == device, f"tokens are on {tokens.device}, expected {device}"
+    return tokens.element_size()
+
+
+def _raise_bad(first_bad, tokens, n_rows):
+    b = int(first_bad.item())
+    if b != INT64_MAX:
+        raise IndexError(f"event {b}: token {int(tokens[b])} is outside [0, {n_rows}) and not the padding -1")
+
+
+def embed_events(table, tokens, weight=None, scale=1.0, out=None, check=True):
+    """Rows of a table for a list of events: out[i] = scale * weight[i] * table[tokens[i]], [T, D] in the table's type.
+
+    table float32 / bfloat16 / float16 [n_rows, D] (rows may be strided), tokens int32 / int64 [T], weight float32 [T] or None.
+    Token -1 is padding and gives a row of zeros.  Any other token outside the table raises IndexError (check=True, which
+    synchronises); with check=False it gives a row of zeros too.  `out` must not overlap the inputs."""
+    _need_cuda(table, "table")
+    dev = table.device
+    size = _tokens(tokens, dev)
+    assert table.dtype in _TYPES, f"table must be float32, bfloat16 or float16, got {table.dtype}"
+    V, D = table.shape
+    T = tokens.shape[0]
+    ld = _rows(table, "table", V, D, table.dtype, dev)
+    w = None if weight is None else _flat(weight, "weight", T, torch.float32, dev)
+    if out is None:
+        out = torch.empty((T, D), dtype=table.dtype, device=dev)
+    ldo = _rows(out, "out", T, D, table.dtype, dev)
+    bad = torch.full((1,), INT64_MAX, dtype=torch.int64, device=dev) if check else None
+    _call("lens_embed_events", table, table.data_ptr(), _TYPES[table.dtype], V, ld, tokens.data_ptr(), size, w, scale, T, D,
+          out.data_ptr(), ldo, _addr(bad))
+    if check:
+        _raise_bad(bad, tokens, V)
+    return out
+
+
+def sort_events(tokens, n_rows):
+    """The tokens in ascending order (int32 [T]; equal ones keep their order) and where each stood (int32 [T]).  Tokens outside
+    [0, n_rows), padding among them, come last as n_rows."""
+    size = _tokens(tokens)
+    T = tokens.shape[0]
+    keys = torch.empty((T,), dtype=torch.int32, device=tokens.device)
+    index = torch.empty((T,), dtype=torch.int32, device=tokens.device)
+    need = _lib.lib().lens_sort_tokens_scratch_bytes(T, n_rows)
+    scratch = torch.empty((need,), dtype=torch.uint8, device=tokens.device)
+    _call("lens_sort_tokens", tokens, tokens.data_ptr(), size, T, n_rows, keys.data_ptr(), index.data_ptr(), scratch.data_ptr(), need)
+    return keys, index
+
+
+def embed_events_grad(grad, tokens, n_rows, weight=None, scale=1.0, table=None, order=None):
+    """Gradients of embed_events for the gradient `grad` [T, D] of its rows: (grad_table float32 [n_rows, D], every row
+    written, and grad_weight float32 [T] where weight is given -- the table is needed for it -- else None).
+
+    Sums are 32-bit and their order is fixed by the tokens: the same call gives the same bits.  order: what
+    sort_events(tokens, n_rows) returned, for a program that passes over the same events again."""
+    _need_cuda(grad, "grad")
+    dev = grad.device
+    size = _tokens(tokens, dev)
+    assert grad.dtype in _TYPES and grad.dim() == 2, f"grad must be [T, D] in float32, bfloat16 or float16, got {list(grad.shape)} {grad.dtype}"
+    T, D = grad.shape
+    assert tokens.shape[0] == T, f"{tokens.shape[0]} tokens, {T} rows of gradient"
+    ld = _rows(grad, "grad", T, D, grad.dtype, dev, spread=True)
+    w = gw = ldt = None
+    if weight is not None:
+        assert table is not None, "the gradient of the weights needs the table"
+        w = _flat(weight, "weight", T, torch.float32, dev)
+        ldt = _rows(table, "table", n_rows, D, grad.dtype, dev)
+        gw = torch.empty((T,), dtype=torch.float32, device=dev)
+    gt = torch.empty((n_rows, D), dtype=torch.float32, device=dev)
+    keys, index = sort_events(tokens, n_rows) if order is None else order
+    k, i = _flat(keys, "order[0]", T, torch.int32, dev), _flat(index, "order[1]", T, torch.int32, dev)
+    need = _lib.lib().lens_embed_events_grad_scratch_bytes(_TYPES[grad.dtype], T, n_rows, D)
+    scratch = torch.empty((need,), dtype=torch.uint8, device=dev)
+    _call("lens_embed_events_grad", grad, grad.data_ptr(), _TYPES[grad.dtype], ld, k, i, w, scale, T, n_rows, D,
+          _addr(table) if gw is not None else None, ldt or 0, gt.data_ptr(), _addr(gw), scratch.data_ptr(), need)
+    return gt, gw
+
+
+def _decay(gate, dt, rate, n, D, x_dtype, dev):
+    """(gate pointer, type, leading dimension, dt pointer, rate pointer) of a call's gates."""
+    if gate is not None:
+        assert dt is None and rate is None, "gates are either `gate` or `dt` and `rate`"
+        assert gate.dtype in (x_dtype, torch.float32), f"gate must be {x_dtype} or float32, got {gate.dtype}"
+        return gate.data_ptr(), _TYPES[gate.dtype], _rows(gate, "gate", n, D, gate.dtype, dev, spread=True), None, None
+    assert dt is not None and rate is not None, "gates are either `gate` or `dt` and `rate`"
+    return None, 0, 0, _flat(dt, "dt", n, torch.float32, dev), _flat(rate, "rate", D, torch.float32, dev)
+
+
+def _sequences(seq_off, T, dev):
+    """seq_off as the kernels take it, and the number of sequences.  Offsets in host memory are checked."""
+    if seq_off is None:
+        return None, 1
+    if not (torch.is_tensor(seq_off) and seq_off.is_cuda):
+        off = np.asarray(seq_off, dtype=np.int64).reshape(-1)
+        if off.size < 2 or off[0] < 0 or off[-1] > T or np.any(np.diff(off) < 0):
+            raise ValueError(f"seq_off must hold at least two non-decreasing offsets within [0, {T}]")
+        seq_off = torch.from_numpy(np.ascontiguousarray(off)).to(dev)
+    assert seq_off.dtype == torch.int64 and seq_off.dim() == 1 and seq_off.is_contiguous() and seq_off.numel() >= 2, \
+        "seq_off must be a contiguous int64 vector of at least two offsets"
+    assert seq_off.device == dev, f"seq_off is on {seq_off.device}, expected {dev}"
+    return seq_off, seq_off.numel() - 1
+
+
+def _scan_marks(T, D):
+    return (T + _lib.lib().lens_scan_mark_rows(D) - 1) // _lib.lib().lens_scan_mark_rows(D)
+
+
+def gated_scan(x, gate=None, dt=None, rate=None, seq_off=None, h0=None, out=None, marks=False):
+    """States after every event: h_t = a_t h_{t-1} + x_t for every channel, sequence by sequence.
+
+    x       [T, D] float32 / bfloat16 / float16, the rows of all sequences one behind the other
+    gate    [T, D] the a_t (x's type or float32), or dt float32 [T] and rate float32 [D]: a_t = exp(-dt_t rate_d), dt the time
+            since the previous event
+    seq_off int64 [S + 1]: rows of sequence s are [seq_off[s], seq_off[s + 1]), possibly none; None: one sequence.  On the device
+            it is trusted (non-decreasing, the last at most T); in host memory it is checked, and copied.
+    h0      float32 [S, D], the state before every sequence's first row; None: zeros
+    Returns (h [T, D] in x's type, last float32 [S, D]), with marks=True also what gated_scan_grad needs of the states.
+    Rows of no sequence are zeros in h; in the caller's `out` (which must not overlap the inputs) they are left as they were.
+    x and gate may be one row expanded to T."""
+    _need_cuda(x, "x")
+    dev = x.device
+    assert x.dim() == 2 and x.dtype in _TYPES, f"x must be [T, D] in float32, bfloat16 or float16, got {list(x.shape)} {x.dtype}"
+    T, D = x.shape
+    ldx = _rows(x, "x", T, D, x.dtype, dev, spread=True)
+    g, gtype, ldg, pdt, prate = _decay(gate, dt, rate, T, D, x.dtype, dev)
+    off, S = _sequences(seq_off, T, dev)
+    p0 = None if h0 is None else _flat(h0, "h0", S * D, torch.float32, dev)
+    fill = out is None
+    if out is None:
+        out = torch.empty((T, D), dtype=x.dtype, device=dev)
+    ldh = _rows(out, "out", T, D, x.dtype, dev)
+    last = torch.empty((S, D), dtype=torch.float32, device=dev)
+    kept = torch.empty((_scan_marks(T, D), D), dtype=torch.float32, device=dev) if marks else None
+    need = _lib.lib().lens_gated_scan_scratch_bytes(T, D, 0)
+    scratch = torch.empty((need,), dtype=torch.uint8, device=dev)
+    _call("lens_gated_scan", x, x.data_ptr(), _TYPES[x.dtype], ldx, g, gtype, ldg, pdt, prate, _addr(off), S, p0, T, D,
+          out.data_ptr(), ldh, int(fill), last.data_ptr(), _addr(kept), scratch.data_ptr(), need)
+    return (out, last, kept) if marks else (out, last)
+
+
+def gated_scan_grad(grad_h, x, marks, gate=None, dt=None, rate=None, seq_off=None, h0=None, grad_last=None):
+    """Gradients of gated_scan for the gradients `grad_h` [T, D] of its states (x's type; None: zeros) and `grad_last` float32
+    [S, D] of its last states (None: zeros); everything else as it was given there, `marks` as it returned them.
+
+    Returns (grad_x [T, D] in x's type, grad_gate [T, D] in the gate's type or grad_rate float32 [D], grad_h0 float32 [S, D] or
+    None where h0 is).  Rows of no sequence get zeros.  There is no gradient for dt, which is recorded."""
+    _need_cuda(x, "x")
+    dev = x.device
+    assert x.dim() == 2 and x.dtype in _TYPES, f"x must be [T, D] in float32, bfloat16 or float16, got {list(x.shape)} {x.dtype}"
+    T, D = x.shape
+    ldx = _rows(x, "x", T, D, x.dtype, dev, spread=True)
+    ldd = 0 if grad_h is None else _rows(grad_h, "grad_h", T, D, x.dtype, dev, spread=True)
+    g, gtype, ldg, pdt, prate = _decay(gate, dt, rate, T, D, x.dtype, dev)
+    off, S = _sequences(seq_off, T, dev)
+    p0 = None if h0 is None else _flat(h0, "h0", S * D, torch.float32, dev)
+    pl = None if grad_last is None else _flat(grad_last, "grad_last", S * D, torch.float32, dev)
+    pm = _flat(marks, "marks", _scan_marks(T, D) * D, torch.float32, dev)
+    gx = torch.empty((T, D), dtype=x.dtype, device=dev)
+    ga = torch.empty((T, D), dtype=gate.dtype, device=dev) if gate is not None else None
+    gr = torch.empty((D,), dtype=torch.float32, device=dev) if gate is None else None
+    g0 = None if h0 is None else torch.empty((S, D), dtype=torch.float32, device=dev)
+    need = _lib.lib().lens_gated_scan_scratch_bytes(T, D, 1)
+    scratch = torch.empty((need,), dtype=torch.uint8, device=dev)
+    _call("lens_gated_scan_grad", x, _addr(grad_h), ldd, pl, x.data_ptr(), _TYPES[x.dtype], ldx, g, gtype, ldg, pdt, prate,
+          _addr(off), S, p0, pm, T, D, gx.data_ptr(), D, _addr(ga), D, _addr(gr), _addr(g0), scratch.data_ptr(), need)
+    return gx, ga if gate is not None else gr, g0
+
+
+def _step(state, x, tokens, weight, scale, gate, dt, rate, out, first_bad):
+    _need_cuda(state, "state")
+    dev = state.device
+    assert state.dim() == 2, f"state must be [n, D], got {list(state.shape)}"
+    n, D = state.shape
+    ld = _rows(state, "state", n, D, torch.float32, dev, spread=out is not None)
+    assert x.dtype in _TYPES, f"rows must be float32, bfloat16 or float16, got {x.dtype}"
+    if tokens is None:
+        size, n_rows, w = 0, 0, None
+        ldx = _rows(x, "x", n, D, x.dtype, dev, spread=True)
+    else:
+        size, n_rows = _tokens(tokens, dev), x.shape[0]
+        assert tokens.shape[0] == n, f"{tokens.shape[0]} tokens, {n} states"
+        ldx = _rows(x, "table", n_rows, D, x.dtype, dev)
+        w = None if weight is None else _flat(weight, "weight", n, torch.float32, dev)
+    g, gtype, ldg, pdt, prate = _decay(gate, dt, rate, n, D, x.dtype, dev)
+    out = state if out is None else out
+    ldo = _rows(out, "out", n, D, torch.float32, dev)
+    _call("lens_gated_step", state, state.data_ptr(), ld, x.data_ptr(), _TYPES[x.dtype], ldx, _addr(tokens), size, n_rows, w, scale,
+          g, gtype, ldg, pdt, prate, n, D, out.data_ptr(), ldo, _addr(first_bad))
+    return out
+
+
+def gated_step(state, x, gate=None, dt=None, rate=None, out=None):
+    """One step of n carried states (float32 [n, D]): a * state + x, gates and x as in gated_scan with one row a state.
+    Written over `state`, or into `out` (float32 [n, D]).  Returns what was written."""
+    return _step(state, x, None, None, 1.0, gate, dt, rate, out, None)
+
+
+def event_step(state, table, tokens, weight=None, scale=1.0, gate=None, dt=None, rate=None, out=None, check=False):
+    """One event for each of n carried states, looked up and integrated in one pass: a * state + scale * weight * table[token].
+    Arguments as in embed_events and gated_step.  A token -1 only decays its state.  check=True synchronises and raises IndexError
+    for any other token outside the table (its state has then decayed without it)."""
+    bad = torch.full((1,), INT64_MAX, dtype=torch.int64, device=state.device) if check else None
+    out = _step(state, table, tokens, weight, scale, gate, dt, rate, out, bad)
+    if check:
+        _raise_bad(bad, tokens, table.shape[0])
+    return out

@@ -11,5 +11,5 @@ rm -rf $W; mkdir -p $W/lens_amd/csrc $W/include $ROOT/variants
 cp $ROOT/lens_amd/csrc/* $W/lens_amd/csrc/; cp $ROOT/include/*.h $W/include/
 env "$@" python3 $ROOT/scripts/gen_output_loop.py $W/lens_amd/csrc > /dev/null
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fno-slp-vectorize -Xclang -target-feature -Xclang -packed-fp32-ops \
-  -fPIC -shared -w $EXTRA_HIPCC -o $ROOT/variants/$NAME.so $W/lens_amd/csrc/lens_kernels.hip
+  -fPIC -shared -w $EXTRA_HIPCC -o $ROOT/variants/$NAME.so $W/lens_amd/csrc/*.hip
 ls -la $ROOT/variants/$NAME.so

@@ -1,0 +1,141 @@
+"""The event-stream operators in 64 bits, row by row (numpy), with bounds of what 32-bit arithmetic may lose.
+
+u = 2^-24 is half a step of float32 relative to the value; half_step(t) that of an output type.
+
+Lookup: scale * w and its product with the element round once each, the output once.
+Table gradient: a sum of n terms, each fma rounding once, in any order and grouping: (n + 3) u times the sum of magnitudes.
+Scan: with S_t = |a_t| S_{t-1} + |x_t| every |h_t| <= S_t.  A step rounds its product and its sum, and a run of rows that is
+joined to another rounds the factor and the sum of its pair once a row: 8 u S_t covers these.  A decay a = exp(z), z = -dt rate:
+z is rounded (u |z|, relative in a), so is its product with log2 e (u |z|); the exponential is good to 2 u, the series below 1/16 to
+5 u of 1/16.  A run's z is a sum of at most 16 terms: 15 u more of it, shared out over its rows.  So (8 + 20 |z_t|) u S_t.
+Results below the normal numbers are rounded to a multiple of 2^-149, not relative to themselves: up to 2^-150 for each of a
+row's four roundings; and an exponential below 2^-126 is zero, which is 2^-126 of what it multiplies.
+An error made at a row decays as the state does: E_t = |a_t| E_{t-1} + (8 + 20 |z_t|) u S_t + 4 2^-150 + 2^-126 S_{t-1}.
+"""
+import numpy as np
+import torch
+
+U = 2.0 ** -24
+TINY, FLUSHED = 2.0 ** -150, 2.0 ** -126
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def least(dtype):
+    """Half of the smallest number of a type: what a result near zero may be off."""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
+def f64(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def embed(table, tokens, weight, scale):
+    tab, tok = f64(table), tokens.cpu().numpy()
+    s = float(np.float32(scale))
+    w = np.ones(len(tok)) if weight is None else f64(weight)
+    ok = (tok >= 0) & (tok < len(tab))
+    out = np.zeros((len(tok), table.shape[1]))
+    out[ok] = s * w[ok, None] * tab[tok[ok]]
+    return out
+
+
+def embed_grad(grad, tokens, n_rows, weight, scale, table):
+    """(grad_table, its bound, grad_weight, its bound)."""
+    g, tok = f64(grad), tokens.cpu().numpy()
+    s = float(np.float32(scale))
+    w = np.ones(len(tok)) if weight is None else f64(weight)
+    gt, mag, n = np.zeros((n_rows, g.shape[1])), np.zeros((n_rows, g.shape[1])), np.zeros((n_rows, 1))
+    gw, gwm = np.zeros(len(tok)), np.zeros(len(tok))
+    tab = f64(table)
+    for i, k in enumerate(tok):
+        if 0 <= k < n_rows:
+            gt[k] += s * w[i] * g[i]
+            mag[k] += np.abs(s * w[i] * g[i])
+            n[k] += 1
+            if tab is not None:
+                gw[i], gwm[i] = s * (g[i] @ tab[k]), abs(s) * (np.abs(g[i]) @ np.abs(tab[k]))
+    return gt, (n + 3) * U * mag, gw, (g.shape[1] + 3) * U * gwm
+
+
+def gates(gate, dt, rate):
+    return f64(gate) if gate is not None else np.exp(-f64(dt)[:, None] * f64(rate)[None, :])
+
+
+def step_loss(a):
+    """(8 + 20 |z|) u of every row and channel (gates have no z: that of |a| stands above it)."""
+    with np.errstate(divide="ignore"):
+        z = np.where(a > 0, np.minimum(np.abs(np.log(np.maximum(a, 1e-300))), 700), 0)
+    return (8 + 20 * z) * U
+
+
+def scan(x, a, off, h0):
+    """states [T, D] (zero in rows of no sequence), last [S, D], the states before every row, and the bounds of the states."""
+    x = f64(x)
+    T, D = x.shape
+    off = [0, T] if off is None else [int(v) for v in off]
+    S = len(off) - 1
+    h0 = np.zeros((S, D)) if h0 is None else f64(h0)
+    h, before, E, Eb = np.zeros((T, D)), np.zeros((T, D)), np.zeros((T, D)), np.zeros((T, D))
+    last, El = h0.copy(), np.zeros((S, D))
+    c = step_loss(a)
+    for s in range(S):
+        v, m, e = h0[s].copy(), np.abs(h0[s]), np.zeros(D)
+        for t in range(off[s], off[s + 1]):
+            before[t], Eb[t] = v, e
+            v = a[t] * v + x[t]
+            e = np.abs(a[t]) * e + 4 * TINY + FLUSHED * m
+            m = np.abs(a[t]) * m + np.abs(x[t])
+            e = e + c[t] * m
+            h[t], E[t] = v, e
+        if off[s] < off[s + 1]:
+            last[s], El[s] = v, e
+    return h, last, before, E, El, Eb
+
+
+def scan_grad(grad_h, grad_last, x, a, dt, off, h0):
+    """grad_x, grad_gate (or grad_rate), grad_h0 and their bounds."""
+    T, D = x.shape
+    h, last, before, E, El, Eb = scan(x, a, off, h0)
+    off = [0, T] if off is None else [int(v) for v in off]
+    S = len(off) - 1
+    d = np.zeros((T, D)) if grad_h is None else f64(grad_h)
+    gl = np.zeros((S, D)) if grad_last is None else f64(grad_last)
+    g, ga, Eg, Ea, r_all, Er_all = (np.zeros((T, D)) for _ in range(6))
+    g0, E0 = gl.copy(), np.zeros((S, D))
+    c = step_loss(a)
+    for s in range(S):
+        r, m, e = gl[s].copy(), np.abs(gl[s]), np.zeros(D)
+        for t in range(off[s + 1] - 1, off[s] - 1, -1):
+            g[t] = d[t] + r
+            m = m + np.abs(d[t])
+            Eg[t] = e + 2 * U * m
+            ga[t] = g[t] * before[t]
+            Ea[t] = Eg[t] * np.abs(before[t]) + Eb[t] * np.abs(g[t]) + Eg[t] * Eb[t] + U * np.abs(ga[t])
+            r = a[t] * g[t]
+            e = np.abs(a[t]) * Eg[t] + 4 * TINY + FLUSHED * m
+            m = np.abs(a[t]) * m
+            e = e + c[t] * m
+            r_all[t], Er_all[t] = r, e
+        if off[s] < off[s + 1]:
+            g0[s], E0[s] = r, e
+    if dt is None:
+        return g, ga, g0, Eg, Ea, E0
+    dt = f64(dt)[:, None]
+    terms = -dt * r_all * before
+    bound = (dt * (Er_all * np.abs(before) + Eb * np.abs(r_all) + Er_all * Eb)).sum(0) + (T + 4) * U * np.abs(terms).sum(0)
+    return g, terms.sum(0), g0, Eg, bound, E0
+
+
+def check(got, want, bound, name=""):
+    """|got - want| <= bound + the rounding of got's type, everywhere."""
+    t = got.dtype
+    got = f64(got)
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    with np.errstate(invalid="ignore"):
+        room = bound + half_step(t) * (np.abs(want) + bound) + least(t)
+        off = np.abs(got - want) - room
+    bad = ~(off <= 0)
+    assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.size} off, first at {np.argwhere(bad)[0].tolist()}: got {got[bad][0]!r}, want {want[bad][0]!r}, room {np.broadcast_to(room, bad.shape)[bad][0]!r}"

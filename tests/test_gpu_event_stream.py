@@ -1,0 +1,454 @@
+"""The event-stream operators (token lookup, gated recurrence, their gradients, single steps) on the GPU against the same in
+64 bits, row by row; the bounds are derived in event_stream_ref."""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+import event_stream_ref as R
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def E():
+    from lens_amd import engine
+    return engine
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rnd(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def decays(kind, T, D, dtype, g):
+    """gate / dt / rate of a call: short and long memories, exact ones and zeros among the gates."""
+    if kind == "time":
+        return dict(dt=torch.rand(T, generator=g, device="cuda") ** 3 * 2, rate=torch.exp(rnd(g, D) * 2 - 2))
+    a = torch.sigmoid(rnd(g, T, D) * 2 + 2)
+    u = torch.rand(T, D, generator=g, device="cuda")
+    a = torch.where(u < 0.05, torch.zeros_like(a), torch.where(u > 0.95, torch.ones_like(a), a))
+    a = torch.where((u > 0.5) & (u < 0.55), -a, a)
+    return dict(gate=a.to(torch.float32 if kind == "gate32" else dtype))
+
+
+# ---------------------------------------------------------------------------------------------------------- lookup
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(1, 1, 1), (3, 5, 2), (7, 4, 3), (17, 9, 7), (33, 20, 8), (64, 50, 63), (129, 1000, 100), (500, 300, 200),
+                                   (70, 40, 257), (40, 30, 2048), (4099, 179920, 16)])
+def test_lookup(dtype, T, V, D):
+    g = gen(T + D)
+    table, w = rnd(g, V, D, dtype=dtype), rnd(g, T)
+    tok = torch.randint(-1, V, (T,), generator=g, device="cuda")
+    for tokens, weight in ((tok, w), (tok.int(), None)):
+        out = E().embed_events(table, tokens, weight=weight, scale=0.3)
+        want = R.embed(table, tokens, weight, 0.3)
+        R.check(out, want, 3 * R.U * np.abs(want))
+        assert not f64_any(out[tokens == -1])
+
+
+def f64_any(t):
+    return bool((t != 0).any()) or bool(torch.isnan(t).any())
+
+
+def test_lookup_strides_and_out():
+    g = gen(1)
+    wide = rnd(g, 40, 70, dtype=torch.bfloat16)
+    table = wide[:, 3:66]                                              # rows 70 elements apart, at an odd offset
+    tok = torch.randint(0, 40, (55,), generator=g, device="cuda")
+    buf = torch.full((57, 80), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = E().embed_events(table, tok, out=buf[1:56, 5:68])
+    R.check(out, R.embed(table, tok, None, 1.0), 0)
+    buf[1:56, 5:68] = 7.0
+    assert bool((buf == 7.0).all())                                    # nothing beside it was written
+
+
+def test_lookup_tokens_that_name_no_row():
+    g = gen(2)
+    table = rnd(g, 10, 8)
+    table[0] = float("nan")                                            # padding must not read row 0
+    tok = torch.tensor([3, -1, 9, 10, -2, 2**40], device="cuda")
+    w = torch.tensor([1.0, float("inf"), 2.0, 1.0, 1.0, float("nan")], device="cuda")
+    with pytest.raises(IndexError, match="event 3: token 10"):
+        E().embed_events(table, tok, weight=w)
+    out = E().embed_events(table, tok, weight=w, check=False)
+    R.check(out, R.embed(table, tok, w, 1.0), 3 * R.U * np.abs(R.embed(table, tok, w, 1.0)))
+    assert not f64_any(out[[1, 3, 4, 5]])
+    with pytest.raises(IndexError, match="event 1"):
+        E().embed_events(table, torch.tensor([-1, -7], device="cuda", dtype=torch.int32))
+    assert E().embed_events(table, tok[:0]).shape == (0, 8)
+    empty = E().embed_events(table[:0], torch.tensor([-1, -1], device="cuda"))
+    assert empty.shape == (2, 8) and not f64_any(empty)
+
+
+# ---------------------------------------------------------------------------------------------- sort, table gradient
+@pytest.mark.parametrize("T,V", [(1, 1), (2, 3), (63, 511), (64, 512), (65, 513), (4095, 12800), (4096, 100), (4097, 179920), (20000, 7),
+                                 (100003, 262144), (300, 2**31 - 700)])
+def test_sort_is_stable(T, V):
+    g = gen(T)
+    tok = torch.randint(-2, V + 1, (T,), generator=g, device="cuda", dtype=torch.int64)
+    for tokens in (tok, tok.to(torch.int32)):
+        keys, index = E().sort_events(tokens, V)
+        k = torch.where((tokens >= 0) & (tokens < V), tokens.long(), V)
+        want, at = torch.sort(k, stable=True)
+        assert torch.equal(keys.long(), want) and torch.equal(index.long(), at)
+
+
+def skewed(T, V, g, dev="cuda"):
+    """A tenth of the events at one row, a stretch of rows without any, padding and tokens outside."""
+    tok = torch.randint(0, V, (T,), generator=g, device=dev)
+    u = torch.rand(T, generator=g, device=dev)
+    tok = torch.where(u < 0.1, torch.full_like(tok, V // 2), tok)
+    tok = torch.where((tok > V // 4) & (tok < V // 3), torch.zeros_like(tok), tok)
+    tok = torch.where((u > 0.4) & (u < 0.45), torch.full_like(tok, -1), tok)
+    return torch.where((u > 0.5) & (u < 0.51), torch.full_like(tok, V + 3), tok)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(1, 1, 1), (1, 700, 4), (2, 3, 2), (9, 4, 3), (17, 9, 7), (60, 5, 8), (64, 64, 63), (500, 30, 9), (1300, 50, 100),
+                                   (3000, 200, 33), (2000, 3, 130), (400, 5000, 200), (700, 60, 257), (130, 20, 600), (90, 8, 1100), (70, 12, 2048)])
+def test_table_gradient(dtype, T, V, D):
+    g = gen(T + V + D)
+    grad, table, w = rnd(g, T, D, dtype=dtype), rnd(g, V, D, dtype=dtype), rnd(g, T)
+    tok = skewed(T, V, g)
+    for weight in (w, None):
+        gt, gw = E().embed_events_grad(grad, tok, V, weight=weight, scale=0.3, table=table)
+        want, bound, want_w, bound_w = R.embed_grad(grad, tok, V, weight, 0.3, table)
+        R.check(gt, want, bound, "table")
+        if weight is None:
+            assert gw is None
+        else:
+            R.check(gw, want_w, bound_w, "weight")
+        again = E().embed_events_grad(grad, tok, V, weight=weight, scale=0.3, table=table, order=E().sort_events(tok, V))
+        assert torch.equal(gt, again[0]) and (gw is None or torch.equal(gw, again[1]))
+
+
+@pytest.mark.parametrize("D", [16, 128, 300])
+def test_table_gradient_of_one_row_and_of_none(D):
+    """Every event at one row (joined over many workgroups), at the first, the last; and no event at all."""
+    g = gen(D)
+    T, V = 40000, 6
+    grad = torch.randint(-8, 9, (T, D), generator=g, device="cuda").to(torch.bfloat16)      # sums of integers are exact
+    want = grad.double().sum(0)
+    for row in (0, 3, V - 1):
+        gt, _ = E().embed_events_grad(grad, torch.full((T,), row, device="cuda"), V)
+        assert torch.equal(gt[row].double(), want)
+        gt[row] = 0
+        assert not f64_any(gt)
+    gt, _ = E().embed_events_grad(grad, torch.full((T,), -1, device="cuda"), V)
+    assert not f64_any(gt)
+    gt, _ = E().embed_events_grad(grad[:0], torch.zeros((0,), device="cuda", dtype=torch.int32), 1000)
+    assert gt.shape == (1000, D) and not f64_any(gt)
+
+
+def test_table_gradient_strides_nan_padding_and_one_gradient_for_all():
+    g = gen(5)
+    T, V, D = 300, 40, 63
+    tok = skewed(T, V, g)
+    wide = rnd(g, T, 70)
+    grad = wide[:, 3:66]
+    grad[(tok < 0) | (tok >= V)] = float("nan")                          # rows of padding count for nothing
+    table = rnd(g, V, 64)[:, :63]
+    w = rnd(g, T)
+    gt, gw = E().embed_events_grad(grad, tok, V, weight=w, table=table)
+    want, bound, want_w, bound_w = R.embed_grad(grad, tok, V, w, 1.0, table)
+    R.check(gt, want, bound)
+    R.check(gw, want_w, bound_w)
+    one = rnd(g, 1, D).expand(T, D)
+    gt, _ = E().embed_events_grad(one, tok, V)
+    R.check(gt, *R.embed_grad(one, tok, V, None, 1.0, None)[:2])
+    grad[5] = float("inf")
+    gt, _ = E().embed_events_grad(grad, torch.arange(T, device="cuda") % V, V)
+    assert bool(torch.isinf(gt[5]).any() | torch.isnan(gt[5]).any())
+
+
+# ------------------------------------------------------------------------------------------------------------- scan
+OFFSETS = [None, [0, 1], [0, 0, 5, 5, 5, 16, 17, 33, 33], [2, 7, 30, 31, 64, 64, 190], [0, 0, 0], [5, 5]]
+
+
+def run_scan(x, d, off, h0, grad_h, grad_last):
+    seq = None if off is None else torch.tensor(off, device="cuda")
+    h, last, marks = E().gated_scan(x, seq_off=seq, h0=h0, marks=True, **d)
+    back = E().gated_scan_grad(grad_h, x, marks, seq_off=seq, h0=h0, grad_last=grad_last, **d)
+    a = R.gates(d.get("gate"), d.get("dt"), d.get("rate"))
+    want = R.scan(x, a, off, h0)
+    R.check(h, want[0], want[3], "h")
+    R.check(last, want[1], want[4], "last")
+    g, da, g0, Eg, Ea, E0 = R.scan_grad(grad_h, grad_last, x, a, d.get("dt"), off, h0)
+    R.check(back[0], g, Eg, "grad_x")
+    R.check(back[1], da, Ea, "grad_gate or grad_rate")
+    if h0 is None:
+        assert back[2] is None
+    else:
+        R.check(back[2], g0, E0, "grad_h0")
+    return (h, last, *back)
+
+
+@pytest.mark.parametrize("kind", ["time", "gate", "gate32"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [1, 2, 3, 4, 5, 63, 64, 200, 259])
+def test_scan_lengths(dtype, kind, D):
+    for T in (0, 1, 2, 15, 16, 17, 79, 128, 257, 700):
+        g = gen(1000 * D + T)
+        x, d = rnd(g, T, D, dtype=dtype), decays(kind, T, D, dtype, g)
+        run_scan(x, d, None, rnd(g, 1, D), rnd(g, T, D, dtype=dtype), rnd(g, 1, D))
+
+
+@pytest.mark.parametrize("kind", ["time", "gate"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("off", OFFSETS[1:])
+def test_scan_sequences(dtype, kind, off):
+    for D, T, given in ((4, 200, True), (63, 200, False), (100, 401, True)):
+        g = gen(D + len(off))
+        x, d = rnd(g, T, D, dtype=dtype), decays(kind, T, D, dtype, g)
+        S = len(off) - 1
+        run_scan(x, d, off, rnd(g, S, D) if given else None, rnd(g, T, D, dtype=dtype), rnd(g, S, D) if given else None)
+
+
+def test_scan_many_sequences_of_every_length():
+    g = gen(9)
+    n = list(range(0, 40)) + [0, 0, 1, 300, 0, 129, 1, 1, 1, 64, 128, 256, 0]
+    off = [0] + list(itertools.accumulate(n))
+    T, D, S = off[-1] + 5, 70, len(n)
+    x, d = rnd(g, T, D), decays("time", T, D, torch.float32, g)
+    run_scan(x, d, off, rnd(g, S, D), rnd(g, T, D), rnd(g, S, D))
+
+
+def test_scan_without_gradient_of_states_and_expanded_rows():
+    g = gen(10)
+    T, D = 300, 96
+    x, gate = rnd(g, 1, D).expand(T, D), torch.sigmoid(rnd(g, 1, D) + 2).expand(T, D)
+    run_scan(x, dict(gate=gate), [0, 100, 300], None, None, rnd(g, 2, D))
+    run_scan(x, dict(gate=gate), None, None, rnd(g, 1, D).expand(T, D), None)
+    run_scan(x, dict(gate=gate), None, rnd(g, 1, D), None, None)
+
+
+def test_scan_strides_and_rows_of_no_sequence():
+    g = gen(11)
+    T, D = 150, 63
+    x = rnd(g, T, 70, dtype=torch.bfloat16)[:, 5:68]
+    gate = torch.sigmoid(rnd(g, T, 64))[:, :63].to(torch.bfloat16)
+    grad = rnd(g, T, 80, dtype=torch.bfloat16)[:, 9:72]
+    off = torch.tensor([3, 60, 60, 120], device="cuda")
+    run_scan(x, dict(gate=gate), off.tolist(), None, grad, None)
+    buf = torch.full((T, 99), 7.0, device="cuda", dtype=torch.bfloat16)
+    h, _ = E().gated_scan(x, gate=gate, seq_off=off, out=buf[:, 17:80])
+    fresh, _ = E().gated_scan(x, gate=gate, seq_off=off)
+    assert torch.equal(h[3:120], fresh[3:120]) and not f64_any(fresh[:3]) and not f64_any(fresh[120:])
+    buf[3:120, 17:80] = 7.0
+    assert bool((buf == 7.0).all())                                    # the caller's rows of no sequence, and what lies beside
+
+
+@pytest.mark.parametrize("kind", ["time", "gate"])
+def test_scan_keeps_infinities_in_their_sequence(kind):
+    """A sequence full of NaN and infinities (and rows of none) leaves every other one as it is without them."""
+    g = gen(12)
+    T, D = 700, 64
+    off = [0, 100, 101, 400, 401, 650]
+    x, d = rnd(g, T, D), decays(kind, T, D, torch.float32, g)
+    grad, gl, h0 = rnd(g, T, D), rnd(g, 5, D), rnd(g, 5, D)
+    seq = torch.tensor(off, device="cuda")
+
+    def both():
+        h, last, marks = E().gated_scan(x, seq_off=seq, h0=h0, marks=True, **d)
+        gx, ga, g0 = E().gated_scan_grad(grad, x, marks, seq_off=seq, h0=h0, grad_last=gl, **d)
+        return [h, gx, ga if kind == "gate" else gx], [last, g0]
+    clean = both()
+    for s, bad in ((0, float("inf")), (2, float("nan")), (4, float("-inf")), (None, float("nan"))):
+        i, j = (650, T) if s is None else (off[s], off[s + 1])
+        kept = [t.clone() for t in (x, grad, gl, h0)]
+        x[i:j], grad[i:j] = bad, bad
+        if s is not None:
+            gl[s], h0[s] = bad, bad
+        rows, ends = both()
+        for got, want in zip(rows, clean[0]):
+            assert torch.equal(got[:i], want[:i]) and torch.equal(got[j:650], want[j:650])
+        for got, want in zip(ends, clean[1]):
+            others = [k for k in range(5) if k != s]
+            assert torch.equal(got[others], want[others])
+        if s is not None:
+            assert not bool(torch.isfinite(rows[0][i:j]).all())
+        for t, k in zip((x, grad, gl, h0), kept):
+            t.copy_(k)
+
+
+def test_scan_remembers_over_a_long_recording():
+    """Microseconds between events against time constants of seconds: what 1 - a of a rounded a would lose."""
+    g = gen(13)
+    T, D = 30000, 8
+    d = dict(dt=torch.rand(T, generator=g, device="cuda") * 2e-6, rate=torch.logspace(-2, 4, D, device="cuda"))
+    run_scan(torch.rand(T, D, generator=g, device="cuda"), d, None, rnd(g, 1, D), rnd(g, T, D), None)
+
+
+def test_scan_gradients_against_differences():
+    """<grad, direction> against the change of sum(weights * h) + sum(weights * last) in 64 bits: exact for x and h0 (linear),
+    a central difference for gates and rates (error of the step squared: third derivative, bounded by the values' own size)."""
+    g = gen(14)
+    T, D, off = 90, 12, [0, 40, 40, 90]
+    x, h0, cw, cl = rnd(g, T, D), rnd(g, 3, D), rnd(g, T, D), rnd(g, 3, D)
+    for kind in ("time", "gate"):
+        d = decays(kind, T, D, torch.float32, g)
+        seq = torch.tensor(off, device="cuda")
+        marks = E().gated_scan(x, seq_off=seq, h0=h0, marks=True, **d)[2]
+        gx, ga, g0 = E().gated_scan_grad(cw, x, marks, seq_off=seq, h0=h0, grad_last=cl, **d)
+
+        def loss(x_, h_, d_):
+            h, last, *_ = R.scan(x_, R.gates(d_.get("gate"), d_.get("dt"), d_.get("rate")), off, h_)
+            return (h * R.f64(cw)).sum() + (last * R.f64(cl)).sum()
+        vx, vh = rnd(g, T, D).double(), rnd(g, 3, D).double()
+        size = float(cw.abs().double().sum())
+        assert abs(float((gx.double() * vx).sum()) - (loss(x.double() + vx, h0, d) - loss(x, h0, d))) < 1e-5 * size
+        assert abs(float((g0.double() * vh).sum()) - (loss(x, h0.double() + vh, d) - loss(x, h0, d))) < 1e-5 * size
+        name = "rate" if kind == "time" else "gate"
+        va, e = rnd(g, *d[name].shape).double() * d[name].abs().double(), 1e-4
+        up = loss(x, h0, {**d, name: d[name].double() + e * va})
+        down = loss(x, h0, {**d, name: d[name].double() - e * va})
+        want = (up - down) / (2 * e)
+        assert abs(float((ga.double() * va).sum()) - want) < 1e-5 * size * max(1.0, abs(want) / size)
+
+
+# ------------------------------------------------------------------------------------------------------ single steps
+@pytest.mark.parametrize("kind", ["time", "gate", "gate32"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,D", [(1, 1), (1, 200), (5, 3), (33, 63), (100, 64), (3, 4096)])
+def test_single_steps(dtype, kind, n, D):
+    g = gen(n + D)
+    state, x, d = rnd(g, n, D), rnd(g, n, D, dtype=dtype), decays(kind, n, D, dtype, g)
+    a = R.gates(d.get("gate"), d.get("dt"), d.get("rate"))
+    want = a * R.f64(state) + R.f64(x)
+    bound = R.step_loss(a) * (np.abs(a * R.f64(state)) + np.abs(R.f64(x)))
+    out = torch.empty_like(state)
+    assert E().gated_step(state, x, out=out, **d) is out
+    R.check(out, want, bound)
+    table, w = rnd(g, 30, D, dtype=dtype), rnd(g, n)
+    tok = torch.randint(-1, 30, (n,), generator=g, device="cuda")
+    rows = R.embed(table, tok, w, 0.3)
+    want = a * R.f64(state) + rows
+    got = E().event_step(state, table, tok, weight=w, scale=0.3, out=out, check=True, **d)
+    R.check(got, want, R.step_loss(a) * (np.abs(a * R.f64(state)) + np.abs(rows)))
+    kept = out.clone()
+    assert E().event_step(state, table, tok.int(), weight=w, scale=0.3, **d) is state       # in place: the same bits
+    assert torch.equal(state, kept)
+
+
+def test_steps_follow_the_scan():
+    """Event by event through event_step, and all at once through lookup and scan."""
+    g = gen(20)
+    n, T, D, V = 3, 50, 63, 40
+    table, rate = rnd(g, V, D), torch.exp(rnd(g, D))
+    tok = torch.randint(-1, V, (n, T), generator=g, device="cuda")
+    dt = torch.rand(n, T, generator=g, device="cuda")
+    state = torch.zeros(n, D, device="cuda")
+    for t in range(T):
+        E().event_step(state, table, tok[:, t].contiguous(), scale=0.5, dt=dt[:, t].contiguous(), rate=rate)
+    x = E().embed_events(table, tok.reshape(-1), scale=0.5)
+    off = torch.arange(n + 1, device="cuda") * T
+    a = R.gates(None, dt.reshape(-1), rate)
+    _, last = E().gated_scan(x, dt=dt.reshape(-1), rate=rate, seq_off=off)
+    want = R.scan(x, a, off.tolist(), None)
+    R.check(state, want[1], want[4] + 3 * R.U * np.abs(want[1]))
+    R.check(last, want[1], want[4])
+
+
+def test_step_with_a_token_outside():
+    g = gen(21)
+    state, table = rnd(g, 4, 8), rnd(g, 5, 8)
+    tok = torch.tensor([0, 5, -1, 4], device="cuda")
+    d = dict(dt=torch.ones(4, device="cuda"), rate=torch.zeros(8, device="cuda"))
+    kept = state.clone()
+    with pytest.raises(IndexError, match="event 1: token 5"):
+        E().event_step(state, table, tok, check=True, **d)
+    assert torch.equal(state[1:3], kept[1:3]) and not torch.equal(state[0], kept[0])
+
+
+# --------------------------------------------------------------------------------- a training pass, streams and graphs
+def encoder_pass(table, tok, w, rate, dt, off, h0, grad):
+    """Lookup, scan and all gradients, as a training step of an event encoder runs them."""
+    V = table.shape[0]
+    x = E().embed_events(table, tok, weight=w, scale=0.5, check=False)
+    h, last, marks = E().gated_scan(x, dt=dt, rate=rate, seq_off=off, h0=h0, marks=True)
+    gx, gr, g0 = E().gated_scan_grad(grad, x, marks, dt=dt, rate=rate, seq_off=off, h0=h0)
+    gt, gw = E().embed_events_grad(gx, tok, V, weight=w, scale=0.5, table=table)
+    return h, last, gt, gw, gr, g0
+
+
+def encoder_inputs(seed, T=600, V=50, D=63):
+    g = gen(seed)
+    off = torch.tensor([0, 250, 250, T - 7], device="cuda")
+    return (rnd(g, V, D), skewed(T, V, g).clamp(max=V - 1), rnd(g, T), torch.exp(rnd(g, D)), torch.rand(T, generator=g, device="cuda"), off,
+            rnd(g, 3, D), rnd(g, T, D))
+
+
+def test_encoder_pass():
+    table, tok, w, rate, dt, off, h0, grad = args = encoder_inputs(30)
+    h, last, gt, gw, gr, g0 = encoder_pass(*args)
+    x = R.embed(table, tok, w, 0.5)
+    a = R.gates(None, dt, rate)
+    x32 = E().embed_events(table, tok, weight=w, scale=0.5)
+    want = R.scan(x32, a, off.tolist(), h0)
+    R.check(h, want[0], want[3])
+    R.check(last, want[1], want[4])
+    g, dr, want0, Eg, Er, E0 = R.scan_grad(grad, None, x32, a, dt, off.tolist(), h0)
+    R.check(gr, dr, Er)
+    R.check(g0, want0, E0)
+    # the table's gradient: 32-bit sums of rows that carry the scan's error
+    t64 = torch.from_numpy(g)
+    want_t, bound, want_w, bound_w = R.embed_grad(t64, tok, table.shape[0], w, 0.5, table)
+    slack = R.embed_grad(torch.from_numpy(Eg + R.U * np.abs(g)), tok, table.shape[0], w.abs(), 0.5, table.abs())
+    R.check(gt, want_t, bound + slack[0])
+    R.check(gw, want_w, bound_w + slack[2])
+    for _ in range(2):
+        for got, first in zip(encoder_pass(*args), (h, last, gt, gw, gr, g0)):
+            assert torch.equal(got, first)
+
+
+def test_encoder_pass_on_another_stream():
+    args = encoder_inputs(31, T=20000)
+    want = encoder_pass(*args)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    other = encoder_inputs(32, T=20000)
+    want_other = encoder_pass(*other)
+    torch.cuda.synchronize()
+    for _ in range(3):                                                   # two passes at once, each with buffers of its own
+        with torch.cuda.stream(a):
+            got = encoder_pass(*args)
+        with torch.cuda.stream(b):
+            got_other = encoder_pass(*other)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        assert all(torch.equal(x, y) for x, y in zip(got_other, want_other))
+
+
+def test_encoder_pass_in_a_graph():
+    args = encoder_inputs(33, T=9000)
+    state = torch.zeros(4, 63, device="cuda")
+    step = dict(dt=torch.full((4,), 0.1, device="cuda"), rate=args[3])
+    tok4 = torch.arange(4, device="cuda")
+    encoder_pass(*args)
+    E().event_step(state, args[0], tok4, **step)
+    state.zero_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        out = encoder_pass(*args)
+        E().event_step(state, args[0], tok4, **step)
+    expect = torch.zeros(4, 63, device="cuda")
+    for k in range(4):
+        fresh = encoder_inputs(40 + k, T=9000)
+        for mine, theirs in zip(args, fresh):
+            mine.copy_(theirs)                                         # other events, other lengths
+        args[5][2] = args[5][3] - 100 * k
+        want = encoder_pass(*args)
+        E().event_step(expect, args[0], tok4, **step)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+        assert torch.equal(state, expect)
