@@ -67,6 +67,7 @@ enum { LENS_F32 = 0, LENS_BF16 = 1, LENS_F16 = 2 };
 #define LENS_EMBED_MAX_DIM 2048              /* channels of a row */
 #define LENS_SCAN_MAX_ROWS 2147000000ll      /* rows (events) of one scan, all sequences together */
 #define LENS_SCAN_MAX_DIM 4096               /* channels of a state */
+#define LENS_SCAN_MAX_LD 1048576             /* elements between two rows of a scan: a tile is addressed with 32 bits */
 
 /* ABI version of the loaded library (== LENS_AMD_ABI_VERSION it was built with). */
 int lens_amd_abi_version(void);
