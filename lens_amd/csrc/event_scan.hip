@@ -7,9 +7,12 @@
 // Sequences lie one behind the other in the rows; row seq_off[s] starts sequence s.
 //
 // A run of rows acts on the state that enters it as h -> f h + H, and two runs in a row act as one such pair again.  So the
-// rows are cut into tiles; inside a tile every thread owns a few rows of V channels, kept in registers from one pass of
-// loads; the threads' pairs are joined through LDS, the tiles' pairs through memory while the rows stay where they are
-// (Chain below), so that inputs are read once and outputs written once.
+// rows are cut into tiles, a workgroup each, a tile into runs of 8 to 128 rows, a thread each (V channels), and there are
+// three launches:
+//   pairs   the pair of every run over its rows; those of a tile are joined in LDS to what is before each run, and the tile's
+//   join    what is before every tile (a few tiles are joined by the next launch itself)
+//   states  the states, a row after the other from what enters the run
+// The rows are read twice.  The second time is in the other order, so that what was read last comes from the Infinity Cache.
 // The order of every composition is fixed by T and D alone: results do not depend on timing.
 // A run with the start of a sequence in it does not depend on what enters: it is marked, and the state is selected, not
 // multiplied by zero (an infinity of one sequence must not reach the next).
@@ -25,13 +28,10 @@
 
 namespace {
 
-// Rows a thread owns in a tile.  Forward 16 (8 where the gates are 32-bit): x and gates are then 64 registers a thread at
-// most, and with at most 128 in all 16 wavefronts fit a CU.  Backward 8: x, gates and the states' gradient, and the
-// states in 32 bits.
-constexpr int BACK_L = 8;
-template <typename G> constexpr int FORWARD_L = 16;
-template <> constexpr int FORWARD_L<float> = 8;
-
+// Rows a thread loads at once (B below): 16 forward where x and gates are 64 registers then, else 8; backward 8, whose states
+// in 32 bits are 32 registers.
+constexpr int MARK_ROWS = 8;                       // rows between two marks: backward starts from one for every batch
+constexpr int MAX_RUN = 128;                       // rows of a run: 8, 16, .. 128
 constexpr int FAR = 1 << 30;                       // rows from a tile's first to one that it never reaches
 constexpr int64_t MAX_THREADS = 0xffff0000ll;      // of a launch in one direction
 
@@ -71,18 +71,36 @@ __device__ __forceinline__ vec<float, V> fma(vec<float, V> a, vec<float, V> b, v
     return r;
 }
 
+// Whole vectors of LDS (rows there are multiples of V floats).
+template <int V>
+__device__ __forceinline__ vec<float, V> lds_load(const float *p) { return *reinterpret_cast<const vec<float, V> *>(p); }
+
+template <int V>
+__device__ __forceinline__ void lds_store(float *p, vec<float, V> v) { *reinterpret_cast<vec<float, V> *>(p) = v; }
+
 __device__ __forceinline__ float exp_fast(float z) { return __builtin_amdgcn_exp2f(z * 1.44269504088896341f); }
 
-// exp(z) h: below 1/16 as h + expm1(z) h with the series to z^4 (the next term is z^4 / 120 = 1.3e-7 of it there), which keeps
-// what a rounded factor near 1 would lose; elsewhere by the factor, whose error is relative.
+// exp(z) h: below 1/2 as h + expm1(z) h, which keeps what a rounded factor near 1 would lose; elsewhere by the factor, whose
+// error is relative.  The polynomial is expm1(z) / z interpolated at the six Chebyshev points of [-1/2, 1/2]: 1.5e-7 of it.
+constexpr float NEAR = 0.5f;
+
+__device__ __forceinline__ float expm1_near(float z)
+{
+    float p = __builtin_fmaf(z, 0.00139822f, 0.00840803f);
+    p = __builtin_fmaf(z, p, 0.04166579f);
+    p = __builtin_fmaf(z, p, 0.16665966f);
+    p = __builtin_fmaf(z, p, 0.50000001f);
+    p = __builtin_fmaf(z, p, 1.0f);
+    return z * p;
+}
+
 __device__ __forceinline__ float decayed(float z, float h)
 {
-    float p = __builtin_fmaf(z, 0.041666668f, 0.16666667f);
-    p = __builtin_fmaf(z, p, 0.5f);
-    p = __builtin_fmaf(z, p, 1.0f);
-    const bool near = __builtin_fabsf(z) < 0.0625f;
-    return __builtin_fmaf(near ? z * p : exp_fast(z), h, near ? h : 0.0f);
+    const bool near = __builtin_fabsf(z) < NEAR;
+    return __builtin_fmaf(near ? expm1_near(z) : exp_fast(z), h, near ? h : 0.0f);
 }
+
+template <typename G> using gate_or_char = std::conditional_t<std::is_void_v<G>, char, G>;
 
 struct ScanArgs {
     const void *x, *gate, *grad;       // grad: gradient of the states (backward)
@@ -92,30 +110,66 @@ struct ScanArgs {
     void *h, *grad_x, *grad_gate;
     float *last, *marks, *grad_h0, *grad_rate;
     const float *marks_in;
-    uint64_t *words;                   // pairs of the tiles and of their groups (Chain)
-    unsigned *ticket;
+    float2 *agg;                       // [tiles][D] pairs of the tiles, in the order in which they are joined
+    float *entry;                      // [tiles][D] what enters them; NULL: few tiles, joined by those that need it
+    float *pre;                        // [tiles][ts][2][D] pairs of what is before a run in its tile
     float *part;                       // [tiles][D] a tile's share of grad_rate
     int64_t T;
     int ldx, ldg, ldh, ld_grad, ld_gx, ld_gg;
-    int n_seq, D, cg, lanes, ts, fill, ny, tiles, levels;
+    int n_seq, D, cg, lanes, ts, run, fill, ny, tiles;
 };
 
-// A tile's first row, and rows counted from it.
+// ------------------------------------------------------------------------------------------ rows, tiles, sequences
+// A tile's first row; rows of the tile are counted from it.  s_lo, s_hi: offsets up to its first, its last row.
 struct Tile {
     int64_t row0;
     int left;                          // rows from there to the end, FAR at most
-    __device__ __forceinline__ Tile(const ScanArgs &p, int tile, int L)
-    {
-        row0 = (int64_t)tile * (p.ts * L);
-        const int64_t n = p.T - row0;
-        left = n < FAR ? (int)n : FAR;
-    }
+    int s_lo, s_hi;
     __device__ __forceinline__ int rel(int64_t row) const
     {
         const int64_t d = row - row0;
         return d > FAR ? FAR : d < -FAR ? -FAR : (int)d;
     }
 };
+
+// How many of the n offsets are at most `row`: a wavefront asks for 64 at once.
+__device__ __forceinline__ int offsets_up_to(const int64_t *off, int n, int64_t row)
+{
+    const int lane = (int)threadIdx.x & 63;
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step - 1;
+        const int found = __builtin_popcountll(__ballot(at < hi && off[at < hi ? at : hi - 1] <= row));
+        lo += found * step;
+        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// All threads call it; ends with a barrier.
+__device__ __forceinline__ Tile tile_of(const ScanArgs &p, int index)
+{
+    __shared__ int found[2];
+    Tile t;
+    const int rows = p.ts * p.run;
+    t.row0 = (int64_t)index * rows;
+    const int64_t n = p.T - t.row0;
+    t.left = n < FAR ? (int)n : FAR;
+    t.s_lo = t.s_hi = 1;
+    if (p.off) {
+        const int wave = (int)threadIdx.x >> 6, last = blockDim.x > 64 ? 1 : 0;
+        for (int q = wave; q < 2; q += last + 1)
+            if (q == wave || !last) {
+                const int f = offsets_up_to(p.off, p.n_seq + 1, q ? t.row0 + rows - 1 : t.row0);
+                if ((threadIdx.x & 63) == 0) found[q] = f;
+            }
+        __syncthreads();
+        t.s_lo = __builtin_amdgcn_readfirstlane(found[0]);
+        t.s_hi = __builtin_amdgcn_readfirstlane(found[1]);
+    }
+    __syncthreads();
+    return t;
+}
 
 // Where a row lies.  s: its sequence (-1: before the first, n_seq: behind the last), next: where the following one starts.
 struct Place {
@@ -127,7 +181,7 @@ __device__ __forceinline__ Place locate(const ScanArgs &p, const Tile &tile, int
 {
     if (!p.off) return {0, tile.left, true, tile.row0 + t == 0};
     const int64_t row = tile.row0 + t;
-    int lo = 0, hi = p.n_seq + 1;
+    int lo = tile.s_lo, hi = tile.s_hi;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (p.off[mid] <= row) lo = mid + 1; else hi = mid;
@@ -151,7 +205,7 @@ __device__ __forceinline__ vec<float, V> row_or_zero(const float *m, int s, int 
     return load<V>(m + (int64_t)s * D + c);
 }
 
-// What a thread owns: L rows from t0, channels c .. c + V - 1.  The last lane of a row is moved back to end with it,
+// What a thread owns: a run of rows from t0, channels c .. c + V - 1.  The last lane of a row is moved back to end with it,
 // so that all lanes load whole vectors inside the row; channels that two lanes hold are computed alike by both.
 template <int V>
 __device__ __forceinline__ int channel_of(const ScanArgs &p, int y, int lane, bool &any)
@@ -162,7 +216,7 @@ __device__ __forceinline__ int channel_of(const ScanArgs &p, int y, int lane, bo
     return cc < p.D - V ? cc : p.D - V;
 }
 
-template <int V, int L>
+template <int V>
 struct Own {
     int lane, ts, c, n, t0;
     bool any;
@@ -171,24 +225,13 @@ struct Own {
         lane = (int)threadIdx.x % p.lanes;
         ts = (int)threadIdx.x / p.lanes;
         c = channel_of<V>(p, y, lane, any);
-        t0 = ts * L;
+        t0 = ts * p.run;
         const int left = tile.left - t0;
-        n = left <= 0 ? 0 : left < L ? left : L;
+        n = left <= 0 ? 0 : left < p.run ? left : p.run;
     }
 };
 
-template <int V, int L, typename T>
-__device__ __forceinline__ void load_rows(vec<T, V> (&r)[L], const T *base, int ld, const Own<V, L> &o, const Tile &tile)
-{
-    const T *first = base + tile.row0 * ld;
-#pragma unroll
-    for (int j = 0; j < L; ++j) {
-        const int t = o.t0 + j < tile.left ? o.t0 + j : tile.left - 1;      // rows behind the end: the last again, not used
-        r[j] = load<V>(behind(first, (uint32_t)(t * ld + o.c)));
-    }
-}
-
-// Keeps rows as they were loaded: what was computed from them before is computed again behind this, not held in registers
+// Keeps values as they were loaded: what was computed from them before is computed again behind this, not held in registers
 // (widened rows and decays' factors would take twice to four times the registers of the rows).
 template <typename T>
 __device__ __forceinline__ void as_loaded(T &v)
@@ -202,45 +245,76 @@ __device__ __forceinline__ void as_loaded(T &v)
     }
 }
 
-// Behind every second row of a walk: the compiler would otherwise work ahead on all rows' gates at once and spill.
-__device__ __forceinline__ void pace(int j)
-{
-    if (j & 1) __builtin_amdgcn_sched_barrier(0);
-}
+// Behind every row of a walk: the compiler would otherwise work ahead on all rows at once and spill.
+__device__ __forceinline__ void pace() { __builtin_amdgcn_sched_barrier(0); }
 
-// The L rows of a thread, a bit each: starts and ends a sequence, lies in one; ids (LDS) their sequences.  plain: all in one,
-// neither started nor ended here -- the walks have a path for these without any question.
+// B rows of an operand from row t on, as they are stored.
+template <int V, int B, typename T>
+struct Raw {
+    vec<T, V> r[B];
+    __device__ __forceinline__ void load_rows(const T *base, int ld, int t, int c, const Tile &tile)
+    {
+        const T *first = base + tile.row0 * ld;
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            const int at = t + j < tile.left ? t + j : tile.left - 1;      // rows behind the end: the last again, not used
+            r[j] = load<V>(behind(first, (uint32_t)(at * ld + c)));
+        }
+    }
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int j = 0; j < B; ++j) r[j] = vec<T, V>((T)0.0f);
+    }
+    __device__ __forceinline__ void again()
+    {
+#pragma unroll
+        for (int j = 0; j < B; ++j) as_loaded(r[j]);
+    }
+    __device__ __forceinline__ vec<float, V> operator[](int j) const { return wide<V, T>(r[j]); }
+};
+
+// The B rows from t on, a bit each: starts and ends a sequence, lies in one; ids (LDS) their sequences.  plain: all in one,
+// neither started nor ended here -- the walks have a short path for these.  What a walk makes of rows of no sequence is not
+// used: a sequence starts (backward: ends) with a value of its own.
 struct Rows {
     unsigned starts, ends, lives;
     bool plain;
 };
 
-template <int V, int L>
-__device__ __forceinline__ Rows rows_of(const ScanArgs &p, const Tile &tile, const Own<V, L> &o, int *ids)
+// `w` is the place of row t, and moves on to row t + B.
+template <int B>
+__device__ __forceinline__ Rows rows_of(const ScanArgs &p, const Tile &tile, Place &w, int t, int *ids)
 {
-    Place w = locate(p, tile, o.t0);
-    Rows r = {0, 0, (1u << L) - 1, w.live && !w.start && o.n == L && w.next > o.t0 + L};
+    const int left = tile.left - t, n = left < B ? left : B;
+    Rows r = {0, 0, (1u << B) - 1, w.live && !w.start && n == B && w.next > t + B};
     if (r.plain) return r;
     r.lives = 0;
     bool start = w.start;
-    for (int j = 0; j < o.n; ++j) {
-        if (o.t0 + j == w.next) {
-            advance(p, tile, w, o.t0 + j);
+    for (int j = 0; j < n; ++j) {
+        if (t + j == w.next) {
+            advance(p, tile, w, t + j);
             start = true;
         }
         if (w.live) {
             r.lives |= 1u << j;
             r.starts |= (start ? 1u : 0u) << j;
-            r.ends |= (o.t0 + j + 1 == w.next ? 1u : 0u) << j;
+            r.ends |= (t + j + 1 == w.next ? 1u : 0u) << j;
         }
         ids[j] = w.s;                                      // the same from every lane of the rows
         start = false;
     }
+    w.start = false;
+    if (n == B && t + B == w.next && p.off) {      // the row behind starts a sequence
+        advance(p, tile, w, t + B);
+        w.start = w.live;
+    }
     return r;
 }
 
+// ------------------------------------------------------------------------------------------ pairs
 // What a run of rows does to the state that enters it, f h + H.  For gates f is their product.  For decays it is kept so that
-// factors near 1 lose nothing when many runs are joined: with the sign bit f = expm1(z) in (-1/16, 0], h -> h + f h, without
+// factors near 1 lose nothing when many runs are joined: with the sign bit f = expm1(z) in (-0.4, 0], h -> h + f h, without
 // it f = exp(z).  MARK instead of a factor: the run does not depend on what enters.
 constexpr uint32_t MARK = 0x7fc00001u, QUIET = 0x7fc00000u;
 
@@ -264,527 +338,506 @@ struct Factor<void> {
     {
         const bool nf = (int)bits(f) < 0, ng = (int)bits(g) < 0;
         const float e = -__builtin_fabsf(__builtin_fmaf(f, g, f + g));
-        if (nf && ng) return e > -0.0606f ? e : 1.0f + e;
-        return (nf ? 1.0f + f : f) * (ng ? 1.0f + g : g);
+        const float far = (nf ? 1.0f + f : f) * (ng ? 1.0f + g : g);
+        return nf && ng ? (e > -0.39f ? e : 1.0f + e) : far;
     }
     static __device__ __forceinline__ float of(float z)
     {
-        float p = __builtin_fmaf(z, 0.041666668f, 0.16666667f);
-        p = __builtin_fmaf(z, p, 0.5f);
-        p = __builtin_fmaf(z, p, 1.0f);
-        return z <= 0.0f && z > -0.0625f ? -__builtin_fabsf(z * p) : exp_fast(z);
+        return z <= 0.0f && z > -NEAR ? -__builtin_fabsf(expm1_near(z)) : exp_fast(z);
     }
 };
 
-// A pair: (f, H) as above with f possibly MARK.  `then` is the later of the two.
+// A pair: (f, H) as above with f possibly MARK.  `then` joins the later one to it.
 template <typename G>
 struct Pair {
     float f, H;
-    __device__ __forceinline__ float over(float h) const { return bits(f) == MARK ? H : Factor<G>::apply(f, h, H); }
+    __device__ __forceinline__ float over(float h) const
+    {
+        const float r = Factor<G>::apply(f, h, H);
+        return bits(f) == MARK ? H : r;
+    }
     __device__ __forceinline__ Pair then(Pair n) const
     {
-        if (bits(n.f) == MARK) return n;
-        return {bits(f) == MARK ? f : Factor<G>::join(f, n.f), Factor<G>::apply(n.f, H, n.H)};
+        const float g = Factor<G>::join(f, n.f), r = Factor<G>::apply(n.f, H, n.H);
+        const bool marked = bits(n.f) == MARK;
+        return {marked || bits(f) == MARK ? __uint_as_float(MARK) : quiet(g), marked ? n.H : r};
     }
-    __device__ __forceinline__ uint64_t word() const
-    {
-        const uint32_t u = f != f && bits(f) != MARK ? QUIET : bits(f);       // a NaN of the inputs is no mark
-        return (uint64_t)bits(H) << 32 | u;
-    }
-    static __device__ __forceinline__ Pair of(uint64_t w) { return {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))}; }
+    static __device__ __forceinline__ float quiet(float f) { return f != f ? __uint_as_float(QUIET) : f; }   // a NaN of the inputs is no mark
     static __device__ __forceinline__ Pair none() { return {Factor<G>::one(), 0.0f}; }
 };
 
-// Gates of a thread's rows.  G = void: decays.
-template <int V, int L, typename G>
+// Gates of B rows.  G = void: decays.
+template <int V, int B, typename G>
 struct Gates {
-    vec<G, V> g[L];
-    __device__ __forceinline__ void load_all(const ScanArgs &p, const Own<V, L> &o, const Tile &tile)
+    Raw<V, B, G> g;
+    vec<float, V> a;                   // product over the rows so far
+    __device__ __forceinline__ Gates(const ScanArgs &, int) : a(1.0f) {}
+    __device__ __forceinline__ void load_rows(const ScanArgs &p, int t, int c, const Tile &tile)
     {
-        load_rows<V, L, G>(g, (const G *)p.gate, p.ldg, o, tile);
+        g.load_rows((const G *)p.gate, p.ldg, t, c, tile);
     }
-    __device__ __forceinline__ void again()
+    static constexpr bool near = true;
+    __device__ __forceinline__ void again() { g.again(); }
+    template <bool NEARBY> __device__ __forceinline__ vec<float, V> times(int j, vec<float, V> h) const { return g[j] * h; }
+    template <bool NEARBY> __device__ __forceinline__ vec<float, V> step(int j, vec<float, V> h, vec<float, V> x) const
     {
-#pragma unroll
-        for (int j = 0; j < L; ++j) as_loaded(g[j]);
-    }
-    __device__ __forceinline__ vec<float, V> times(int j, vec<float, V> h) const { return wide<V, G>(g[j]) * h; }
-    __device__ __forceinline__ vec<float, V> step(int j, vec<float, V> h, vec<float, V> x) const
-    {
-        return fma<V>(wide<V, G>(g[j]), h, x);
+        return fma<V>(g[j], h, x);
     }
     // of all rows; a run that is shorter, or not of one sequence, ends in a mark or behind all that counts
-    __device__ __forceinline__ vec<float, V> factor() const
+    __device__ __forceinline__ void add_rows()
     {
-        vec<float, V> a = wide<V, G>(g[0]);
 #pragma unroll
-        for (int j = 1; j < L; ++j) {
-            a *= wide<V, G>(g[j]);
-            pace(j);
-        }
-        return a;
+        for (int j = 0; j < B; ++j) a *= g[j];
     }
+    __device__ __forceinline__ vec<float, V> factor() const { return a; }
 };
 
-template <int V, int L>
-struct Gates<V, L, void> {
-    float dt[L];
+template <int V, int B>
+struct Gates<V, B, void> {
+    float dt[B], sum;
     vec<float, V> rate;
-    __device__ __forceinline__ void load_all(const ScanArgs &p, const Own<V, L> &o, const Tile &tile)
+    float fastest;
+    bool near;                         // all of the thread's are: no exponentials
+    __device__ __forceinline__ Gates(const ScanArgs &p, int c) : sum(0.0f), rate(load<V>(p.rate + c)), fastest(0.0f)
+    {
+#pragma unroll
+        for (int i = 0; i < V; ++i) fastest = __builtin_fmaxf(fastest, __builtin_fabsf(rate[i]));
+    }
+    __device__ __forceinline__ void load_rows(const ScanArgs &p, int t, int c, const Tile &tile)
     {
         const float *first = p.dt + tile.row0;
-        if (o.t0 + L <= tile.left) {
-            __builtin_memcpy(dt, behind(first, o.t0), sizeof(dt));
+        if (t + B <= tile.left) {
+            __builtin_memcpy(dt, behind(first, t), sizeof(dt));
         } else {
 #pragma unroll
-            for (int j = 0; j < L; ++j) dt[j] = first[o.t0 + j < tile.left ? o.t0 + j : tile.left - 1];
+            for (int j = 0; j < B; ++j) dt[j] = first[t + j < tile.left ? t + j : tile.left - 1];
         }
-        rate = load<V>(p.rate + o.c);
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < B; ++j) most = __builtin_fmaxf(most, __builtin_fabsf(dt[j]));
+        near = most * fastest < NEAR;
     }
     __device__ __forceinline__ void again()
     {
 #pragma unroll
-        for (int j = 0; j < L; ++j) as_loaded(dt[j]);
+        for (int j = 0; j < B; ++j) as_loaded(dt[j]);
     }
-    __device__ __forceinline__ vec<float, V> times(int j, vec<float, V> h) const
+    template <bool NEARBY> __device__ __forceinline__ vec<float, V> times(int j, vec<float, V> h) const
     {
         vec<float, V> r;
 #pragma unroll
-        for (int i = 0; i < V; ++i) r[i] = decayed(-dt[j] * rate[i], h[i]);
+        for (int i = 0; i < V; ++i) {
+            const float z = -dt[j] * rate[i];
+            r[i] = NEARBY ? __builtin_fmaf(expm1_near(z), h[i], h[i]) : decayed(z, h[i]);
+        }
         return r;
     }
-    __device__ __forceinline__ vec<float, V> step(int j, vec<float, V> h, vec<float, V> x) const { return times(j, h) + x; }
+    template <bool NEARBY> __device__ __forceinline__ vec<float, V> step(int j, vec<float, V> h, vec<float, V> x) const
+    {
+        return times<NEARBY>(j, h) + x;
+    }
+    __device__ __forceinline__ void add_rows()
+    {
+#pragma unroll
+        for (int j = 0; j < B; ++j) sum += dt[j];
+    }
     __device__ __forceinline__ vec<float, V> factor() const
     {
-        float z = 0.0f;
+        vec<float, V> f;
 #pragma unroll
-        for (int j = 0; j < L; ++j) z -= dt[j];
-        vec<float, V> a;
-#pragma unroll
-        for (int i = 0; i < V; ++i) a[i] = Factor<void>::of(z * rate[i]);
-        return a;
+        for (int i = 0; i < V; ++i) f[i] = Factor<void>::of(-sum * rate[i]);
+        return f;
     }
 };
 
-// Whole vectors of LDS (rows there are multiples of V floats).
+// ------------------------------------------------------------------------------------------ LDS, and joining pairs
+// LDS of a workgroup.  slots: its channels, `lanes` x V.
 template <int V>
-__device__ __forceinline__ vec<float, V> lds_load(const float *p) { return *reinterpret_cast<const vec<float, V> *>(p); }
-
-template <int V>
-__device__ __forceinline__ void lds_store(float *p, vec<float, V> v) { *reinterpret_cast<vec<float, V> *>(p) = v; }
-
-// The pairs of the sub-runs of a tile, in LDS: [ts][lanes * V] f, then H, then a mark each.
-template <int V, typename G>
-struct Pairs {
-    float *a, *h;
-    int *f;
-    int stride;
-    __device__ __forceinline__ Pairs(unsigned char *smem, const ScanArgs &p)
+struct Lds {
+    float *f, *h;                      // [ts][slots] pairs of the runs
+    int *ids;                          // [ts][16] sequences of the rows of a batch
+    int slots;
+    __device__ __forceinline__ Lds(const ScanArgs &p)
     {
-        stride = p.lanes * V;
-        a = reinterpret_cast<float *>(smem);
-        h = a + p.ts * stride;
-        f = reinterpret_cast<int *>(h + p.ts * stride);
+        extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+        slots = p.lanes * V;
+        f = reinterpret_cast<float *>(smem);
+        h = f + p.ts * slots;
+        ids = reinterpret_cast<int *>(h + p.ts * slots);
     }
-    __device__ __forceinline__ void put(int ts, int lane, vec<float, V> A, vec<float, V> H, bool mark)
-    {
-        lds_store<V>(a + ts * stride + lane * V, A);
-        lds_store<V>(h + ts * stride + lane * V, H);
-        if (lane == 0) f[ts] = mark;
-    }
-    // state behind sub-run k
-    __device__ __forceinline__ vec<float, V> over(int k, int lane, vec<float, V> st) const
-    {
-        const vec<float, V> A = lds_load<V>(a + k * stride + lane * V), H = lds_load<V>(h + k * stride + lane * V);
-        if (f[k]) return H;
-        vec<float, V> r;
-#pragma unroll
-        for (int i = 0; i < V; ++i) r[i] = Factor<G>::apply(A[i], st[i], H[i]);
-        return r;
-    }
-    // all sub-runs as one pair, from the first (or, BACK, the last) on; slot: the channel's place in a row
-    template <bool BACK>
-    __device__ __forceinline__ Pair<G> whole(const ScanArgs &p, int slot) const
-    {
-        Pair<G> w = Pair<G>::none();
-        for (int q = 0; q < p.ts; ++q) {
-            const int k = BACK ? p.ts - 1 - q : q;
-            w = w.then({f[k] ? __uint_as_float(MARK) : a[k * stride + slot], h[k * stride + slot]});
-        }
-        return w;
-    }
-    static __host__ __device__ size_t bytes(int ts, int lanes) { return ((size_t)ts * (2 * lanes * V + 1) * 4 + 15) & ~(size_t)15; }
+    static size_t bytes(int ts, int lanes) { return ((size_t)2 * ts * lanes * V + ts * 16) * 4; }
 };
 
-// What enters a tile.  The tiles of a launch are numbered by a ticket that every workgroup draws when it starts: a workgroup
-// waits only for such with smaller tickets, which run already, so every wait ends.  A tile's pair is published as soon
-// as its rows are read; 8 tiles are a group, 8 groups a group of the next level, and the last tile of a group
-// publishes the group's pair from the 8 below.  What enters tile i are the pairs before it in its group, before that
-// group in its own, and so on: about 3.5 pairs a level, read at once by a wavefront a level, always composed in the
-// same order.  A word is the pair of one channel: 8 bytes, stored and read whole, all ones until it is there (a lane a
-// channel: seven words in flight and few registers beside the rows).
-constexpr uint64_t EMPTY = ~0ull;
+// The channel of a slot, -1: none.
+template <int V>
+__device__ __forceinline__ int slot_channel(const ScanArgs &p, int y, int slot)
+{
+    bool any;
+    const int c = channel_of<V>(p, y, slot / V, any) + slot % V;
+    return any ? c : -1;
+}
 
-template <int V, typename G>
-struct Chain {
-    const ScanArgs &p;
-    const int tile, y, slots;          // slots: channels of the workgroup, one a lane of as many wavefronts as that takes
-    float *fs, *hs;                    // LDS [levels][slots]: the pairs before the tile, a level each
-    float *own_f, *own_h;              // LDS [slots]: the pair of the tile, then of what it completes
-    __device__ __forceinline__ Chain(const ScanArgs &p_, int tile_, int y_, unsigned char *smem)
-        : p(p_), tile(tile_), y(y_), slots(p_.lanes * V)
-    {
-        fs = reinterpret_cast<float *>(smem);
-        hs = fs + p.levels * slots;
-        own_f = hs + p.levels * slots;
-        own_h = own_f + slots;
-    }
-    static __host__ __device__ size_t bytes(int levels, int lanes) { return levels ? (size_t)(2 * levels + 2) * lanes * V * 4 : 0; }
-    // the word of a tile or group; false: the slot has no channel
-    __device__ __forceinline__ bool at(int level, int index, int slot, uint64_t *&word) const
-    {
-        bool any;
-        const int c = channel_of<V>(p, y, slot / V, any) + slot % V;
-        int64_t before = 0;
-        for (int l = 0; l < level; ++l) before += p.tiles >> (3 * l);
-        word = p.words + (before + index) * p.D + c;
-        return any && slot < slots;
-    }
-    __device__ __forceinline__ void publish(int level, int slot, Pair<G> w) const
-    {
-        uint64_t *to;
-        if (at(level, tile >> (3 * level), slot, to)) __hip_atomic_store(to, w.word(), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    // the pairs before the tile on one level, as one
-    __device__ __forceinline__ Pair<G> before(int level, int slot) const
-    {
-        const int index = tile >> (3 * level), n = index & 7;
-        Pair<G> w = Pair<G>::none();
-        uint64_t *from;
-        if (!at(level, index & ~7, slot, from) || n == 0) return w;
-        uint64_t v[7];
-        bool there;
-        do {
-            there = true;
+// The runs' pairs of a tile in LDS -> what is before each of them, and the tile's pair.  BACK: from the last run to the first.
+// A thread a channel.
+template <int V, typename G, bool BACK>
+__device__ __forceinline__ void join_runs(const ScanArgs &p, const Lds<V> &lds, int tile, int y, int order)
+{
+    const int slot = (int)threadIdx.x;
+    if (slot >= lds.slots) return;
+    const int c = slot_channel<V>(p, y, slot);
+    if (c < 0) return;
+    float *to = p.pre + (int64_t)tile * p.ts * 2 * p.D + c;
+    Pair<G> w = Pair<G>::none();
+    for (int q0 = 0; q0 < p.ts; q0 += 4) {
+        Pair<G> n[4];
 #pragma unroll
-            for (int k = 0; k < 7; ++k)
-                if (k < n) v[k] = __hip_atomic_load(from + (int64_t)k * p.D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-            for (int k = 0; k < 7; ++k)
-                if (k < n) there &= v[k] != EMPTY;
-            if (!there) __builtin_amdgcn_s_sleep(2);
-        } while (!there);
-#pragma unroll
-        for (int k = 0; k < 7; ++k)
-            if (k < n) w = w.then(Pair<G>::of(v[k]));
-        return w;
-    }
-    __device__ __forceinline__ void keep(float *f, float *h, int slot, Pair<G> w) const
-    {
-        if (slot >= slots) return;
-        f[slot] = w.f;
-        h[slot] = w.H;
-    }
-    // Publishes the tile's pair and collects what is before it.  All threads call it; the sub-runs' pairs are in `lds`.
-    template <bool BACK>
-    __device__ __forceinline__ void run(const Pairs<V, G> &lds) const
-    {
-        const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-        const int waves = blockDim.x < 64 ? 1 : (int)blockDim.x >> 6;      // whole ones
-        const int per = (slots + 63) / 64;                                 // wavefronts a level
-        int full = 0;                                                      // groups that end with this tile
-        while (full + 1 < p.levels && ((tile >> (3 * full)) & 7) == 7) ++full;
-        Pair<G> w = Pair<G>::none();
-        if (wave < per) {
-            const int slot = wave * 64 + lane;
-            w = lds.template whole<BACK>(p, slot < slots ? slot : 0);
-            if (tile + 1 < p.tiles) publish(0, slot, w);
-            if (full > 1) keep(own_f, own_h, slot, w);
+        for (int i = 0; i < 4; ++i) {
+            const int q = q0 + i < p.ts ? q0 + i : p.ts - 1, k = (BACK ? p.ts - 1 - q : q) * lds.slots + slot;
+            n[i] = {lds.f[k], lds.h[k]};
         }
-        if (full <= 1) {
-            for (int q = wave < waves ? wave : p.levels * per; q < p.levels * per; q += waves) {
-                const int l = q / per, slot = q % per * 64 + lane;
-                const Pair<G> b = before(l, slot);
-                if (l == 0 && full) publish(1, slot, b.then(w));           // q == wave: w is its own
-                keep(fs + l * slots, hs + l * slots, slot, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (q0 + i < p.ts) {
+                const int k = BACK ? p.ts - 1 - q0 - i : q0 + i;
+                to[2 * k * p.D] = w.f;
+                to[(2 * k + 1) * p.D] = w.H;
+                w = w.then(n[i]);
             }
-        } else {                                                           // level by level: what ends here waits for no higher one
-            for (int l = 0; l < p.levels; ++l) {
-                __syncthreads();
-                for (int k = 0; k < per; ++k) {
-                    if (wave != (l * per + k) % waves) continue;
-                    const int slot = k * 64 + lane;
-                    const Pair<G> b = before(l, slot);
-                    if (l < full && slot < slots) {
-                        w = b.then({own_f[slot], own_h[slot]});
-                        publish(l + 1, slot, w);
-                        keep(own_f, own_h, slot, w);
-                    }
-                    keep(fs + l * slots, hs + l * slots, slot, b);
-                }
-            }
+    }
+    p.agg[(int64_t)order * p.D + c] = make_float2(w.f, w.H);
+}
+
+// Tiles' pairs -> what enters every tile.  A workgroup holds 4 channels x 256 runs of up to JOIN tiles at once: every thread joins
+// its run, the 16 runs of a wavefront are joined by shuffles, the 16 wavefronts through LDS.
+constexpr int JOIN = 8;
+
+template <typename G>
+__global__ void __launch_bounds__(1024) k_scan_join(const float2 *__restrict__ agg, float *__restrict__ entry, int tiles, int D)
+{
+    __shared__ float2 waves[16][4];
+    const int lane = threadIdx.x & 3, run = threadIdx.x >> 2, wave = threadIdx.x >> 6;
+    const int c = blockIdx.x * 4 + lane < D ? blockIdx.x * 4 + lane : D - 1;
+    float enters = 0.0f;                                             // what enters the tiles from t0 on
+    for (int t0 = 0; t0 < tiles; t0 += 256 * JOIN) {
+        const int here = tiles - t0 < 256 * JOIN ? tiles - t0 : 256 * JOIN, per = (here + 255) / 256;
+        const int i0 = t0 + (run * per < here ? run * per : here), i1 = i0 + per < t0 + here ? i0 + per : t0 + here;
+        float2 v[JOIN];
+#pragma unroll
+        for (int k = 0; k < JOIN; ++k)
+            if (i0 + k < i1) v[k] = agg[(int64_t)(i0 + k) * D + c];
+        Pair<G> w = Pair<G>::none();
+#pragma unroll
+        for (int k = 0; k < JOIN; ++k)
+            if (i0 + k < i1) w = w.then({v[k].x, v[k].y});
+#pragma unroll
+        for (int d = 4; d < 64; d *= 2) {                            // w: from the wavefront's first run up to this one
+            const Pair<G> o = {__shfl_up(w.f, d, 64), __shfl_up(w.H, d, 64)};
+            if ((int)(threadIdx.x & 63) >= d) w = o.then(w);
+        }
+        if ((threadIdx.x & 63) >= 60) waves[wave][lane] = make_float2(w.f, w.H);
+        __syncthreads();
+        float st = enters;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            if (k == wave) st = enters;
+            enters = Pair<G>{waves[k][lane].x, waves[k][lane].y}.over(enters);
         }
         __syncthreads();
-    }
-    // the state that enters the tile, for a lane of the rows
-    __device__ __forceinline__ vec<float, V> entry(int lane) const
-    {
-        vec<float, V> st(0.0f);
-        for (int l = p.levels - 1; l >= 0; --l) {
-            const vec<float, V> f = lds_load<V>(fs + l * slots + lane * V), H = lds_load<V>(hs + l * slots + lane * V);
+        const Pair<G> o = {__shfl_up(w.f, 4, 64), __shfl_up(w.H, 4, 64)};
+        if ((threadIdx.x & 63) >= 4) st = o.over(st);
 #pragma unroll
-            for (int i = 0; i < V; ++i) st[i] = Pair<G>{f[i], H[i]}.over(st[i]);
-        }
-        return st;
+        for (int k = 0; k < JOIN; ++k)
+            if (i0 + k < i1) {
+                entry[(int64_t)(i0 + k) * D + c] = st;
+                st = Pair<G>{v[k].x, v[k].y}.over(st);
+            }
     }
-};
-
-// Before every launch of k_scan_states or k_scan_back with more than one tile.
-__global__ void __launch_bounds__(256) k_scan_clear(uint4 *words, int64_t n, unsigned *ticket)
-{
-    if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-        words[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
 }
 
-// The tile and channels of a workgroup.
-__device__ __forceinline__ unsigned draw_ticket(const ScanArgs &p)
+// What enters a thread's run.  All threads call it.  order: the tile's place among those that are joined.
+template <int V, typename G>
+__device__ __forceinline__ vec<float, V> run_entry(const ScanArgs &p, const Lds<V> &lds, const Own<V> &o, int tile, int y, int order)
 {
-    if (p.tiles == 1) return blockIdx.x;
-    __shared__ unsigned mine;
-    if (threadIdx.x == 0) mine = atomicAdd(p.ticket, 1u);
-    __syncthreads();
-    return __builtin_amdgcn_readfirstlane(mine);
-}
-
-// Pair of the rows of one thread.
-template <int V, int L, typename X, typename G>
-__device__ __forceinline__ void forward_pair(const ScanArgs &p, const Own<V, L> &o, const Rows &r, const int *ids,
-                                             const vec<X, V> (&x)[L], const Gates<V, L, G> &g, vec<float, V> &H)
-{
-    H = vec<float, V>(0.0f);
-    if (r.plain) {
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            H = g.step(j, H, wide<V, X>(x[j]));
-            pace(j);
-        }
+    const float *from = p.pre + ((int64_t)tile * p.ts + o.ts) * 2 * p.D + o.c;
+    const vec<float, V> f = load<V>(from), H = load<V>(from + p.D);
+    vec<float, V> st;
+    if (p.entry) {
+        st = load<V>(p.entry + (int64_t)order * p.D + o.c);
     } else {
+        const int slot = (int)threadIdx.x, c = slot < lds.slots ? slot_channel<V>(p, y, slot) : -1;
+        if (c >= 0) {
+            float h = 0.0f;
+            for (int b = 0; b < order; b += 8) {
+                float2 v[8];
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-            if (r.starts >> j & 1) H = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-            if (r.lives >> j & 1) H = g.step(j, H, wide<V, X>(x[j]));
-            pace(j);
+                for (int k = 0; k < 8; ++k) v[k] = p.agg[(int64_t)(b + k < order ? b + k : order - 1) * p.D + c];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (b + k < order) h = Pair<G>{v[k].x, v[k].y}.over(h);
+            }
+            lds.f[slot] = h;
         }
+        __syncthreads();
+        st = lds_load<V>(lds.f + o.lane * V);
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) st[i] = Pair<G>{f[i], H[i]}.over(st[i]);
+    return st;
 }
 
-// Rows -> states, and what is kept of them.
-template <int V, typename X, typename G>
-__global__ void __launch_bounds__(512, 4) k_scan_states(const ScanArgs p)
+// A run's pair into LDS.
+template <int V, typename G>
+__device__ __forceinline__ void put_pair(const Lds<V> &lds, const Own<V> &o, vec<float, V> f, vec<float, V> H, bool mark)
 {
-    constexpr int L = FORWARD_L<G>;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const unsigned ticket = draw_ticket(p);
-    const int index = ticket / p.ny, y = ticket % p.ny;
-    const Tile tile(p, index, L);
-    const Own<V, L> o(p, tile, y);
-    // a sequence without rows ends as it began
-    if (p.off)
-        for (int64_t s = index; s < p.n_seq; s += p.tiles)
-            if (p.off[s] == p.off[s + 1] && o.any && o.ts == 0)
-                store<V>(p.last + s * p.D + o.c, row_or_zero<V>(p.h0, (int)s, p.D, o.c));
-    if (p.T == 0) {
-        if (!p.off && o.any && o.ts == 0) store<V>(p.last + o.c, row_or_zero<V>(p.h0, 0, p.D, o.c));
-        return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = mark ? __uint_as_float(MARK) : Pair<G>::quiet(f[i]);
+    lds_store<V>(lds.f + o.ts * lds.slots + o.lane * V, f);
+    lds_store<V>(lds.h + o.ts * lds.slots + o.lane * V, H);
+}
+
+// ------------------------------------------------------------------------------------------ forward
+template <int V, int B, typename X, typename G>
+__global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
+{
+    const Lds<V> lds(p);
+    const int index = blockIdx.x, y = blockIdx.y;
+    const Tile tile = tile_of(p, index);
+    const Own<V> o(p, tile, y);
+    int *ids = lds.ids + o.ts * 16;
+    Gates<V, B, G> g(p, o.c);
+    vec<float, V> H(0.0f);
+    bool mark = false;
+    if (o.n > 0) {
+        Place w = locate(p, tile, o.t0);
+#pragma unroll 1
+        for (int b = 0; b < o.n; b += B) {
+            Raw<V, B, X> x;
+            x.load_rows((const X *)p.x, p.ldx, o.t0 + b, o.c, tile);
+            g.load_rows(p, o.t0 + b, o.c, tile);
+            const Rows r = rows_of<B>(p, tile, w, o.t0 + b, ids);
+            mark |= r.starts != 0;
+            if (__all(r.plain && g.near)) {
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    H = g.template step<true>(j, H, x[j]);
+                    pace();
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    if (r.starts >> j & 1) H = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+                    H = g.template step<false>(j, H, x[j]);
+                    pace();
+                }
+            }
+            g.again();
+            g.add_rows();
+        }
     }
-    const size_t pairs = Pairs<V, G>::bytes(p.ts, p.lanes);
-    Pairs<V, G> lds(smem, p);
-    Chain<V, G> chain(p, index, y, smem + pairs);
-    vec<X, V> x[L];
-    Gates<V, L, G> g;
-    load_rows<V, L, X>(x, (const X *)p.x, p.ldx, o, tile);
-    g.load_all(p, o, tile);
-    int *ids = reinterpret_cast<int *>(smem + pairs + Chain<V, G>::bytes(p.levels, p.lanes)) + o.t0;
-    const Rows rows = rows_of<V, L>(p, tile, o, ids);
-    {
-        vec<float, V> H;
-        forward_pair<V, L, X, G>(p, o, rows, ids, x, g, H);
-        lds.put(o.ts, o.lane, g.factor(), H, rows.starts != 0);
-    }
+    put_pair<V, G>(lds, o, g.factor(), H, mark);
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < L; ++j) as_loaded(x[j]);
-    g.again();
-    vec<float, V> st(0.0f);
-    if (p.levels) {
-        chain.template run<false>(lds);
-        st = chain.entry(o.lane);
-    }
-    if (!o.any || o.n == 0) return;
-    for (int k = 0; k < o.ts; ++k) st = lds.over(k, o.lane, st);
-    const int per_mark = BACK_L * p.ts;
-    if (p.marks && o.t0 % per_mark == 0) store<V>(p.marks + ((tile.row0 + o.t0) / per_mark) * p.D + o.c, st);
-    X *out = (X *)p.h + tile.row0 * p.ldh;
-    const uint32_t at = (uint32_t)(o.t0 * p.ldh + o.c);
-    if (rows.plain) {
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            st = g.step(j, st, wide<V, X>(x[j]));
-            store<V>(behind(out, at + j * p.ldh), st);
-            pace(j);
-        }
+    join_runs<V, G, false>(p, lds, index, y, index);
+}
+
+template <int V, int B, typename X, typename G>
+__global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
+{
+    const Lds<V> lds(p);
+    const int index = p.tiles - 1 - (int)blockIdx.x, y = blockIdx.y;       // what the first pass read last
+    // a sequence without rows ends as it began
+    if (p.off && y == 0)
+        for (int64_t s = index; s < p.n_seq; s += p.tiles)
+            if (p.off[s] == p.off[s + 1])
+                for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x) p.last[s * p.D + c] = p.h0 ? p.h0[s * p.D + c] : 0.0f;
+    if (p.T == 0) {
+        if (!p.off && y == 0)
+            for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x) p.last[c] = p.h0 ? p.h0[c] : 0.0f;
         return;
     }
+    const Tile tile = tile_of(p, index);
+    const Own<V> o(p, tile, y);
+    int *ids = lds.ids + o.ts * 16;
+    Gates<V, B, G> g(p, o.c);
+    Raw<V, B, X> x;
+    vec<float, V> st = run_entry<V, G>(p, lds, o, index, y, index);
+    if (!o.any || o.n == 0) return;
+    Place w = locate(p, tile, o.t0);
+    X *out = (X *)p.h + tile.row0 * p.ldh;
+#pragma unroll 1
+    for (int b = 0; b < o.n; b += B) {
+        const int t = o.t0 + b;
+        x.load_rows((const X *)p.x, p.ldx, t, o.c, tile);
+        g.load_rows(p, t, o.c, tile);
+        const Rows r = rows_of<B>(p, tile, w, t, ids);
+        float *mark = p.marks ? p.marks + (tile.row0 + t) / MARK_ROWS * p.D + o.c : nullptr;
+        const uint32_t at = (uint32_t)(t * p.ldh + o.c);
+        if (__all(r.plain && g.near)) {
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-        if (rows.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-        if (rows.lives >> j & 1) {
-            st = g.step(j, st, wide<V, X>(x[j]));
-            store<V>(behind(out, at + j * p.ldh), st);
-            if (rows.ends >> j & 1) store<V>(p.last + (int64_t)ids[j] * p.D + o.c, st);
-        } else if (j < o.n && p.fill) {
-            store<V>(behind(out, at + j * p.ldh), vec<float, V>(0.0f));
+            for (int j = 0; j < B; ++j) {
+                if (j % MARK_ROWS == 0 && mark) store<V>(mark + j / MARK_ROWS * p.D, st);
+                st = g.template step<true>(j, st, x[j]);
+                store<V>(behind(out, at + j * p.ldh), st);
+                pace();
+            }
+        } else {
+            const int n = tile.left - t;
+            const unsigned in = n < B ? (1u << n) - 1 : (1u << B) - 1, written = p.fill ? in : r.lives;
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                if (j % MARK_ROWS == 0 && mark && (in >> j & 1)) store<V>(mark + j / MARK_ROWS * p.D, st);
+                if (r.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+                st = g.template step<false>(j, st, x[j]);
+                if (written >> j & 1) store<V>(behind(out, at + j * p.ldh), r.lives >> j & 1 ? st : vec<float, V>(0.0f));
+                if (r.ends >> j & 1) store<V>(p.last + (int64_t)ids[j] * p.D + o.c, st);
+                pace();
+            }
         }
-        pace(j);
     }
 }
 
 // ------------------------------------------------------------------------------------------
 // Backward.  With r_t = a_t g_t the message that row t sends back: g_t = dh_t + r_{t+1}, so a run of rows acts on the
-// message that enters from behind as r -> A r + U with the A of the forward direction.
+// message that enters from behind as r -> f r + U with the f of the forward direction.  The states before the rows are
+// computed again from the marks, MARK_ROWS rows at a time.
 // ------------------------------------------------------------------------------------------
-
-template <int V, int L, typename X>
-__device__ __forceinline__ void load_grad(vec<X, V> (&d)[L], const ScanArgs &p, const Own<V, L> &o, const Tile &tile)
+template <int V, int B, typename X, typename G>
+__global__ void __launch_bounds__(256) k_scan_back_pairs(const ScanArgs p)
 {
-    if (p.grad) {
-        load_rows<V, L, X>(d, (const X *)p.grad, p.ld_grad, o, tile);
-    } else {
+    const Lds<V> lds(p);
+    const int index = blockIdx.x, y = blockIdx.y;
+    const Tile tile = tile_of(p, index);
+    const Own<V> o(p, tile, y);
+    int *ids = lds.ids + o.ts * 16;
+    Gates<V, B, G> g(p, o.c);
+    vec<float, V> U(0.0f);
+    bool mark = false;
+#pragma unroll 1
+    for (int b = p.run - B; b >= 0; b -= B) {
+        if (b >= o.n) continue;
+        Raw<V, B, X> d;
+        g.load_rows(p, o.t0 + b, o.c, tile);
+        if (p.grad) d.load_rows((const X *)p.grad, p.ld_grad, o.t0 + b, o.c, tile);
+        else d.zero();
+        Place w = locate(p, tile, o.t0 + b);
+        const Rows r = rows_of<B>(p, tile, w, o.t0 + b, ids);
+        mark |= r.ends != 0;
+        if (__all(r.plain && g.near)) {
 #pragma unroll
-        for (int j = 0; j < L; ++j) d[j] = vec<X, V>((X)0.0f);
+            for (int j = B - 1; j >= 0; --j) {
+                U = g.template times<true>(j, U + d[j]);
+                pace();
+            }
+        } else {
+#pragma unroll
+            for (int j = B - 1; j >= 0; --j) {
+                if (r.ends >> j & 1) U = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
+                U = g.template times<false>(j, U + d[j]);
+                pace();
+            }
+        }
+        g.again();
+        g.add_rows();
     }
+    put_pair<V, G>(lds, o, g.factor(), U, mark);
+    __syncthreads();
+    join_runs<V, G, true>(p, lds, index, y, p.tiles - 1 - index);
 }
 
-template <int V, int L, typename X, typename G>
-__device__ __forceinline__ void backward_pair(const ScanArgs &p, const Own<V, L> &o, const Rows &r, const int *ids,
-                                              const vec<X, V> (&d)[L], const Gates<V, L, G> &g, vec<float, V> &U)
+template <int V, int B, typename X, typename G>
+__global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
 {
-    U = vec<float, V>(0.0f);
-    if (r.plain) {
-#pragma unroll
-        for (int j = L - 1; j >= 0; --j) {
-            U = g.times(j, U + wide<V, X>(d[j]));
-            pace(j);
-        }
-    } else {
-#pragma unroll
-        for (int j = L - 1; j >= 0; --j) {
-            if (r.ends >> j & 1) U = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
-            if (r.lives >> j & 1) U = g.times(j, U + wide<V, X>(d[j]));
-            pace(j);
-        }
-    }
-}
-
-template <typename G> using G_or_char = std::conditional_t<std::is_void_v<G>, char, G>;
-
-template <int V, typename X, typename G>
-__global__ void __launch_bounds__(512, 4) k_scan_back(const ScanArgs p)
-{
-    constexpr int L = BACK_L;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const unsigned ticket = draw_ticket(p);
-    const int from_end = ticket / p.ny, index = p.tiles - 1 - from_end, y = ticket % p.ny;
-    const Tile tile(p, index, L);
-    const Own<V, L> o(p, tile, y);
+    const Lds<V> lds(p);
+    const int index = p.tiles - 1 - (int)blockIdx.x, y = blockIdx.y;       // what the first pass read last
     const vec<float, V> zero(0.0f);
-    if (p.off && p.grad_h0)
+    if (p.off && p.grad_h0 && y == 0)
         for (int64_t s = index; s < p.n_seq; s += p.tiles)
-            if (p.off[s] == p.off[s + 1] && o.any && o.ts == 0)
-                store<V>(p.grad_h0 + s * p.D + o.c, row_or_zero<V>(p.grad_last, (int)s, p.D, o.c));
+            if (p.off[s] == p.off[s + 1])
+                for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x)
+                    p.grad_h0[s * p.D + c] = p.grad_last ? p.grad_last[s * p.D + c] : 0.0f;
     if (p.T == 0) {
-        if (!p.off && p.grad_h0 && o.any && o.ts == 0) store<V>(p.grad_h0 + o.c, row_or_zero<V>(p.grad_last, 0, p.D, o.c));
-        if (__is_same(G, void) && o.any && o.ts == 0) store<V>(p.part + o.c, zero);
+        for (int c = (int)threadIdx.x; c < p.D && y == 0; c += blockDim.x) {
+            if (!p.off && p.grad_h0) p.grad_h0[c] = p.grad_last ? p.grad_last[c] : 0.0f;
+            if (__is_same(G, void)) p.part[c] = 0.0f;
+        }
         return;
     }
-    const size_t pairs = Pairs<V, G>::bytes(p.ts, p.lanes);
-    Pairs<V, G> fwd(smem, p), bwd(smem + pairs, p);
-    Chain<V, G> chain(p, from_end, y, smem + 2 * pairs);
-    vec<X, V> x[L], d[L];
-    Gates<V, L, G> g;
-    g.load_all(p, o, tile);
-    load_grad<V, L, X>(d, p, o, tile);
-    load_rows<V, L, X>(x, (const X *)p.x, p.ldx, o, tile);
-    int *ids = reinterpret_cast<int *>(smem + 2 * pairs + Chain<V, G>::bytes(p.levels, p.lanes)) + o.t0;
-    const Rows rows = rows_of<V, L>(p, tile, o, ids);
-    {
-        vec<float, V> U;
-        backward_pair<V, L, X, G>(p, o, rows, ids, d, g, U);
-        const vec<float, V> A = g.factor();
-        bwd.put(o.ts, o.lane, A, U, rows.ends != 0);
+    const Tile tile = tile_of(p, index);
+    const Own<V> o(p, tile, y);
+    int *ids = lds.ids + o.ts * 16;
+    vec<float, V> r = run_entry<V, G>(p, lds, o, index, y, p.tiles - 1 - index), share(0.0f);
+    Gates<V, B, G> g(p, o.c);
+    X *gx = (X *)p.grad_x + tile.row0 * p.ld_gx;
+    gate_or_char<G> *gg = (gate_or_char<G> *)p.grad_gate + tile.row0 * p.ld_gg;
+#pragma unroll 1
+    for (int b = p.run - B; b >= 0; b -= B) {
+        if (b >= o.n || !o.any) continue;
+        const int t = o.t0 + b;
+        Raw<V, B, X> x, d;
+        vec<float, V> before[B];
+        g.load_rows(p, t, o.c, tile);
+        x.load_rows((const X *)p.x, p.ldx, t, o.c, tile);
+        constexpr bool wide_rows = sizeof(X) == 4 && !__is_same(G, void);      // x, gates and gradient at once would not fit
+        auto load_d = [&]() {
+            if (p.grad) d.load_rows((const X *)p.grad, p.ld_grad, t, o.c, tile);
+            else d.zero();
+        };
+        if (!wide_rows) load_d();
+        vec<float, V> st = load<V>(p.marks_in + (tile.row0 + t) / MARK_ROWS * p.D + o.c);
+        Place w = locate(p, tile, t);
+        const Rows q = rows_of<B>(p, tile, w, t, ids);
+        const uint32_t at_x = (uint32_t)(t * p.ld_gx + o.c), at_g = (uint32_t)(t * p.ld_gg + o.c);
+        if (__all(q.plain && g.near)) {
 #pragma unroll
-        for (int j = 0; j < L; ++j) as_loaded(d[j]);
-        g.again();
-        forward_pair<V, L, X, G>(p, o, rows, ids, x, g, U);
-        fwd.put(o.ts, o.lane, A, U, rows.starts != 0);
-    }
-    __syncthreads();
+            for (int j = 0; j < B; ++j) {
+                before[j] = st;
+                if (j + 1 < B) st = g.template step<true>(j, st, x[j]);
+                pace();
+            }
+            g.again();
+            if (wide_rows) load_d();
 #pragma unroll
-    for (int j = 0; j < L; ++j) as_loaded(x[j]);
-    g.again();
-    vec<float, V> r(0.0f);
-    if (p.levels) {
-        chain.template run<true>(bwd);
-        r = chain.entry(o.lane);
-    }
-    vec<float, V> share(0.0f);
-    if (o.any && o.n > 0) {
-        // the state before every row of the thread
-        vec<float, V> before[L];
-        vec<float, V> st = load<V>(p.marks_in + (int64_t)index * p.D + o.c);
-        for (int k = 0; k < o.ts; ++k) st = fwd.over(k, o.lane, st);
+            for (int j = B - 1; j >= 0; --j) {
+                const vec<float, V> gt = r + d[j];
+                r = g.template times<true>(j, gt);
+                store<V>(behind(gx, at_x + j * p.ld_gx), gt);
+                if constexpr (__is_same(G, void)) share = fma<V>(r * -g.dt[j], before[j], share);
+                else store<V>(behind(gg, at_g + j * p.ld_gg), gt * before[j]);
+                pace();
+            }
+        } else {
+            const int n = tile.left - t;
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-            if (!rows.plain && (rows.starts >> j & 1)) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-            before[j] = st;
-            st = g.step(j, st, wide<V, X>(x[j]));
-            pace(j);
-        }
-        // the message from behind
-        g.again();
-        for (int k = p.ts - 1; k > o.ts; --k) r = bwd.over(k, o.lane, r);
-        X *gx = (X *)p.grad_x + tile.row0 * p.ld_gx;
-        G_or_char<G> *gg = (G_or_char<G> *)p.grad_gate + tile.row0 * p.ld_gg;
+            for (int j = 0; j < B; ++j) {
+                if (q.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+                before[j] = st;
+                st = g.template step<false>(j, st, x[j]);
+                pace();
+            }
+            g.again();
+            if (wide_rows) load_d();
 #pragma unroll
-        for (int j = L - 1; j >= 0; --j) {
-            vec<float, V> gt = zero, ga = zero;
-            if (!rows.plain && (rows.ends >> j & 1)) r = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
-            if (rows.plain || (rows.lives >> j & 1)) {
-                gt = r + wide<V, X>(d[j]);
-                r = g.times(j, gt);
+            for (int j = B - 1; j >= 0; --j) {
+                const bool live = q.lives >> j & 1;
+                if (q.ends >> j & 1) r = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
+                const vec<float, V> gt = r + d[j];
+                r = g.template times<false>(j, gt);
+                if (live && (q.starts >> j & 1) && p.grad_h0) store<V>(p.grad_h0 + (int64_t)ids[j] * p.D + o.c, r);
+                if (j < n) store<V>(behind(gx, at_x + j * p.ld_gx), live ? gt : zero);
                 if constexpr (__is_same(G, void)) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) share[i] = __builtin_fmaf(-g.dt[j] * r[i], before[j][i], share[i]);
+                    if (live) share = fma<V>(r * -g.dt[j], before[j], share);
                 } else {
-                    ga = gt * before[j];
+                    if (j < n) store<V>(behind(gg, at_g + j * p.ld_gg), live ? gt * before[j] : zero);
                 }
-                if (!rows.plain && (rows.starts >> j & 1) && p.grad_h0) store<V>(p.grad_h0 + (int64_t)ids[j] * p.D + o.c, r);
+                pace();
             }
-            if (rows.plain || j < o.n) {
-                store<V>(behind(gx, (uint32_t)((o.t0 + j) * p.ld_gx + o.c)), gt);
-                if constexpr (!__is_same(G, void)) store<V>(behind(gg, (uint32_t)((o.t0 + j) * p.ld_gg + o.c)), ga);
-            }
-            pace(j);
         }
     }
     if constexpr (__is_same(G, void)) {
         __syncthreads();
-        lds_store<V>(fwd.a + o.ts * fwd.stride + o.lane * V, share);
+        lds_store<V>(lds.f + o.ts * lds.slots + o.lane * V, share);
         __syncthreads();
         if (o.ts == 0 && o.any) {
-            share = zero;
-            for (int k = 0; k < p.ts; ++k) share += lds_load<V>(fwd.a + k * fwd.stride + o.lane * V);
+            for (int k = 1; k < p.ts; ++k) share += lds_load<V>(lds.f + k * lds.slots + o.lane * V);
             store<V>(p.part + (int64_t)index * p.D + o.c, share);
         }
     }
@@ -797,8 +850,17 @@ __global__ void __launch_bounds__(1024) k_scan_rate(const float *__restrict__ pa
     const int lane = threadIdx.x & 15, run = threadIdx.x >> 4;
     const int c = blockIdx.x * 16 + lane;
     float v = 0.0f;
-    if (c < D)
-        for (int i = run; i < tiles; i += 64) v += part[(int64_t)i * D + c];
+    if (c < D) {
+        int i = run;
+        for (; i + 7 * 64 < tiles; i += 8 * 64) {
+            float u[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[k] = part[(int64_t)(i + 64 * k) * D + c];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += u[k];
+        }
+        for (; i < tiles; i += 64) v += part[(int64_t)i * D + c];
+    }
     sum[run][lane] = v;
     __syncthreads();
     for (int k = 32; k > 0; k >>= 1) {
@@ -858,70 +920,84 @@ __global__ void __launch_bounds__(256) k_step(const StepArgs p)
 
 // ------------------------------------------------------------------------------------------ launches
 struct Shape {
-    int V, cg, ny, lanes, ts;
+    int V, cg, ny, lanes, ts, run;
 };
 
-Shape shape_of(int D)
+// run: the longest that leaves 1024 workgroups (four a CU), the shortest where there is less
+Shape shape_of(int64_t T, int D)
 {
     Shape s;
     s.V = D >= 4 ? 4 : 1;
     s.cg = (D + s.V - 1) / s.V;
     s.ny = (s.cg + 63) / 64;
     s.lanes = (s.cg + s.ny - 1) / s.ny;
-    s.ts = 512 / s.lanes;
+    s.ts = 256 / s.lanes;
     if (s.ts > 32) s.ts = 32;
-    s.ts &= ~1;                         // a forward tile of 16 rows a thread is two marks long
+    s.run = MAX_RUN;
+    while (s.run > 8 && T * s.ny < (int64_t)1024 * s.run * s.ts) s.run /= 2;
     return s;
 }
 
+constexpr int FEW_TILES = 64;
+
 struct Scratch {
-    int64_t tiles, words;
-    int levels;
-    size_t ticket, part, bytes;
+    int64_t tiles;
+    size_t agg, entry, pre, part, bytes;
 };
 
-Scratch scratch_of(int64_t T, int D, int rows_a_thread, bool back)
+Scratch scratch_of(int64_t T, int D, bool back)
 {
-    const int64_t rows = (int64_t)rows_a_thread * shape_of(D).ts;
+    const Shape s = shape_of(T, D);
+    const int64_t rows = (int64_t)s.run * s.ts;
     Scratch r;
     r.tiles = T > 0 ? (T + rows - 1) / rows : 1;
-    r.levels = 0;
-    r.words = 0;
-    while ((r.tiles - 1) >> (3 * r.levels)) r.words += (r.tiles >> (3 * r.levels++)) * D;
-    r.words = (r.words + 1) & ~(int64_t)1;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t here = at; at += (n + 255) & ~(size_t)255; return here; };
-    take((size_t)r.words * 8);
-    r.ticket = take(4);
+    r.agg = take((size_t)r.tiles * D * 8);
+    r.entry = take((size_t)r.tiles * D * 4);
+    r.pre = take((size_t)r.tiles * s.ts * 2 * D * 4);
     r.part = back ? take((size_t)r.tiles * D * 4) : at;
     r.bytes = at;
     return r;
 }
 
-int forward_rows(int gates, int gate_type) { return gates && gate_type == LENS_F32 ? FORWARD_L<float> : FORWARD_L<void>; }
-
-void clear_words(const ScanArgs &p, const Scratch &r, hipStream_t st)
+template <typename G>
+void launch_join(const ScanArgs &p, hipStream_t st)
 {
-    if (!r.levels) return;
-    const int64_t n = r.words / 2, blocks = (n + 256 * 4 - 1) / (256 * 4);
-    hipLaunchKernelGGL(k_scan_clear, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (uint4 *)p.words, n, p.ticket);
+    if (p.entry) hipLaunchKernelGGL(k_scan_join<G>, dim3((p.D + 3) / 4), dim3(1024), 0, st, p.agg, p.entry, p.tiles, p.D);
+}
+
+template <int V, int B, typename X, typename G>
+void launch_forward_of(const ScanArgs &p, hipStream_t st)
+{
+    const dim3 grid(p.tiles, p.ny), block(p.lanes * p.ts);
+    const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
+    if (p.T > 0) {
+        hipLaunchKernelGGL((k_scan_pairs<V, B, X, G>), grid, block, lds, st, p);
+        launch_join<G>(p, st);
+    }
+    hipLaunchKernelGGL((k_scan_states<V, B, X, G>), grid, block, lds, st, p);
 }
 
 template <int V, typename X, typename G>
-int launch_forward(ScanArgs &p, const Scratch &r, hipStream_t st)
+int launch_forward(const ScanArgs &p, hipStream_t st)
 {
-    clear_words(p, r, st);
-    const size_t lds = Pairs<V, G>::bytes(p.ts, p.lanes) + Chain<V, G>::bytes(r.levels, p.lanes) + p.ts * FORWARD_L<G> * 4;
-    hipLaunchKernelGGL((k_scan_states<V, X, G>), dim3((unsigned)(p.tiles * p.ny)), dim3(p.lanes * p.ts), lds, st, p);
+    constexpr int B = sizeof(X) + (__is_same(G, void) ? 0 : sizeof(gate_or_char<G>)) <= 4 ? 16 : 8;
+    if (p.run >= B) launch_forward_of<V, B, X, G>(p, st);
+    else launch_forward_of<V, 8, X, G>(p, st);
     return (int)hipGetLastError();
 }
 
 template <int V, typename X, typename G>
-int launch_backward(ScanArgs &p, const Scratch &r, hipStream_t st)
+int launch_backward(const ScanArgs &p, hipStream_t st)
 {
-    clear_words(p, r, st);
-    const size_t lds = 2 * Pairs<V, G>::bytes(p.ts, p.lanes) + Chain<V, G>::bytes(r.levels, p.lanes) + p.ts * BACK_L * 4;
-    hipLaunchKernelGGL((k_scan_back<V, X, G>), dim3((unsigned)(p.tiles * p.ny)), dim3(p.lanes * p.ts), lds, st, p);
+    const dim3 grid(p.tiles, p.ny), block(p.lanes * p.ts);
+    const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
+    if (p.T > 0) {
+        hipLaunchKernelGGL((k_scan_back_pairs<V, MARK_ROWS, X, G>), grid, block, lds, st, p);
+        launch_join<G>(p, st);
+    }
+    hipLaunchKernelGGL((k_scan_back<V, MARK_ROWS, X, G>), grid, block, lds, st, p);
     if (__is_same(G, void))
         hipLaunchKernelGGL(k_scan_rate, dim3((p.D + 15) / 16), dim3(1024), 0, st, p.part, p.grad_rate, p.tiles, p.D);
     return (int)hipGetLastError();
@@ -956,13 +1032,13 @@ int by_types(int V, int x_type, bool gates, int gate_type, F f)
 }
 
 struct ForwardCall {
-    ScanArgs &p; const Scratch &r; hipStream_t st;
-    template <int V, typename X, typename G> int go() { return launch_forward<V, X, G>(p, r, st); }
+    ScanArgs &p; hipStream_t st;
+    template <int V, typename X, typename G> int go() { return launch_forward<V, X, G>(p, st); }
 };
 
 struct BackwardCall {
-    ScanArgs &p; const Scratch &r; hipStream_t st;
-    template <int V, typename X, typename G> int go() { return launch_backward<V, X, G>(p, r, st); }
+    ScanArgs &p; hipStream_t st;
+    template <int V, typename X, typename G> int go() { return launch_backward<V, X, G>(p, st); }
 };
 
 struct StepCall {
@@ -1002,14 +1078,13 @@ extern "C" {
 int lens_scan_mark_rows(int D)
 {
     if (D < 1 || D > LENS_SCAN_MAX_DIM) return 0;
-    return BACK_L * shape_of(D).ts;
+    return MARK_ROWS;
 }
 
 size_t lens_gated_scan_scratch_bytes(int64_t T, int D, int backward)
 {
     if (T < 0 || T > LENS_SCAN_MAX_ROWS || D < 1 || D > LENS_SCAN_MAX_DIM) return 0;
-    // 8 rows a thread: the forward pass of other gates has half as many tiles
-    return scratch_of(T, D, BACK_L, backward != 0).bytes;
+    return scratch_of(T, D, backward != 0).bytes;
 }
 
 int lens_gated_scan(const void *d_x, int x_type, int64_t ldx, const void *d_gate, int gate_type, int64_t ldg,
@@ -1021,17 +1096,18 @@ int lens_gated_scan(const void *d_x, int x_type, int64_t ldx, const void *d_gate
     if (!d_last || !d_scratch || (T > 0 && !d_h)) return LENS_ERR_NULL;
     if ((T > 1 && ldh < D) || ldh > LENS_SCAN_MAX_LD) return LENS_ERR_SIZE;
     if (off_element(d_h, x_type) || (((uintptr_t)d_last | (uintptr_t)d_marks) & 3) || ((uintptr_t)d_scratch & 15)) return LENS_ERR_ALIGN;
-    const Shape s = shape_of(D);
-    const Scratch r = scratch_of(T, D, forward_rows(d_gate != nullptr, gate_type), false);
-    if (scratch_bytes < lens_gated_scan_scratch_bytes(T, D, 0)) return LENS_ERR_SCRATCH;
-    if (r.tiles * s.ny * 512 > MAX_THREADS) return LENS_ERR_SIZE;
+    const Shape s = shape_of(T, D);
+    const Scratch r = scratch_of(T, D, false);
+    if (scratch_bytes < r.bytes) return LENS_ERR_SCRATCH;
+    if (r.tiles * 256 > MAX_THREADS) return LENS_ERR_SIZE;
     unsigned char *base = (unsigned char *)d_scratch;
     ScanArgs p = {};
     p.x = d_x; p.gate = d_gate; p.dt = d_dt; p.rate = d_rate; p.off = d_seq_off; p.h0 = d_h0; p.h = d_h; p.last = d_last;
-    p.marks = d_marks; p.words = (uint64_t *)base; p.ticket = (unsigned *)(base + r.ticket);
+    p.marks = d_marks; p.agg = (float2 *)(base + r.agg); p.pre = (float *)(base + r.pre);
+    p.entry = r.tiles > FEW_TILES ? (float *)(base + r.entry) : nullptr;
     p.T = T; p.ldx = (int)ldx; p.ldg = (int)ldg; p.ldh = (int)ldh; p.n_seq = n_seq; p.D = D; p.cg = s.cg;
-    p.lanes = s.lanes; p.ts = s.ts; p.ny = s.ny; p.fill = fill; p.tiles = (int)r.tiles; p.levels = r.levels;
-    return by_types(s.V, x_type, d_rate == nullptr, gate_type, ForwardCall{p, r, (hipStream_t)stream});
+    p.lanes = s.lanes; p.ts = s.ts; p.run = s.run; p.ny = s.ny; p.fill = fill; p.tiles = (int)r.tiles;
+    return by_types(s.V, x_type, d_rate == nullptr, gate_type, ForwardCall{p, (hipStream_t)stream});
 }
 
 int lens_gated_scan_grad(const void *d_grad_h, int64_t ld_grad, const float *d_grad_last, const void *d_x, int x_type, int64_t ldx,
@@ -1049,19 +1125,20 @@ int lens_gated_scan_grad(const void *d_grad_h, int64_t ld_grad, const float *d_g
     if ((((uintptr_t)d_grad_last | (uintptr_t)d_marks | (uintptr_t)d_grad_rate | (uintptr_t)d_grad_h0) & 3) ||
         ((uintptr_t)d_scratch & 15))
         return LENS_ERR_ALIGN;
-    const Shape s = shape_of(D);
-    const Scratch r = scratch_of(T, D, BACK_L, true);
-    if (scratch_bytes < lens_gated_scan_scratch_bytes(T, D, 1)) return LENS_ERR_SCRATCH;
-    if (r.tiles * s.ny * 512 > MAX_THREADS) return LENS_ERR_SIZE;
+    const Shape s = shape_of(T, D);
+    const Scratch r = scratch_of(T, D, true);
+    if (scratch_bytes < r.bytes) return LENS_ERR_SCRATCH;
+    if (r.tiles * 256 > MAX_THREADS) return LENS_ERR_SIZE;
     unsigned char *base = (unsigned char *)d_scratch;
     ScanArgs p = {};
     p.x = d_x; p.gate = d_gate; p.grad = d_grad_h; p.dt = d_dt; p.rate = d_rate; p.off = d_seq_off; p.h0 = d_h0;
     p.grad_last = d_grad_last; p.grad_x = d_grad_x; p.grad_gate = d_grad_gate; p.grad_h0 = d_grad_h0; p.grad_rate = d_grad_rate;
-    p.marks_in = d_marks; p.words = (uint64_t *)base; p.ticket = (unsigned *)(base + r.ticket);
+    p.marks_in = d_marks; p.agg = (float2 *)(base + r.agg); p.pre = (float *)(base + r.pre);
+    p.entry = r.tiles > FEW_TILES ? (float *)(base + r.entry) : nullptr;
     p.part = (float *)(base + r.part);
     p.T = T; p.ldx = (int)ldx; p.ldg = (int)ldg; p.ld_grad = (int)ld_grad; p.ld_gx = (int)ld_gx; p.ld_gg = (int)ld_gg;
-    p.n_seq = n_seq; p.D = D; p.cg = s.cg; p.lanes = s.lanes; p.ts = s.ts; p.ny = s.ny; p.tiles = (int)r.tiles; p.levels = r.levels;
-    return by_types(s.V, x_type, d_rate == nullptr, gate_type, BackwardCall{p, r, (hipStream_t)stream});
+    p.n_seq = n_seq; p.D = D; p.cg = s.cg; p.lanes = s.lanes; p.ts = s.ts; p.run = s.run; p.ny = s.ny; p.tiles = (int)r.tiles;
+    return by_types(s.V, x_type, d_rate == nullptr, gate_type, BackwardCall{p, (hipStream_t)stream});
 }
 
 int lens_gated_step(const float *d_state, int64_t lds, const void *d_x, int x_type, int64_t ldx,

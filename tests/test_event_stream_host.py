@@ -84,7 +84,7 @@ def test_scan_refusals(L):
         assert call(**bad) == ALIGN, bad
     assert call(bytes=L.lens_gated_scan_scratch_bytes(100, 64, 0) - 1) == SCRATCH
     assert L.lens_gated_scan_scratch_bytes(-1, 4, 0) == 0 and L.lens_scan_mark_rows(0) == 0 and L.lens_scan_mark_rows(4097) == 0
-    assert all(L.lens_scan_mark_rows(D) >= 16 for D in range(1, 4097))
+    assert all(L.lens_scan_mark_rows(D) >= 8 for D in range(1, 4097))
 
 
 def test_scan_gradient_refusals(L):
