@@ -490,14 +490,15 @@ def sad_matrix(query, reference):
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # LENS_F32, LENS_BF16, LENS_F16
 
 
-def _call(name, t, *args):
-    """One entry point on the current stream of t's device (which need not be the current one)."""
+# The checks below are made in one go where nothing is wrong: a call of a few microseconds is mostly its host side.
+def _call(name, dev, *args):
+    """One entry point on the current stream of device `dev` (an index; it need not be the current device)."""
     fn = getattr(_lib.lib(), name)
-    if t.device.index == torch.cuda.current_device():
-        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if dev == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(t.device):
-            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if st:
         _lib.check(st, name)
 
@@ -506,11 +507,23 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _rows(t, name, n, D, dtype, device, spread=False):
+def _device(t, name):
+    """The index of t's device; a LensAmdError for a tensor in host memory."""
+    dev = t.get_device()
+    if dev < 0:
+        _need_cuda(t, name)
+    return dev
+
+
+def _rows(t, name, n, D, dtype, dev, spread=False):
     """The leading dimension of a [n, D] operand, checked; spread: rows may be one row, expanded."""
+    if t.dtype is dtype and t.shape == (n, D) and t.get_device() == dev:
+        ld, last = t.stride()
+        if last == 1 and ld >= D:
+            return ld
     assert t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}"
-    assert t.dim() == 2 and t.shape[0] == n and t.shape[1] == D, f"{name} must be [{n}, {D}], got {list(t.shape)}"
-    assert t.device == device, f"{name} is on {t.device}, expected {device}"
+    assert tuple(t.shape) == (n, D), f"{name} must be [{n}, {D}], got {list(t.shape)}"
+    assert t.get_device() == dev, f"{name} is on {t.device}, expected device {dev}"
     ld, last = t.stride()
     assert last == 1 or D <= 1, f"{name}: the last index must be contiguous"
     if n <= 1:
@@ -519,18 +532,25 @@ def _rows(t, name, n, D, dtype, device, spread=False):
     return ld
 
 
-def _flat(t, name, n, dtype, device):
+def _flat(t, name, n, dtype, dev):
+    """The address of n contiguous elements, checked."""
+    if t.dtype is dtype and t.numel() == n and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
     assert t.dtype == dtype and t.is_contiguous() and t.numel() == n, f"{name} must be {n} contiguous {dtype}, got {list(t.shape)} {t.dtype}"
-    assert t.device == device, f"{name} is on {t.device}, expected {device}"
+    assert t.get_device() == dev, f"{name} is on {t.device}, expected device {dev}"
     return t.data_ptr()
 
 
-def _tokens(tokens, device=None):
-    _need_cuda(tokens, "tokens")
-    assert tokens.dtype in (torch.int32, torch.int64) and tokens.dim() == 1 and tokens.is_contiguous(), \
-        "tokens must be a contiguous int32 or int64 vector"
-    assert device is None or tokens.device == device, f"tokens are on {tokens.device}, expected {device}"
-    return tokens.element_size()
+_TOKENS = {torch.int32: 4, torch.int64: 8}
+
+
+def _tokens(tokens, n, dev):
+    """The size of a token of the vector, checked (n: how many there must be)."""
+    size = _TOKENS.get(tokens.dtype)
+    assert size and tokens.dim() == 1 and tokens.is_contiguous(), "tokens must be a contiguous int32 or int64 vector"
+    assert tokens.shape[0] == n, f"{tokens.shape[0]} tokens, expected {n}"
+    assert tokens.get_device() == dev, f"tokens are on {tokens.device}, expected device {dev}"
+    return size
 
 
 def _raise_bad(first_bad, tokens, n_rows):
@@ -545,19 +565,20 @@ def embed_events(table, tokens, weight=None, scale=1.0, out=None, check=True):
     table float32 / bfloat16 / float16 [n_rows, D] (rows may be strided), tokens int32 / int64 [T], weight float32 [T] or None.
     Token -1 is padding and gives a row of zeros.  Any other token outside the table raises IndexError (check=True, which
     synchronises); with check=False it gives a row of zeros too.  `out` must not overlap the inputs."""
-    _need_cuda(table, "table")
-    dev = table.device
-    size = _tokens(tokens, dev)
-    assert table.dtype in _TYPES, f"table must be float32, bfloat16 or float16, got {table.dtype}"
+    dev = _device(table, "table")
+    assert table.dtype in _TYPES and table.dim() == 2, f"table must be [n, D] in float32, bfloat16 or float16, got {list(table.shape)} {table.dtype}"
     V, D = table.shape
-    T = tokens.shape[0]
+    T = tokens.shape[0] if tokens.dim() else -1
+    size = _tokens(tokens, T, dev)
     ld = _rows(table, "table", V, D, table.dtype, dev)
     w = None if weight is None else _flat(weight, "weight", T, torch.float32, dev)
     if out is None:
-        out = torch.empty((T, D), dtype=table.dtype, device=dev)
-    ldo = _rows(out, "out", T, D, table.dtype, dev)
-    bad = torch.full((1,), INT64_MAX, dtype=torch.int64, device=dev) if check else None
-    _call("lens_embed_events", table, table.data_ptr(), _TYPES[table.dtype], V, ld, tokens.data_ptr(), size, w, scale, T, D,
+        out = table.new_empty((T, D))
+        ldo = D
+    else:
+        ldo = _rows(out, "out", T, D, table.dtype, dev)
+    bad = torch.full((1,), INT64_MAX, dtype=torch.int64, device=table.device) if check else None
+    _call("lens_embed_events", dev, table.data_ptr(), _TYPES[table.dtype], V, ld, tokens.data_ptr(), size, w, scale, T, D,
           out.data_ptr(), ldo, _addr(bad))
     if check:
         _raise_bad(bad, tokens, V)
@@ -567,13 +588,14 @@ def embed_events(table, tokens, weight=None, scale=1.0, out=None, check=True):
 def sort_events(tokens, n_rows):
     """The tokens in ascending order (int32 [T]; equal ones keep their order) and where each stood (int32 [T]).  Tokens outside
     [0, n_rows), padding among them, come last as n_rows."""
-    size = _tokens(tokens)
-    T = tokens.shape[0]
+    dev = _device(tokens, "tokens")
+    T = tokens.shape[0] if tokens.dim() else -1
+    size = _tokens(tokens, T, dev)
     keys = torch.empty((T,), dtype=torch.int32, device=tokens.device)
     index = torch.empty((T,), dtype=torch.int32, device=tokens.device)
     need = _lib.lib().lens_sort_tokens_scratch_bytes(T, n_rows)
     scratch = torch.empty((need,), dtype=torch.uint8, device=tokens.device)
-    _call("lens_sort_tokens", tokens, tokens.data_ptr(), size, T, n_rows, keys.data_ptr(), index.data_ptr(), scratch.data_ptr(), need)
+    _call("lens_sort_tokens", dev, tokens.data_ptr(), size, T, n_rows, keys.data_ptr(), index.data_ptr(), scratch.data_ptr(), need)
     return keys, index
 
 
@@ -583,25 +605,23 @@ def embed_events_grad(grad, tokens, n_rows, weight=None, scale=1.0, table=None, 
 
     Sums are 32-bit and their order is fixed by the tokens: the same call gives the same bits.  order: what
     sort_events(tokens, n_rows) returned, for a program that passes over the same events again."""
-    _need_cuda(grad, "grad")
-    dev = grad.device
-    size = _tokens(tokens, dev)
+    dev = _device(grad, "grad")
     assert grad.dtype in _TYPES and grad.dim() == 2, f"grad must be [T, D] in float32, bfloat16 or float16, got {list(grad.shape)} {grad.dtype}"
     T, D = grad.shape
-    assert tokens.shape[0] == T, f"{tokens.shape[0]} tokens, {T} rows of gradient"
+    _tokens(tokens, T, dev)
     ld = _rows(grad, "grad", T, D, grad.dtype, dev, spread=True)
     w = gw = ldt = None
     if weight is not None:
         assert table is not None, "the gradient of the weights needs the table"
         w = _flat(weight, "weight", T, torch.float32, dev)
         ldt = _rows(table, "table", n_rows, D, grad.dtype, dev)
-        gw = torch.empty((T,), dtype=torch.float32, device=dev)
-    gt = torch.empty((n_rows, D), dtype=torch.float32, device=dev)
+        gw = torch.empty((T,), dtype=torch.float32, device=grad.device)
+    gt = torch.empty((n_rows, D), dtype=torch.float32, device=grad.device)
     keys, index = sort_events(tokens, n_rows) if order is None else order
     k, i = _flat(keys, "order[0]", T, torch.int32, dev), _flat(index, "order[1]", T, torch.int32, dev)
     need = _lib.lib().lens_embed_events_grad_scratch_bytes(_TYPES[grad.dtype], T, n_rows, D)
-    scratch = torch.empty((need,), dtype=torch.uint8, device=dev)
-    _call("lens_embed_events_grad", grad, grad.data_ptr(), _TYPES[grad.dtype], ld, k, i, w, scale, T, n_rows, D,
+    scratch = grad.new_empty((need,), dtype=torch.uint8)
+    _call("lens_embed_events_grad", dev, grad.data_ptr(), _TYPES[grad.dtype], ld, k, i, w, scale, T, n_rows, D,
           _addr(table) if gw is not None else None, ldt or 0, gt.data_ptr(), _addr(gw), scratch.data_ptr(), need)
     return gt, gw
 
@@ -624,10 +644,10 @@ def _sequences(seq_off, T, dev):
         off = np.asarray(seq_off, dtype=np.int64).reshape(-1)
         if off.size < 2 or off[0] < 0 or off[-1] > T or np.any(np.diff(off) < 0):
             raise ValueError(f"seq_off must hold at least two non-decreasing offsets within [0, {T}]")
-        seq_off = torch.from_numpy(np.ascontiguousarray(off)).to(dev)
+        seq_off = torch.from_numpy(np.ascontiguousarray(off)).to(dev if dev >= 0 else "cpu")
     assert seq_off.dtype == torch.int64 and seq_off.dim() == 1 and seq_off.is_contiguous() and seq_off.numel() >= 2, \
         "seq_off must be a contiguous int64 vector of at least two offsets"
-    assert seq_off.device == dev, f"seq_off is on {seq_off.device}, expected {dev}"
+    assert seq_off.get_device() == dev, f"seq_off is on {seq_off.device}, expected device {dev}"
     return seq_off, seq_off.numel() - 1
 
 
@@ -647,8 +667,7 @@ def gated_scan(x, gate=None, dt=None, rate=None, seq_off=None, h0=None, out=None
     Returns (h [T, D] in x's type, last float32 [S, D]), with marks=True also what gated_scan_grad needs of the states.
     Rows of no sequence are zeros in h; in the caller's `out` (which must not overlap the inputs) they are left as they were.
     x and gate may be one row expanded to T."""
-    _need_cuda(x, "x")
-    dev = x.device
+    dev = _device(x, "x")
     assert x.dim() == 2 and x.dtype in _TYPES, f"x must be [T, D] in float32, bfloat16 or float16, got {list(x.shape)} {x.dtype}"
     T, D = x.shape
     ldx = _rows(x, "x", T, D, x.dtype, dev, spread=True)
@@ -657,13 +676,16 @@ def gated_scan(x, gate=None, dt=None, rate=None, seq_off=None, h0=None, out=None
     p0 = None if h0 is None else _flat(h0, "h0", S * D, torch.float32, dev)
     fill = out is None
     if out is None:
-        out = torch.empty((T, D), dtype=x.dtype, device=dev)
-    ldh = _rows(out, "out", T, D, x.dtype, dev)
-    last = torch.empty((S, D), dtype=torch.float32, device=dev)
-    kept = torch.empty((_scan_marks(T, D), D), dtype=torch.float32, device=dev) if marks else None
+        out = x.new_empty((T, D))
+        ldh = D
+    else:
+        ldh = _rows(out, "out", T, D, x.dtype, dev)
+        assert out.data_ptr() != x.data_ptr() and (gate is None or out.data_ptr() != gate.data_ptr()), "out must not be an input"
+    last = x.new_empty((S, D), dtype=torch.float32)
+    kept = x.new_empty((_scan_marks(T, D), D), dtype=torch.float32) if marks else None
     need = _lib.lib().lens_gated_scan_scratch_bytes(T, D, 0)
-    scratch = torch.empty((need,), dtype=torch.uint8, device=dev)
-    _call("lens_gated_scan", x, x.data_ptr(), _TYPES[x.dtype], ldx, g, gtype, ldg, pdt, prate, _addr(off), S, p0, T, D,
+    scratch = x.new_empty((need,), dtype=torch.uint8)
+    _call("lens_gated_scan", dev, x.data_ptr(), _TYPES[x.dtype], ldx, g, gtype, ldg, pdt, prate, _addr(off), S, p0, T, D,
           out.data_ptr(), ldh, int(fill), last.data_ptr(), _addr(kept), scratch.data_ptr(), need)
     return (out, last, kept) if marks else (out, last)
 
@@ -674,8 +696,7 @@ def gated_scan_grad(grad_h, x, marks, gate=None, dt=None, rate=None, seq_off=Non
 
     Returns (grad_x [T, D] in x's type, grad_gate [T, D] in the gate's type or grad_rate float32 [D], grad_h0 float32 [S, D] or
     None where h0 is).  Rows of no sequence get zeros.  There is no gradient for dt, which is recorded."""
-    _need_cuda(x, "x")
-    dev = x.device
+    dev = _device(x, "x")
     assert x.dim() == 2 and x.dtype in _TYPES, f"x must be [T, D] in float32, bfloat16 or float16, got {list(x.shape)} {x.dtype}"
     T, D = x.shape
     ldx = _rows(x, "x", T, D, x.dtype, dev, spread=True)
@@ -685,37 +706,37 @@ def gated_scan_grad(grad_h, x, marks, gate=None, dt=None, rate=None, seq_off=Non
     p0 = None if h0 is None else _flat(h0, "h0", S * D, torch.float32, dev)
     pl = None if grad_last is None else _flat(grad_last, "grad_last", S * D, torch.float32, dev)
     pm = _flat(marks, "marks", _scan_marks(T, D) * D, torch.float32, dev)
-    gx = torch.empty((T, D), dtype=x.dtype, device=dev)
-    ga = torch.empty((T, D), dtype=gate.dtype, device=dev) if gate is not None else None
-    gr = torch.empty((D,), dtype=torch.float32, device=dev) if gate is None else None
-    g0 = None if h0 is None else torch.empty((S, D), dtype=torch.float32, device=dev)
+    gx = x.new_empty((T, D))
+    ga = gate.new_empty((T, D)) if gate is not None else None
+    gr = x.new_empty((D,), dtype=torch.float32) if gate is None else None
+    g0 = None if h0 is None else x.new_empty((S, D), dtype=torch.float32)
     need = _lib.lib().lens_gated_scan_scratch_bytes(T, D, 1)
-    scratch = torch.empty((need,), dtype=torch.uint8, device=dev)
-    _call("lens_gated_scan_grad", x, _addr(grad_h), ldd, pl, x.data_ptr(), _TYPES[x.dtype], ldx, g, gtype, ldg, pdt, prate,
+    scratch = x.new_empty((need,), dtype=torch.uint8)
+    _call("lens_gated_scan_grad", dev, _addr(grad_h), ldd, pl, x.data_ptr(), _TYPES[x.dtype], ldx, g, gtype, ldg, pdt, prate,
           _addr(off), S, p0, pm, T, D, gx.data_ptr(), D, _addr(ga), D, _addr(gr), _addr(g0), scratch.data_ptr(), need)
     return gx, ga if gate is not None else gr, g0
 
 
 def _step(state, x, tokens, weight, scale, gate, dt, rate, out, first_bad):
-    _need_cuda(state, "state")
-    dev = state.device
+    dev = _device(state, "state")
     assert state.dim() == 2, f"state must be [n, D], got {list(state.shape)}"
     n, D = state.shape
     ld = _rows(state, "state", n, D, torch.float32, dev, spread=out is not None)
-    assert x.dtype in _TYPES, f"rows must be float32, bfloat16 or float16, got {x.dtype}"
+    assert x.dtype in _TYPES and x.dim() == 2, f"rows must be [n, D] in float32, bfloat16 or float16, got {list(x.shape)} {x.dtype}"
     if tokens is None:
         size, n_rows, w = 0, 0, None
         ldx = _rows(x, "x", n, D, x.dtype, dev, spread=True)
     else:
-        size, n_rows = _tokens(tokens, dev), x.shape[0]
-        assert tokens.shape[0] == n, f"{tokens.shape[0]} tokens, {n} states"
+        size, n_rows = _tokens(tokens, n, dev), x.shape[0]
         ldx = _rows(x, "table", n_rows, D, x.dtype, dev)
         w = None if weight is None else _flat(weight, "weight", n, torch.float32, dev)
     g, gtype, ldg, pdt, prate = _decay(gate, dt, rate, n, D, x.dtype, dev)
-    out = state if out is None else out
-    ldo = _rows(out, "out", n, D, torch.float32, dev)
-    _call("lens_gated_step", state, state.data_ptr(), ld, x.data_ptr(), _TYPES[x.dtype], ldx, _addr(tokens), size, n_rows, w, scale,
-          g, gtype, ldg, pdt, prate, n, D, out.data_ptr(), ldo, _addr(first_bad))
+    if out is None:
+        out, ldo = state, ld
+    else:
+        ldo = _rows(out, "out", n, D, torch.float32, dev)
+    _call("lens_gated_step", dev, state.data_ptr(), ld, x.data_ptr(), _TYPES[x.dtype], ldx, None if tokens is None else tokens.data_ptr(),
+          size, n_rows, w, scale, g, gtype, ldg, pdt, prate, n, D, out.data_ptr(), ldo, None if first_bad is None else first_bad.data_ptr())
     return out
 
 

@@ -127,9 +127,9 @@ def test_python_callers_refuse_host_tensors_and_wrong_shapes():
             call()
     for off in ([0], [0, 5], [3, 2, 4], [-1, 4]):
         with pytest.raises(ValueError, match="seq_off"):
-            E._sequences(off, 4, torch.device("cpu"))
-    assert E._sequences([0, 2, 4], 4, torch.device("cpu"))[1] == 2 and E._sequences(None, 4, None) == (None, 1)
-    dev = torch.device("cpu")
+            E._sequences(off, 4, -1)
+    assert E._sequences([0, 2, 4], 4, -1)[1] == 2 and E._sequences(None, 4, -1) == (None, 1)
+    dev = -1
     with pytest.raises(AssertionError, match="overlap"):
         E._rows(f[:1].expand(4, 8), "out", 4, 8, torch.float32, dev)
     with pytest.raises(AssertionError, match="contiguous"):
