@@ -386,23 +386,23 @@ int lens_embed_events(const void *d_table, int type, int64_t n_rows, int64_t ld_
                       int64_t *d_first_bad, void *stream);
 
 /*
- * Tokens in ascending order:  d_keys int32 [T] the sorted tokens, d_index int32 [T] where each stood; equal tokens keep their
- * order.  Tokens outside [0, n_rows), padding among them, get the key n_rows and stand behind the others.
+ * Tokens in ascending order:  d_order int64 [T], token << 32 | where it stood; equal tokens keep their order.  Tokens outside
+ * [0, n_rows), padding among them, get n_rows and stand behind the others.
  * Scratch: lens_sort_tokens_scratch_bytes(T, n_rows).
  */
 size_t lens_sort_tokens_scratch_bytes(int64_t T, int64_t n_rows);
-int lens_sort_tokens(const void *d_tokens, int token_bytes, int64_t T, int64_t n_rows, int32_t *d_keys, int32_t *d_index,
+int lens_sort_tokens(const void *d_tokens, int token_bytes, int64_t T, int64_t n_rows, int64_t *d_order,
                      void *d_scratch, size_t scratch_bytes, void *stream);
 
 /*
- * Gradients of lens_embed_events, from the sorted tokens (d_keys, d_index as lens_sort_tokens wrote them):
+ * Gradients of lens_embed_events, from the sorted tokens (d_order as lens_sort_tokens wrote it for these tokens):
  *   grad_table[v] = scale * sum_{i : tokens[i] = v} weight[i] * grad[i]          float [n_rows][D], every row written
  *   grad_weight[i] = scale * <grad[i], table[tokens[i]]>                         float [T], optional; 0 for tokens without a row
  * d_grad type [T][ld_grad] (ld_grad 0: one row for all events); d_table is read for grad_weight only.
  * Sums are 32-bit, in an order that the tokens alone fix.  Scratch: lens_embed_events_grad_scratch_bytes(type, T, n_rows, D).
  */
 size_t lens_embed_events_grad_scratch_bytes(int type, int64_t T, int64_t n_rows, int D);
-int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const int32_t *d_keys, const int32_t *d_index,
+int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const int64_t *d_order,
                            const float *d_weight, float scale, int64_t T, int64_t n_rows, int D, const void *d_table,
                            int64_t ld_table, float *d_grad_table, float *d_grad_weight, void *d_scratch, size_t scratch_bytes,
                            void *stream);

@@ -66,9 +66,9 @@ SIGNATURES = {
                               _i, _i, _i, _c_p]),
     "lens_embed_events": (_i, [_c_p, _i, _l, _l, _c_p, _i, _c_p, _f, _l, _i, _c_p, _l, _c_p, _c_p]),
     "lens_sort_tokens_scratch_bytes": (_z, [_l, _l]),
-    "lens_sort_tokens": (_i, [_c_p, _i, _l, _l, _c_p, _c_p, _c_p, _z, _c_p]),
+    "lens_sort_tokens": (_i, [_c_p, _i, _l, _l, _c_p, _c_p, _z, _c_p]),
     "lens_embed_events_grad_scratch_bytes": (_z, [_i, _l, _l, _i]),
-    "lens_embed_events_grad": (_i, [_c_p, _i, _l, _c_p, _c_p, _c_p, _f, _l, _l, _i, _c_p, _l, _c_p, _c_p, _c_p, _z, _c_p]),
+    "lens_embed_events_grad": (_i, [_c_p, _i, _l, _c_p, _c_p, _f, _l, _l, _i, _c_p, _l, _c_p, _c_p, _c_p, _z, _c_p]),
     "lens_scan_mark_rows": (_i, [_i]),
     "lens_gated_scan_scratch_bytes": (_z, [_l, _i, _i]),
     "lens_gated_scan": (_i, [_c_p, _i, _l, _c_p, _i, _l, _c_p, _c_p, _c_p, _i, _c_p, _l, _i, _c_p, _l, _i, _c_p, _c_p,

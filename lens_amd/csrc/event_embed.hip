@@ -86,94 +86,137 @@ __global__ void __launch_bounds__(256) k_embed(const EmbedArgs p)
 }
 
 // ------------------------------------------------------------------------------------------
-// Sort: stable, least significant digit first, digits of at most SORT_BITS bits.  A pass counts the digits of every
-// block of SORT_BLOCK tokens, adds the counts up for every digit over the blocks, and moves the tokens.
+// Sort: stable, least significant digit first, digits of at most SORT_BITS bits.  An element is token << 32 | position, so the
+// sorted list holds both.  A pass counts the digits of every block, adds the counts up for every digit over the blocks,
+// and moves the elements, through LDS in the order of their digits (elements of one digit leave side by side: 32 bytes
+// and more a digit at once instead of 8).  A short list has smaller blocks, and those add the counts up themselves.
 // Tokens that name no row get the key V_rows and end behind all others.
 // ------------------------------------------------------------------------------------------
-constexpr int SORT_BITS = 9, SORT_THREADS = 256, SORT_EACH = 16, SORT_BLOCK = SORT_THREADS * SORT_EACH;
-constexpr int SORT_WAVES = SORT_THREADS / 64;
+constexpr int SORT_BITS = 9, SORT_THREADS = 256, SORT_WAVES = SORT_THREADS / 64;
+constexpr int SORT_EACH = 16, SORT_EACH_SHORT = 4;           // elements a thread; a short list has more blocks
 
 struct SortArgs {
     const void *tokens;              // first pass: the caller's; else NULL
-    const int32_t *keys, *index;
-    int32_t *keys_out, *index_out;
+    const uint64_t *from;
+    uint64_t *to;
     int32_t *count;                  // [digits][blocks] counts, then what lies before (k_sort_add)
     int32_t *total;                  // [digits]
     int64_t T, V_rows;
     int wide_tokens, shift, bits, blocks;
 };
 
-__device__ __forceinline__ int32_t sort_key(const SortArgs &p, int64_t i)
+__device__ __forceinline__ uint32_t sort_key(const SortArgs &p, int64_t i)
 {
-    if (!p.tokens) return p.keys[i];
+    if (!p.tokens) return (uint32_t)(p.from[i] >> 32);
     const int64_t k = token_at(p.tokens, p.wide_tokens, i);
-    return (int32_t)(k >= 0 && k < p.V_rows ? k : p.V_rows);
+    return (uint32_t)(k >= 0 && k < p.V_rows ? k : p.V_rows);
 }
 
+__device__ __forceinline__ uint64_t sort_element(const SortArgs &p, int64_t i)
+{
+    return p.tokens ? (uint64_t)sort_key(p, i) << 32 | (uint64_t)i : p.from[i];
+}
+
+template <int SORT_EACH>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_count(const SortArgs p)
 {
     __shared__ int n[1 << SORT_BITS];
     const int digits = 1 << p.bits;
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) n[d] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * SORT_BLOCK;
-#pragma unroll 4
-    for (int r = 0; r < SORT_EACH; ++r) {
-        const int64_t i = base + r * SORT_THREADS + threadIdx.x;
-        if (i < p.T) atomicAdd(&n[(sort_key(p, i) >> p.shift) & (digits - 1)], 1);
-    }
+    const int64_t base = (int64_t)blockIdx.x * SORT_THREADS * SORT_EACH + threadIdx.x;
+    uint32_t key[SORT_EACH];
+#pragma unroll
+    for (int r = 0; r < SORT_EACH; ++r) key[r] = base + r * SORT_THREADS < p.T ? sort_key(p, base + r * SORT_THREADS) : 0;
+#pragma unroll
+    for (int r = 0; r < SORT_EACH; ++r)
+        if (base + r * SORT_THREADS < p.T) atomicAdd(&n[(key[r] >> p.shift) & (digits - 1)], 1);
     __syncthreads();
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) p.count[(int64_t)d * p.blocks + blockIdx.x] = n[d];
 }
 
-// One workgroup a digit: counts -> how many tokens of the digit lie in earlier blocks.
-__global__ void __launch_bounds__(256) k_sort_add(int32_t *__restrict__ count, int32_t *__restrict__ total, int blocks)
+// v of every thread -> the sum of those before it; all: the sum of all.
+__device__ __forceinline__ int sum_before(int v, int *part, int &all)
 {
-    __shared__ int part[4];
-    int32_t *row = count + (int64_t)blockIdx.x * blocks;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(s, d, 64);
+        if (lane >= d) s += o;
+    }
+    if (lane == 63) part[wave] = s;
+    __syncthreads();
+    int w = 0;
+    all = 0;
+    for (int k = 0; k < SORT_WAVES; ++k) {
+        if (k < wave) w += part[k];
+        all += part[k];
+    }
+    __syncthreads();
+    return w + s - v;
+}
+
+// One workgroup a digit: counts -> how many elements of the digit lie in earlier blocks.
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_add(int32_t *__restrict__ count, int32_t *__restrict__ total, int blocks)
+{
+    __shared__ int part[SORT_WAVES];
+    int32_t *row = count + (int64_t)blockIdx.x * blocks;
     int before = 0;
-    for (int base = 0; base < blocks; base += 256) {
-        const int i = base + threadIdx.x;
-        const int v = i < blocks ? row[i] : 0;
-        int s = v;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(s, d, 64);
-            if (lane >= d) s += o;
-        }
-        if (lane == 63) part[wave] = s;
-        __syncthreads();
-        int w = 0, all = 0;
-        for (int k = 0; k < 4; ++k) {
-            if (k < wave) w += part[k];
-            all += part[k];
-        }
-        if (i < blocks) row[i] = before + w + s - v;
+    for (int base = 0; base < blocks; base += SORT_THREADS) {
+        const int i = base + threadIdx.x, v = i < blocks ? row[i] : 0;
+        int all;
+        const int s = sum_before(v, part, all);
+        if (i < blocks) row[i] = before + s;
         before += all;
-        __syncthreads();
     }
     if (threadIdx.x == 0) total[blockIdx.x] = before;
 }
 
+template <int EACH, bool SHORT>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
 {
-    __shared__ volatile int n[SORT_WAVES][1 << SORT_BITS];       // a wave's tokens of a digit so far; then where its first one goes
+    constexpr int BLOCK = SORT_THREADS * EACH;
+    __shared__ volatile int n[SORT_WAVES][1 << SORT_BITS];   // a wavefront's elements of a digit so far; then where they start
+    __shared__ int start[1 << SORT_BITS], goes[1 << SORT_BITS];   // a digit's elements: where they start in the block, in the list
+    __shared__ uint64_t sorted[BLOCK];
     __shared__ int part[SORT_WAVES];
     const int digits = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int d = threadIdx.x; d < digits * SORT_WAVES; d += SORT_THREADS) n[d / digits][d % digits] = 0;
-    __syncthreads();
-    // every wave takes 64 x SORT_EACH tokens that follow each other, 64 at a time: their order is the list's
-    const int64_t base = (int64_t)blockIdx.x * SORT_BLOCK + wave * (64 * SORT_EACH);
-    int32_t key[SORT_EACH], rank[SORT_EACH];
-#pragma unroll
-    for (int r = 0; r < SORT_EACH; ++r) {
-        const int64_t i = base + r * 64 + lane;
-        key[r] = i < p.T ? sort_key(p, i) : -1;
+    const int64_t first = (int64_t)blockIdx.x * BLOCK;
+    const int here = p.T - first < BLOCK ? (int)(p.T - first) : BLOCK;
+    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) {
+        for (int k = 0; k < SORT_WAVES; ++k) n[k][d] = 0;
+        start[d] = goes[d] = 0;
     }
+    __syncthreads();
+    if (SHORT) {                                             // start: all elements of a digit; goes: those of earlier blocks
+        for (int d = threadIdx.x; d < digits; d += SORT_THREADS) {
+            const int32_t *row = p.count + (int64_t)d * p.blocks;
+            int all = 0, earlier = 0;
+            for (int k0 = 0; k0 < p.blocks; k0 += 8) {
+                int v[8];
 #pragma unroll
-    for (int r = 0; r < SORT_EACH; ++r) {
-        const bool in = base + r * 64 + lane < p.T;
-        const int d = (key[r] >> p.shift) & (digits - 1);
+                for (int k = 0; k < 8; ++k) v[k] = row[k0 + k < p.blocks ? k0 + k : p.blocks - 1];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    all += k0 + k < p.blocks ? v[k] : 0;
+                    earlier += k0 + k < (int)blockIdx.x ? v[k] : 0;
+                }
+            }
+            start[d] = all;
+            goes[d] = earlier;
+        }
+        __syncthreads();
+    }
+    // every wavefront takes 64 x EACH elements that follow each other, 64 at a time: their order is the list's
+    const int base = wave * (64 * EACH) + lane;
+    uint64_t e[EACH];
+    int rank[EACH];
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) e[r] = base + r * 64 < here ? sort_element(p, first + base + r * 64) : 0;
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+        const bool in = base + r * 64 < here;
+        const int d = (int)(e[r] >> (32 + p.shift)) & (digits - 1);
         uint64_t same = __ballot(in);
         for (int b = 0; b < p.bits; ++b) {
             const uint64_t on = __ballot((d >> b) & 1);
@@ -188,25 +231,19 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
         rank[r] = at + below;
     }
     __syncthreads();
-    // where the first token of every digit goes: those of smaller digits, of earlier blocks, of earlier waves
-    int before = 0;
+    // where a digit's elements go: behind those of smaller digits, of earlier blocks, of earlier wavefronts
+    int before = 0, before_here = 0;
     for (int d0 = 0; d0 < digits; d0 += SORT_THREADS) {
         const int d = d0 + threadIdx.x;
-        const int v = d < digits ? p.total[d] : 0;
-        int s = v;
-        for (int k = 1; k < 64; k <<= 1) {
-            const int o = __shfl_up(s, k, 64);
-            if (lane >= k) s += o;
-        }
-        if (lane == 63) part[wave] = s;
-        __syncthreads();
-        int w = 0, all = 0;
-        for (int k = 0; k < SORT_WAVES; ++k) {
-            if (k < wave) w += part[k];
-            all += part[k];
-        }
+        int mine = 0, all, all_here;
+        if (d < digits)
+            for (int k = 0; k < SORT_WAVES; ++k) mine += n[k][d];
+        const int list = sum_before(d < digits ? (SHORT ? start[d] : p.total[d]) : 0, part, all);
+        const int block = sum_before(mine, part, all_here);
         if (d < digits) {
-            int at = before + w + s - v + p.count[(int64_t)d * p.blocks + blockIdx.x];
+            goes[d] = before + list + (SHORT ? goes[d] : p.count[(int64_t)d * p.blocks + blockIdx.x]);
+            start[d] = before_here + block;
+            int at = before_here + block;
             for (int k = 0; k < SORT_WAVES; ++k) {
                 const int m = n[k][d];
                 n[k][d] = at;
@@ -214,63 +251,69 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
             }
         }
         before += all;
-        __syncthreads();
+        before_here += all_here;
     }
+    __syncthreads();
 #pragma unroll
-    for (int r = 0; r < SORT_EACH; ++r) {
-        const int64_t i = base + r * 64 + lane;
-        if (i >= p.T) continue;
-        const int64_t to = (int64_t)n[wave][(key[r] >> p.shift) & (digits - 1)] + rank[r];
-        p.keys_out[to] = key[r];
-        p.index_out[to] = p.tokens ? (int32_t)i : p.index[i];
+    for (int r = 0; r < EACH; ++r)
+        if (base + r * 64 < here) sorted[n[wave][(int)(e[r] >> (32 + p.shift)) & (digits - 1)] + rank[r]] = e[r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < here; i += SORT_THREADS) {
+        const uint64_t v = sorted[i];
+        const int d = (int)(v >> (32 + p.shift)) & (digits - 1);
+        p.to[(int64_t)goes[d] + (i - start[d])] = v;
     }
 }
 
 // ------------------------------------------------------------------------------------------
 // Gradient.  The sorted tokens and the ends of the rows 0 .. V_rows (the last one: tokens that name no row) merge into one
-// list: token t stands at place t + key[t], the end of row r behind the last token of r.  A workgroup takes GRAD_ITEMS
-// places a group, a group is `G` lanes that hold one row of the table's width, NV vectors each.
+// list: token t stands at place t + key[t], the end of row r behind the last token of r.  A workgroup takes `items` places
+// a group, a group is `G` lanes that hold one row of the table's width, NV vectors each.
 // A row that begins in one group and ends in a later one is joined in LDS, over workgroups by k_grad_join.
 // ------------------------------------------------------------------------------------------
 constexpr int GRAD_ITEMS = 64, GRAD_U = 4;
 
 struct GradArgs {
     const void *grad, *table;
-    const int32_t *keys, *index;
+    const uint64_t *order;
     const float *weight;
     float *out, *grad_weight;
     float *head, *tail;              // [workgroups][D] what a workgroup adds to its first row, and to the one behind its last
+    int64_t *first_row;              // [workgroups] the row of `head`: it began in an earlier workgroup and ends here; else -1
+    int32_t *open;                   // [workgroups] the row behind the last begins here, or there is none
     int64_t T, V_rows, ld_grad, ld_table;
     float scale;
-    int D;
+    int D, items;
 };
 
 // A sorted token and its event, kept inside the table and the list whatever order the caller passed.
-__device__ __forceinline__ int32_t key_at(const GradArgs &p, int64_t t)
+__device__ __forceinline__ int32_t key_of(const GradArgs &p, uint64_t e)
 {
-    const int32_t k = p.keys[t];
-    return k < 0 ? 0 : k < p.V_rows ? k : (int32_t)p.V_rows;
+    const int64_t k = (int64_t)e >> 32;
+    return k < 0 ? 0 : k < p.V_rows ? (int32_t)k : (int32_t)p.V_rows;
 }
 
-__device__ __forceinline__ int32_t event_at(const GradArgs &p, int64_t t)
+__device__ __forceinline__ int32_t event_of(const GradArgs &p, uint64_t e)
 {
-    const int32_t i = p.index[t];
-    return i < 0 ? 0 : i < p.T ? i : (int32_t)(p.T - 1);
+    const int64_t i = (int64_t)(e & 0xffffffffu);
+    return i < p.T ? (int32_t)i : (int32_t)(p.T - 1);
 }
 
-// Tokens among the first `place` places.
+// Tokens among the first `place` places; a wavefront asks for 64 of them at once.
 __device__ __forceinline__ int64_t tokens_before(const GradArgs &p, int64_t place)
 {
-    const int64_t T = p.T;
-    int64_t lo = 0, hi = place < T ? place : T;
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0, hi = place < p.T ? place : p.T;
     while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (mid + key_at(p, mid) < place) lo = mid + 1; else hi = mid;
+        const int64_t step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step - 1;
+        const bool before = at < hi && at + key_of(p, p.order[at < hi ? at : hi - 1]) < place;
+        lo += __builtin_popcountll(__ballot(before)) * step;
+        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
     }
     return lo;
 }
 
-template <int V, int NV, typename X>
+template <int V, int NV>
 struct Row {                         // a lane's share of a row
     vec<float, V> v[NV];
     __device__ __forceinline__ void zero()
@@ -296,35 +339,47 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
 {
     constexpr int NG = 256 / G;
     __shared__ int32_t keys[NG * GRAD_ITEMS], index[NG * GRAD_ITEMS];
-    __shared__ int64_t first[NG + 1];
+    __shared__ int64_t ends[2];
+    __shared__ int32_t before_first;                 // the key before the workgroup's first token, -1: none
     __shared__ int closed[NG], open[NG];
     __shared__ vec<float, V> part[2][NV][256];       // [0] what a group adds to its first row, [1] to the one behind its last
     const int lane = (int)threadIdx.x % G, group = (int)threadIdx.x / G;
-    const int64_t places = p.T + p.V_rows + 1;
-    const int64_t place0 = (int64_t)blockIdx.x * NG * GRAD_ITEMS;
-    if (threadIdx.x <= NG) {
-        const int64_t d = place0 + (int64_t)threadIdx.x * GRAD_ITEMS;
-        first[threadIdx.x] = tokens_before(p, d < places ? d : places);
+    const int64_t places = p.T + p.V_rows + 1, per = (int64_t)NG * p.items;
+    const int64_t place0 = (int64_t)blockIdx.x * per;
+    const int here = places - place0 < per ? (int)(places - place0) : (int)per;
+    if (threadIdx.x < 128) {
+        const int64_t t = tokens_before(p, place0 + (threadIdx.x >> 6 ? here : 0));
+        if ((threadIdx.x & 63) == 0) ends[threadIdx.x >> 6] = t;
+        if (threadIdx.x == 0) before_first = t > 0 ? key_of(p, p.order[t - 1]) : -1;
     }
     __syncthreads();
-    const int64_t t_block = first[0];
-    const int n_block = (int)(first[NG] - t_block);
+    const int64_t t_block = ends[0], r_block = place0 - t_block;
+    const int n_block = (int)(ends[1] - t_block);
     for (int i = threadIdx.x; i < n_block; i += 256) {
-        keys[i] = key_at(p, t_block + i);
-        index[i] = event_at(p, t_block + i);
+        const uint64_t e = p.order[t_block + i];
+        keys[i] = key_of(p, e);
+        index[i] = event_of(p, e);
     }
     __syncthreads();
     int skip[NV], c[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) c[k] = channel<V, G>(k, lane, p.D, skip[k]);
-    const int64_t d0 = place0 + (int64_t)group * GRAD_ITEMS, d1 = d0 + GRAD_ITEMS;
-    const int t0 = (int)(first[group] - t_block), t1 = (int)(first[group + 1] - t_block);
-    int64_t r = (d0 < places ? d0 : places) - first[group];
-    const int64_t r1 = (d1 < places ? d1 : places) - first[group + 1];
-    // the row begins before this group
-    bool begun = first[group] > 0 && (t0 > 0 ? keys[t0 - 1] : key_at(p, first[group] - 1)) == r;
-    const bool begun0 = begun;
-    Row<V, NV, X> acc, head, row;
+    // tokens among the first d places of the workgroup
+    auto among = [&](int d) {
+        int lo = 0, hi = d < n_block ? d : n_block;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (mid + (keys[mid] - r_block) < d) lo = mid + 1; else hi = mid;
+        }
+        return lo;
+    };
+    const int d0 = group * p.items < here ? group * p.items : here, d1 = d0 + p.items < here ? d0 + p.items : here;
+    const int t0 = among(d0), t1 = among(d1);
+    const int64_t r0 = r_block + (d0 - t0), r1 = r_block + (d1 - t1);
+    int64_t r = r0;
+    const bool begun0 = (t0 > 0 ? keys[t0 - 1] : before_first) == r0;     // the row begins before this group
+    bool begun = begun0;
+    Row<V, NV> acc, head, row;
     acc.zero();
     head.zero();
     auto end_row = [&]() {
@@ -395,7 +450,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     }
     __syncthreads();
     if (closed[group]) {
-        Row<V, NV, X> sum;
+        Row<V, NV> sum;
         sum.zero();
         int k0 = group;
         while (k0 > 0 && !open[k0 - 1]) --k0;
@@ -404,8 +459,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
 #pragma unroll
             for (int k = 0; k < NV; ++k) sum.v[k] += part[1][k][q * G + lane];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) sum.v[k] += head.v[k];
-        const int64_t r0 = (d0 < places ? d0 : places) - first[group];
+        for (int k = 0; k < NV; ++k) sum.v[k] += part[0][k][threadIdx.x];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (skip[k] >= V) continue;
@@ -416,7 +470,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     if (group == NG - 1) {
         int q0 = NG - 1;
         while (q0 > 0 && !open[q0]) --q0;
-        Row<V, NV, X> sum;
+        Row<V, NV> sum;
         sum.zero();
         for (int q = q0; q < NG; ++q)
 #pragma unroll
@@ -424,6 +478,12 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
 #pragma unroll
         for (int k = 0; k < NV; ++k)
             if (skip[k] < V) store<V>(p.tail + (int64_t)blockIdx.x * p.D + c[k], sum.v[k]);
+        if (lane == 0) {
+            int k0 = 0;                                               // the first group that closes a row of earlier workgroups
+            while (k0 < NG && !open[k0]) ++k0;
+            p.first_row[blockIdx.x] = k0 < NG && closed[k0] && r_block < p.V_rows ? r_block : -1;
+            p.open[blockIdx.x] = k0 < NG;
+        }
     }
 }
 
@@ -434,21 +494,23 @@ __global__ void __launch_bounds__(256) k_grad_join(const GradArgs p)
 {
     constexpr int NG = 256 / G;
     __shared__ vec<float, V> part[NV][256];
-    const int lane = (int)threadIdx.x % G, group = (int)threadIdx.x / G;
-    const int64_t per = (int64_t)NG * GRAD_ITEMS, places = p.T + p.V_rows + 1;
-    const int64_t d0 = (int64_t)blockIdx.x * per, d1 = d0 + per < places ? d0 + per : places;
-    const int64_t t0 = tokens_before(p, d0);
-    const int64_t r = d0 - t0;
-    if (t0 == 0 || key_at(p, t0 - 1) != r || r >= p.V_rows) return;          // no row of earlier workgroups
-    if (d1 - tokens_before(p, d1) == r) return;                  // it ends in a later one
-    int64_t lo = 0, hi = t0;                                               // its first token
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (key_at(p, mid) < r) lo = mid + 1; else hi = mid;
+    __shared__ int nearest;
+    const int lane = (int)threadIdx.x % G, group = (int)threadIdx.x / G, block = blockIdx.x;
+    const int64_t r = p.first_row[block];
+    if (r < 0) return;
+    int b0 = -1;                                                      // where the row begins: the nearest earlier one that is open
+    for (int top = block - 1; top >= 0 && b0 < 0; top -= 256) {
+        if (threadIdx.x == 0) nearest = -1;
+        __syncthreads();
+        const int q = top - (int)threadIdx.x;
+        if (q >= 0 && p.open[q]) atomicMax(&nearest, q);
+        __syncthreads();
+        b0 = nearest;
+        __syncthreads();
     }
-    const int64_t b0 = (lo + r) / per, n = blockIdx.x - b0;
-    const int64_t each = (n + NG - 1) / NG;
-    const int64_t q0 = b0 + group * each, q1 = q0 + each < blockIdx.x ? q0 + each : blockIdx.x;
+    if (b0 < 0) b0 = 0;
+    const int n = block - b0, each = (n + NG - 1) / NG;
+    const int q0 = b0 + group * each < block ? b0 + group * each : block, q1 = q0 + each < block ? q0 + each : block;
     vec<float, V> sum[NV];
     int c[NV], skip[NV];
 #pragma unroll
@@ -467,7 +529,7 @@ __global__ void __launch_bounds__(256) k_grad_join(const GradArgs p)
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         for (int q = 1; q < NG; ++q) sum[k] += part[k][q * G + lane];
-        sum[k] += load<V>(p.head + (int64_t)blockIdx.x * p.D + c[k]);
+        sum[k] += load<V>(p.head + (int64_t)block * p.D + c[k]);
         if (skip[k] < V) store<V>(p.out + r * p.D + c[k], sum[k]);
     }
 }
@@ -497,9 +559,12 @@ Width width_of(int type, int D)
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// A list of this many tokens at most is short (64 blocks, whose counts every block adds up: 256 bytes a digit).
+constexpr int64_t SORT_SHORT = 64 * SORT_THREADS * SORT_EACH_SHORT;
+
 struct SortPlan {
     int bits, passes, blocks;
-    size_t keys, index, count, total, bytes;
+    size_t other, count, total, bytes;
 };
 
 SortPlan sort_plan(int64_t T, int64_t V_rows)
@@ -509,20 +574,33 @@ SortPlan sort_plan(int64_t T, int64_t V_rows)
     while (bits < 31 && (V_rows >> bits) != 0) ++bits;
     s.passes = (bits + SORT_BITS - 1) / SORT_BITS;
     s.bits = (bits + s.passes - 1) / s.passes;
-    s.blocks = (int)((T + SORT_BLOCK - 1) / SORT_BLOCK);
-    s.keys = 0;
-    s.index = up((size_t)T * 4);
-    s.count = s.index + up((size_t)T * 4);
+    const int64_t block = (int64_t)SORT_THREADS * (T <= SORT_SHORT ? SORT_EACH_SHORT : SORT_EACH);
+    s.blocks = (int)((T + block - 1) / block);
+    s.other = 0;
+    s.count = up((size_t)T * 8);
     s.total = s.count + up((size_t)s.blocks * 4 << s.bits);
     s.bytes = s.total + up((size_t)4 << s.bits);
     return s;
 }
 
+// Places a group of k_grad: as many as leave 1024 workgroups, 8 at least.
+int grad_items(int64_t T, int64_t V_rows, int G)
+{
+    int items = GRAD_ITEMS;
+    while (items > 8 && T + V_rows + 1 < (int64_t)1024 * (256 / G) * items) items /= 2;
+    return items;
+}
+
+int64_t grad_blocks(int64_t T, int64_t V_rows, int G)
+{
+    const int64_t per = (int64_t)(256 / G) * grad_items(T, V_rows, G);
+    return (T + V_rows + 1 + per - 1) / per;
+}
+
 template <int V, int NV, int G, typename X>
 int launch_grad(const GradArgs &p, hipStream_t st)
 {
-    const int64_t per = (int64_t)(256 / G) * GRAD_ITEMS;
-    const dim3 grid((unsigned)((p.T + p.V_rows + 1 + per - 1) / per)), block(256);
+    const dim3 grid((unsigned)grad_blocks(p.T, p.V_rows, G)), block(256);
     if (p.grad_weight) hipLaunchKernelGGL((k_grad<V, NV, G, X, true>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((k_grad<V, NV, G, X, false>), grid, block, 0, st, p);
     hipLaunchKernelGGL((k_grad_join<V, NV, G>), grid, block, 0, st, p);
@@ -595,32 +673,37 @@ size_t lens_sort_tokens_scratch_bytes(int64_t T, int64_t n_rows)
     return sort_plan(T, n_rows).bytes;
 }
 
-int lens_sort_tokens(const void *d_tokens, int token_bytes, int64_t T, int64_t n_rows, int32_t *d_keys, int32_t *d_index,
+int lens_sort_tokens(const void *d_tokens, int token_bytes, int64_t T, int64_t n_rows, int64_t *d_order,
                      void *d_scratch, size_t scratch_bytes, void *stream)
 {
     if (T < 0 || T > LENS_EMBED_MAX_TOKENS || n_rows < 0 || n_rows > LENS_EMBED_MAX_ROWS || (token_bytes != 4 && token_bytes != 8))
         return LENS_ERR_SIZE;
     if (T == 0) return LENS_OK;
-    if (!d_tokens || !d_keys || !d_index || !d_scratch) return LENS_ERR_NULL;
-    if (((uintptr_t)d_tokens & (token_bytes - 1)) || (((uintptr_t)d_keys | (uintptr_t)d_index) & 3) || ((uintptr_t)d_scratch & 15))
-        return LENS_ERR_ALIGN;
+    if (!d_tokens || !d_order || !d_scratch) return LENS_ERR_NULL;
+    if (((uintptr_t)d_tokens & (token_bytes - 1)) || ((uintptr_t)d_order & 7) || ((uintptr_t)d_scratch & 15)) return LENS_ERR_ALIGN;
     const SortPlan s = sort_plan(T, n_rows);
     if (scratch_bytes < s.bytes) return LENS_ERR_SCRATCH;
     unsigned char *base = (unsigned char *)d_scratch;
-    int32_t *keys[2] = {(int32_t *)(base + s.keys), d_keys}, *index[2] = {(int32_t *)(base + s.index), d_index};
+    uint64_t *list[2] = {(uint64_t *)(base + s.other), (uint64_t *)d_order};
     SortArgs p = {};
     p.count = (int32_t *)(base + s.count); p.total = (int32_t *)(base + s.total);
     p.T = T; p.V_rows = n_rows; p.wide_tokens = token_bytes == 8; p.bits = s.bits; p.blocks = s.blocks;
     hipStream_t st = (hipStream_t)stream;
+    const dim3 grid(s.blocks), block(SORT_THREADS);
     for (int i = 0; i < s.passes; ++i) {
-        const int to = (s.passes - 1 - i) & 1 ? 0 : 1;                 // the last pass writes the caller's arrays
+        const int to = (s.passes - 1 - i) & 1 ? 0 : 1;                 // the last pass writes the caller's list
         p.tokens = i == 0 ? d_tokens : nullptr;
-        p.keys = keys[to ^ 1]; p.index = index[to ^ 1];
-        p.keys_out = keys[to]; p.index_out = index[to];
+        p.from = list[to ^ 1];
+        p.to = list[to];
         p.shift = i * s.bits;
-        hipLaunchKernelGGL(k_sort_count, dim3(s.blocks), dim3(SORT_THREADS), 0, st, p);
-        hipLaunchKernelGGL(k_sort_add, dim3(1 << s.bits), dim3(256), 0, st, p.count, p.total, s.blocks);
-        hipLaunchKernelGGL(k_sort_move, dim3(s.blocks), dim3(SORT_THREADS), 0, st, p);
+        if (T <= SORT_SHORT) {
+            hipLaunchKernelGGL(k_sort_count<SORT_EACH_SHORT>, grid, block, 0, st, p);
+            hipLaunchKernelGGL((k_sort_move<SORT_EACH_SHORT, true>), grid, block, 0, st, p);
+        } else {
+            hipLaunchKernelGGL(k_sort_count<SORT_EACH>, grid, block, 0, st, p);
+            hipLaunchKernelGGL(k_sort_add, dim3(1 << s.bits), block, 0, st, p.count, p.total, s.blocks);
+            hipLaunchKernelGGL((k_sort_move<SORT_EACH, false>), grid, block, 0, st, p);
+        }
     }
     return (int)hipGetLastError();
 }
@@ -630,11 +713,11 @@ size_t lens_embed_events_grad_scratch_bytes(int type, int64_t T, int64_t n_rows,
     if (!type_ok(type) || T < 0 || T > LENS_EMBED_MAX_TOKENS || n_rows < 0 || n_rows > LENS_EMBED_MAX_ROWS || D < 1 ||
         D > LENS_EMBED_MAX_DIM)
         return 0;
-    const int64_t per = (int64_t)(256 / width_of(type, D).G) * GRAD_ITEMS;
-    return 2 * up((size_t)((T + n_rows + 1 + per - 1) / per) * D * 4);
+    const size_t blocks = (size_t)grad_blocks(T, n_rows, width_of(type, D).G);
+    return 2 * up(blocks * D * 4) + up(blocks * 8) + up(blocks * 4);
 }
 
-int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const int32_t *d_keys, const int32_t *d_index,
+int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const int64_t *d_order,
                            const float *d_weight, float scale, int64_t T, int64_t n_rows, int D, const void *d_table,
                            int64_t ld_table, float *d_grad_table, float *d_grad_weight, void *d_scratch, size_t scratch_bytes,
                            void *stream)
@@ -643,19 +726,23 @@ int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const 
     if (T < 0 || T > LENS_EMBED_MAX_TOKENS || D < 1 || D > LENS_EMBED_MAX_DIM || n_rows < 0 || n_rows > LENS_EMBED_MAX_ROWS)
         return LENS_ERR_SIZE;
     if (T == 0 && n_rows == 0) return LENS_OK;
-    if (!d_scratch || (n_rows > 0 && !d_grad_table) || (T > 0 && (!d_grad || !d_keys || !d_index))) return LENS_ERR_NULL;
+    if (!d_scratch || (n_rows > 0 && !d_grad_table) || (T > 0 && (!d_grad || !d_order))) return LENS_ERR_NULL;
     if (d_grad_weight && n_rows > 0 && !d_table) return LENS_ERR_NULL;
     if ((T > 1 && ld_grad != 0 && ld_grad < D) || (d_grad_weight && n_rows > 1 && ld_table < D)) return LENS_ERR_SIZE;
-    if (off_element(d_grad, type) || off_element(d_table, type) || ((uintptr_t)d_scratch & 15) ||
-        (((uintptr_t)d_keys | (uintptr_t)d_index | (uintptr_t)d_weight | (uintptr_t)d_grad_table | (uintptr_t)d_grad_weight) & 3))
+    if (off_element(d_grad, type) || off_element(d_table, type) || ((uintptr_t)d_scratch & 15) || ((uintptr_t)d_order & 7) ||
+        (((uintptr_t)d_weight | (uintptr_t)d_grad_table | (uintptr_t)d_grad_weight) & 3))
         return LENS_ERR_ALIGN;
     const size_t need = lens_embed_events_grad_scratch_bytes(type, T, n_rows, D);
     if (scratch_bytes < need) return LENS_ERR_SCRATCH;
     GradArgs p = {};
-    p.grad = d_grad; p.table = d_table; p.keys = d_keys; p.index = d_index; p.weight = d_weight; p.out = d_grad_table;
-    p.grad_weight = d_grad_weight; p.head = (float *)d_scratch; p.tail = (float *)((unsigned char *)d_scratch + need / 2);
-    p.T = T; p.V_rows = n_rows; p.ld_grad = ld_grad; p.ld_table = ld_table; p.scale = scale; p.D = D;
     const Width w = width_of(type, D);
+    const size_t blocks = (size_t)grad_blocks(T, n_rows, w.G);
+    unsigned char *base = (unsigned char *)d_scratch;
+    p.grad = d_grad; p.table = d_table; p.order = (const uint64_t *)d_order; p.weight = d_weight; p.out = d_grad_table;
+    p.grad_weight = d_grad_weight; p.head = (float *)base; p.tail = (float *)(base + up(blocks * D * 4));
+    p.first_row = (int64_t *)(base + 2 * up(blocks * D * 4)); p.open = (int32_t *)(base + 2 * up(blocks * D * 4) + up(blocks * 8));
+    p.items = grad_items(T, n_rows, w.G);
+    p.T = T; p.V_rows = n_rows; p.ld_grad = ld_grad; p.ld_table = ld_table; p.scale = scale; p.D = D;
     hipStream_t st = (hipStream_t)stream;
     if (type == LENS_F32) return w.V == 4 ? grad_by_width<4, float>(w, p, st) : grad_by_width<1, float>(w, p, st);
     if (type == LENS_BF16) return w.V == 8 ? grad_by_width<8, __bf16>(w, p, st) : grad_by_width<1, __bf16>(w, p, st);

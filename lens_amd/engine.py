@@ -586,17 +586,16 @@ def embed_events(table, tokens, weight=None, scale=1.0, out=None, check=True):
 
 
 def sort_events(tokens, n_rows):
-    """The tokens in ascending order (int32 [T]; equal ones keep their order) and where each stood (int32 [T]).  Tokens outside
-    [0, n_rows), padding among them, come last as n_rows."""
+    """The events sorted by token: int64 [T], token << 32 | position; equal tokens keep their order.  Tokens outside [0, n_rows),
+    padding among them, come last with n_rows in their place."""
     dev = _device(tokens, "tokens")
     T = tokens.shape[0] if tokens.dim() else -1
     size = _tokens(tokens, T, dev)
-    keys = torch.empty((T,), dtype=torch.int32, device=tokens.device)
-    index = torch.empty((T,), dtype=torch.int32, device=tokens.device)
+    order = tokens.new_empty((T,), dtype=torch.int64)
     need = _lib.lib().lens_sort_tokens_scratch_bytes(T, n_rows)
-    scratch = torch.empty((need,), dtype=torch.uint8, device=tokens.device)
-    _call("lens_sort_tokens", dev, tokens.data_ptr(), size, T, n_rows, keys.data_ptr(), index.data_ptr(), scratch.data_ptr(), need)
-    return keys, index
+    scratch = tokens.new_empty((need,), dtype=torch.uint8)
+    _call("lens_sort_tokens", dev, tokens.data_ptr(), size, T, n_rows, order.data_ptr(), scratch.data_ptr(), need)
+    return order
 
 
 def embed_events_grad(grad, tokens, n_rows, weight=None, scale=1.0, table=None, order=None):
@@ -617,11 +616,12 @@ def embed_events_grad(grad, tokens, n_rows, weight=None, scale=1.0, table=None, 
         ldt = _rows(table, "table", n_rows, D, grad.dtype, dev)
         gw = torch.empty((T,), dtype=torch.float32, device=grad.device)
     gt = torch.empty((n_rows, D), dtype=torch.float32, device=grad.device)
-    keys, index = sort_events(tokens, n_rows) if order is None else order
-    k, i = _flat(keys, "order[0]", T, torch.int32, dev), _flat(index, "order[1]", T, torch.int32, dev)
+    if order is None:
+        order = sort_events(tokens, n_rows)
+    po = _flat(order, "order", T, torch.int64, dev)
     need = _lib.lib().lens_embed_events_grad_scratch_bytes(_TYPES[grad.dtype], T, n_rows, D)
     scratch = grad.new_empty((need,), dtype=torch.uint8)
-    _call("lens_embed_events_grad", dev, grad.data_ptr(), _TYPES[grad.dtype], ld, k, i, w, scale, T, n_rows, D,
+    _call("lens_embed_events_grad", dev, grad.data_ptr(), _TYPES[grad.dtype], ld, po, w, scale, T, n_rows, D,
           _addr(table) if gw is not None else None, ldt or 0, gt.data_ptr(), _addr(gw), scratch.data_ptr(), need)
     return gt, gw
 

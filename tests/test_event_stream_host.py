@@ -37,23 +37,23 @@ def test_lookup_refusals(L):
 
 def test_sort_and_table_gradient_refusals(L):
     need = L.lens_sort_tokens_scratch_bytes(100, 50)
-    ok = dict(tokens=P, size=4, T=100, n_rows=50, keys=P, index=P, scratch=P, bytes=need, stream=None)
+    ok = dict(tokens=P, size=4, T=100, n_rows=50, order=P, scratch=P, bytes=need, stream=None)
 
     def sort(**kw):
         return L.lens_sort_tokens(*{**ok, **kw}.values())
     assert sort(T=0) == 0
-    assert sort(tokens=None) == NULL and sort(keys=None) == NULL and sort(index=None) == NULL and sort(scratch=None) == NULL
+    assert sort(tokens=None) == NULL and sort(order=None) == NULL and sort(order=P + 4) == ALIGN and sort(scratch=None) == NULL
     assert sort(size=3) == SIZE and sort(T=-1) == SIZE and sort(n_rows=2**31) == SIZE
     assert sort(scratch=P + 8) == ALIGN and sort(bytes=need - 1) == SCRATCH
     assert L.lens_sort_tokens_scratch_bytes(-1, 5) == 0 and need >= 100 * 8
     need = L.lens_embed_events_grad_scratch_bytes(1, 100, 50, 64)
-    ok_g = dict(grad=P, type=1, ld=64, keys=P, index=P, weight=None, scale=1.0, T=100, n_rows=50, D=64, table=None, ldt=0, gt=P,
+    ok_g = dict(grad=P, type=1, ld=64, order=P, weight=None, scale=1.0, T=100, n_rows=50, D=64, table=None, ldt=0, gt=P,
                 gw=None, scratch=P, bytes=need, stream=None)
 
     def grad(**kw):
         return L.lens_embed_events_grad(*{**ok_g, **kw}.values())
     assert grad(T=0, n_rows=0) == 0
-    for bad in (dict(grad=None), dict(keys=None), dict(index=None), dict(gt=None), dict(scratch=None), dict(gw=P)):
+    for bad in (dict(grad=None), dict(order=None), dict(gt=None), dict(scratch=None), dict(gw=P)):
         assert grad(**bad) == NULL, bad
     for bad in (dict(ld=63), dict(D=0), dict(D=2049), dict(gw=P, table=P, ldt=63), dict(T=-1)):
         assert grad(**bad) == SIZE, bad
