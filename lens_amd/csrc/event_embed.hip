@@ -34,6 +34,15 @@ __device__ __forceinline__ void store(T *p, vec<float, V> v)
     __builtin_memcpy(p, &r, sizeof(T) * V);
 }
 
+// Past the caches: for what is written once and not read here.
+template <int V, typename T>
+__device__ __forceinline__ void store_past(T *p, vec<float, V> v)
+{
+    typedef vec<T, V> __attribute__((aligned(sizeof(T)))) U;
+    const vec<T, V> r = __builtin_convertvector(v, vec<T, V>);
+    __builtin_nontemporal_store(r, reinterpret_cast<U *>(p));
+}
+
 __device__ __forceinline__ int64_t token_at(const void *tokens, int wide_tokens, int64_t i)
 {
     return wide_tokens ? ((const int64_t *)tokens)[i] : (int64_t)((const int32_t *)tokens)[i];
@@ -81,7 +90,7 @@ __global__ void __launch_bounds__(256) k_embed(const EmbedArgs p)
     for (int u = 0; u < EMBED_U; ++u) {
         const int64_t i = i0 + u * p.rows;
         if (i >= p.T) continue;
-        store<V>((X *)p.out + i * p.ld_out + c, ok[u] ? wide<V, X>(v[u]) * f[u] : vec<float, V>(0.0f));
+        store_past<V>((X *)p.out + i * p.ld_out + c, ok[u] ? wide<V, X>(v[u]) * f[u] : vec<float, V>(0.0f));
     }
 }
 
@@ -389,7 +398,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
         } else if (r < p.V_rows) {
 #pragma unroll
             for (int k = 0; k < NV; ++k)
-                if (skip[k] < V) store<V>(p.out + r * p.D + c[k], acc.v[k]);
+                if (skip[k] < V) store_past<V>(p.out + r * p.D + c[k], acc.v[k]);
         }
         acc.zero();
         ++r;

@@ -52,6 +52,15 @@ __device__ __forceinline__ void store(T *p, vec<float, V> v)
     __builtin_memcpy(p, &r, sizeof(T) * V);
 }
 
+// Past the caches: for what is written once and not read here.
+template <int V, typename T>
+__device__ __forceinline__ void store_past(T *p, vec<float, V> v)
+{
+    typedef vec<T, V> __attribute__((aligned(sizeof(T)))) U;
+    const vec<T, V> r = __builtin_convertvector(v, vec<T, V>);
+    __builtin_nontemporal_store(r, reinterpret_cast<U *>(p));
+}
+
 // Element `at` behind a pointer that all lanes share: 32 bits of address a lane.
 template <typename T>
 __device__ __forceinline__ T *behind(T *base, uint32_t at)
@@ -120,18 +129,6 @@ struct ScanArgs {
 };
 
 // ------------------------------------------------------------------------------------------ rows, tiles, sequences
-// A tile's first row; rows of the tile are counted from it.  s_lo, s_hi: offsets up to its first, its last row.
-struct Tile {
-    int64_t row0;
-    int left;                          // rows from there to the end, FAR at most
-    int s_lo, s_hi;
-    __device__ __forceinline__ int rel(int64_t row) const
-    {
-        const int64_t d = row - row0;
-        return d > FAR ? FAR : d < -FAR ? -FAR : (int)d;
-    }
-};
-
 // How many of the n offsets are at most `row`: a wavefront asks for 64 at once.
 __device__ __forceinline__ int offsets_up_to(const int64_t *off, int n, int64_t row)
 {
@@ -146,30 +143,50 @@ __device__ __forceinline__ int offsets_up_to(const int64_t *off, int n, int64_t 
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// All threads call it; ends with a barrier.
-__device__ __forceinline__ Tile tile_of(const ScanArgs &p, int index)
-{
-    __shared__ int found[2];
-    Tile t;
-    const int rows = p.ts * p.run;
-    t.row0 = (int64_t)index * rows;
-    const int64_t n = p.T - t.row0;
-    t.left = n < FAR ? (int)n : FAR;
-    t.s_lo = t.s_hi = 1;
-    if (p.off) {
-        const int wave = (int)threadIdx.x >> 6, last = blockDim.x > 64 ? 1 : 0;
-        for (int q = wave; q < 2; q += last + 1)
-            if (q == wave || !last) {
-                const int f = offsets_up_to(p.off, p.n_seq + 1, q ? t.row0 + rows - 1 : t.row0);
-                if ((threadIdx.x & 63) == 0) found[q] = f;
-            }
-        __syncthreads();
-        t.s_lo = __builtin_amdgcn_readfirstlane(found[0]);
-        t.s_hi = __builtin_amdgcn_readfirstlane(found[1]);
+// A tile's first row; rows of the tile are counted from it.  off: the offsets, in LDS where they are few; s_lo, s_hi: how many of
+// them are at most the tile's first, its last row (or wider).
+constexpr int FEW_OFFSETS = 256;
+
+struct Tile {
+    int64_t row0;
+    int left;                          // rows from there to the end, FAR at most
+    int s_lo, s_hi;
+    const int64_t *off;
+    __device__ __forceinline__ Tile(const ScanArgs &p, int index) : s_lo(1), s_hi(1), off(p.off)
+    {
+        row0 = (int64_t)index * (p.ts * p.run);
+        const int64_t n = p.T - row0;
+        left = n < FAR ? (int)n : FAR;
     }
-    __syncthreads();
-    return t;
-}
+    // before any row is located; all threads call it
+    __device__ __forceinline__ void find(const ScanArgs &p)
+    {
+        __shared__ int64_t few[FEW_OFFSETS];
+        __shared__ int found[2];
+        if (!p.off) return;
+        if (p.n_seq < FEW_OFFSETS) {
+            for (int i = (int)threadIdx.x; i <= p.n_seq; i += blockDim.x) few[i] = p.off[i];
+            off = few;
+            s_lo = 0;
+            s_hi = p.n_seq + 1;
+            __syncthreads();
+            return;
+        }
+        const int wave = (int)threadIdx.x >> 6;
+        for (int q = wave; q < 2; q += blockDim.x > 64 ? 2 : 1) {
+            const int f = offsets_up_to(p.off, p.n_seq + 1, q ? row0 + p.ts * p.run - 1 : row0);
+            if ((threadIdx.x & 63) == 0) found[q] = f;
+        }
+        __syncthreads();
+        s_lo = __builtin_amdgcn_readfirstlane(found[0]);
+        s_hi = __builtin_amdgcn_readfirstlane(found[1]);
+    }
+    __device__ __forceinline__ int rel(int64_t row) const
+    {
+        const int64_t d = row - row0;
+        return d > FAR ? FAR : d < -FAR ? -FAR : (int)d;
+    }
+};
 
 // Where a row lies.  s: its sequence (-1: before the first, n_seq: behind the last), next: where the following one starts.
 struct Place {
@@ -184,18 +201,18 @@ __device__ __forceinline__ Place locate(const ScanArgs &p, const Tile &tile, int
     int lo = tile.s_lo, hi = tile.s_hi;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (p.off[mid] <= row) lo = mid + 1; else hi = mid;
+        if (tile.off[mid] <= row) lo = mid + 1; else hi = mid;
     }
     const int s = lo - 1;
-    return {s, s < p.n_seq ? tile.rel(p.off[s + 1]) : FAR, s >= 0 && s < p.n_seq, s >= 0 && p.off[s] == row};
+    return {s, s < p.n_seq ? tile.rel(tile.off[s + 1]) : FAR, s >= 0 && s < p.n_seq, s >= 0 && tile.off[s] == row};
 }
 
 __device__ __forceinline__ void advance(const ScanArgs &p, const Tile &tile, Place &w, int t)      // t == w.next
 {
     ++w.s;
-    while (w.s < p.n_seq && p.off[w.s + 1] <= tile.row0 + t) ++w.s;                                // sequences without rows
+    while (w.s < p.n_seq && tile.off[w.s + 1] <= tile.row0 + t) ++w.s;                                // sequences without rows
     w.live = w.s < p.n_seq;
-    w.next = w.live ? tile.rel(p.off[w.s + 1]) : FAR;
+    w.next = w.live ? tile.rel(tile.off[w.s + 1]) : FAR;
 }
 
 template <int V>
@@ -567,12 +584,12 @@ __device__ __forceinline__ vec<float, V> run_entry(const ScanArgs &p, const Lds<
         const int slot = (int)threadIdx.x, c = slot < lds.slots ? slot_channel<V>(p, y, slot) : -1;
         if (c >= 0) {
             float h = 0.0f;
-            for (int b = 0; b < order; b += 8) {
-                float2 v[8];
+            for (int b = 0; b < order; b += 16) {
+                float2 v[16];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = p.agg[(int64_t)(b + k < order ? b + k : order - 1) * p.D + c];
+                for (int k = 0; k < 16; ++k) v[k] = p.agg[(int64_t)(b + k < order ? b + k : order - 1) * p.D + c];
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < 16; ++k)
                     if (b + k < order) h = Pair<G>{v[k].x, v[k].y}.over(h);
             }
             lds.f[slot] = h;
@@ -601,19 +618,24 @@ __global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
 {
     const Lds<V> lds(p);
     const int index = blockIdx.x, y = blockIdx.y;
-    const Tile tile = tile_of(p, index);
+    Tile tile(p, index);
     const Own<V> o(p, tile, y);
     int *ids = lds.ids + o.ts * 16;
     Gates<V, B, G> g(p, o.c);
+    Raw<V, B, X> x;
     vec<float, V> H(0.0f);
     bool mark = false;
+    auto load_batch = [&](int b) {
+        x.load_rows((const X *)p.x, p.ldx, o.t0 + b, o.c, tile);
+        g.load_rows(p, o.t0 + b, o.c, tile);
+    };
+    if (o.n > 0) load_batch(0);
+    tile.find(p);
     if (o.n > 0) {
         Place w = locate(p, tile, o.t0);
 #pragma unroll 1
         for (int b = 0; b < o.n; b += B) {
-            Raw<V, B, X> x;
-            x.load_rows((const X *)p.x, p.ldx, o.t0 + b, o.c, tile);
-            g.load_rows(p, o.t0 + b, o.c, tile);
+            if (b) load_batch(b);
             const Rows r = rows_of<B>(p, tile, w, o.t0 + b, ids);
             mark |= r.starts != 0;
             if (__all(r.plain && g.near)) {
@@ -654,11 +676,17 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
             for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x) p.last[c] = p.h0 ? p.h0[c] : 0.0f;
         return;
     }
-    const Tile tile = tile_of(p, index);
+    Tile tile(p, index);
     const Own<V> o(p, tile, y);
     int *ids = lds.ids + o.ts * 16;
     Gates<V, B, G> g(p, o.c);
     Raw<V, B, X> x;
+    auto load_batch = [&](int b) {
+        x.load_rows((const X *)p.x, p.ldx, o.t0 + b, o.c, tile);
+        g.load_rows(p, o.t0 + b, o.c, tile);
+    };
+    if (o.n > 0) load_batch(0);
+    tile.find(p);
     vec<float, V> st = run_entry<V, G>(p, lds, o, index, y, index);
     if (!o.any || o.n == 0) return;
     Place w = locate(p, tile, o.t0);
@@ -666,8 +694,7 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
 #pragma unroll 1
     for (int b = 0; b < o.n; b += B) {
         const int t = o.t0 + b;
-        x.load_rows((const X *)p.x, p.ldx, t, o.c, tile);
-        g.load_rows(p, t, o.c, tile);
+        if (b) load_batch(b);
         const Rows r = rows_of<B>(p, tile, w, t, ids);
         float *mark = p.marks ? p.marks + (tile.row0 + t) / MARK_ROWS * p.D + o.c : nullptr;
         const uint32_t at = (uint32_t)(t * p.ldh + o.c);
@@ -676,7 +703,7 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
             for (int j = 0; j < B; ++j) {
                 if (j % MARK_ROWS == 0 && mark) store<V>(mark + j / MARK_ROWS * p.D, st);
                 st = g.template step<true>(j, st, x[j]);
-                store<V>(behind(out, at + j * p.ldh), st);
+                store_past<V>(behind(out, at + j * p.ldh), st);
                 pace();
             }
         } else {
@@ -687,7 +714,7 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
                 if (j % MARK_ROWS == 0 && mark && (in >> j & 1)) store<V>(mark + j / MARK_ROWS * p.D, st);
                 if (r.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
                 st = g.template step<false>(j, st, x[j]);
-                if (written >> j & 1) store<V>(behind(out, at + j * p.ldh), r.lives >> j & 1 ? st : vec<float, V>(0.0f));
+                if (written >> j & 1) store_past<V>(behind(out, at + j * p.ldh), r.lives >> j & 1 ? st : vec<float, V>(0.0f));
                 if (r.ends >> j & 1) store<V>(p.last + (int64_t)ids[j] * p.D + o.c, st);
                 pace();
             }
@@ -705,19 +732,24 @@ __global__ void __launch_bounds__(256) k_scan_back_pairs(const ScanArgs p)
 {
     const Lds<V> lds(p);
     const int index = blockIdx.x, y = blockIdx.y;
-    const Tile tile = tile_of(p, index);
+    Tile tile(p, index);
     const Own<V> o(p, tile, y);
     int *ids = lds.ids + o.ts * 16;
     Gates<V, B, G> g(p, o.c);
+    Raw<V, B, X> d;
     vec<float, V> U(0.0f);
     bool mark = false;
-#pragma unroll 1
-    for (int b = p.run - B; b >= 0; b -= B) {
-        if (b >= o.n) continue;
-        Raw<V, B, X> d;
+    auto load_batch = [&](int b) {
         g.load_rows(p, o.t0 + b, o.c, tile);
         if (p.grad) d.load_rows((const X *)p.grad, p.ld_grad, o.t0 + b, o.c, tile);
         else d.zero();
+    };
+    const int last = o.n > 0 ? (o.n - 1) & ~(B - 1) : -1;           // the run's last batch; -1: no rows
+    if (last >= 0) load_batch(last);
+    tile.find(p);
+#pragma unroll 1
+    for (int b = last; b >= 0; b -= B) {
+        if (b != last) load_batch(b);
         Place w = locate(p, tile, o.t0 + b);
         const Rows r = rows_of<B>(p, tile, w, o.t0 + b, ids);
         mark |= r.ends != 0;
@@ -761,16 +793,16 @@ __global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
         }
         return;
     }
-    const Tile tile = tile_of(p, index);
+    Tile tile(p, index);
     const Own<V> o(p, tile, y);
     int *ids = lds.ids + o.ts * 16;
+    tile.find(p);
     vec<float, V> r = run_entry<V, G>(p, lds, o, index, y, p.tiles - 1 - index), share(0.0f);
     Gates<V, B, G> g(p, o.c);
     X *gx = (X *)p.grad_x + tile.row0 * p.ld_gx;
     gate_or_char<G> *gg = (gate_or_char<G> *)p.grad_gate + tile.row0 * p.ld_gg;
 #pragma unroll 1
-    for (int b = p.run - B; b >= 0; b -= B) {
-        if (b >= o.n || !o.any) continue;
+    for (int b = o.any && o.n > 0 ? (o.n - 1) & ~(B - 1) : -1; b >= 0; b -= B) {
         const int t = o.t0 + b;
         Raw<V, B, X> x, d;
         vec<float, V> before[B];
@@ -799,9 +831,9 @@ __global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
             for (int j = B - 1; j >= 0; --j) {
                 const vec<float, V> gt = r + d[j];
                 r = g.template times<true>(j, gt);
-                store<V>(behind(gx, at_x + j * p.ld_gx), gt);
+                store_past<V>(behind(gx, at_x + j * p.ld_gx), gt);
                 if constexpr (__is_same(G, void)) share = fma<V>(r * -g.dt[j], before[j], share);
-                else store<V>(behind(gg, at_g + j * p.ld_gg), gt * before[j]);
+                else store_past<V>(behind(gg, at_g + j * p.ld_gg), gt * before[j]);
                 pace();
             }
         } else {
@@ -822,11 +854,11 @@ __global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
                 const vec<float, V> gt = r + d[j];
                 r = g.template times<false>(j, gt);
                 if (live && (q.starts >> j & 1) && p.grad_h0) store<V>(p.grad_h0 + (int64_t)ids[j] * p.D + o.c, r);
-                if (j < n) store<V>(behind(gx, at_x + j * p.ld_gx), live ? gt : zero);
+                if (j < n) store_past<V>(behind(gx, at_x + j * p.ld_gx), live ? gt : zero);
                 if constexpr (__is_same(G, void)) {
                     if (live) share = fma<V>(r * -g.dt[j], before[j], share);
                 } else {
-                    if (j < n) store<V>(behind(gg, at_g + j * p.ld_gg), live ? gt * before[j] : zero);
+                    if (j < n) store_past<V>(behind(gg, at_g + j * p.ld_gg), live ? gt * before[j] : zero);
                 }
                 pace();
             }
@@ -982,7 +1014,7 @@ void launch_forward_of(const ScanArgs &p, hipStream_t st)
 template <int V, typename X, typename G>
 int launch_forward(const ScanArgs &p, hipStream_t st)
 {
-    constexpr int B = sizeof(X) + (__is_same(G, void) ? 0 : sizeof(gate_or_char<G>)) <= 4 ? 16 : 8;
+    constexpr int B = 8;
     if (p.run >= B) launch_forward_of<V, B, X, G>(p, st);
     else launch_forward_of<V, 8, X, G>(p, st);
     return (int)hipGetLastError();
