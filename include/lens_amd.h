@@ -16,10 +16,10 @@
  *     never change a result: the tuning overrides LENS_AMD_OUTPUT_PPL / LENS_AMD_OUTPUT_WHOLE / LENS_AMD_TRAIN_LPR
  *     (read from the environment at first use), two "kernel attributes checked" flags (atomic), and the per-device
  *     address of the scratch array of lens_forward_counts_static (behind a mutex).  The overrides of the carried-state
- *     layout, LENS_AMD_CARRY_L2 and LENS_AMD_CARRY_SHARED, are read from the environment at every call (tests walk one
- *     shape through every layout); they change lens_event_scale too, so they must not change between a stream's
- *     producer and its consumer.  Calls from several host threads are safe; work on one device is ordered by the streams
- *     the caller passes.
+ *     layout, LENS_AMD_CARRY_L2 and LENS_AMD_CARRY_SHARED, and of the launches of a scan, LENS_AMD_SCAN_LAUNCHES, are
+ *     read from the environment at every call (tests walk one shape through every layout); the first two change
+ *     lens_event_scale too, so they must not change between a stream's producer and its consumer.  Calls from
+ *     several host threads are safe; work on one device is ordered by the streams the caller passes.
  *
  * Data layouts (row-major, last index fastest)
  *   frames      uint8  [Q][HW]            event-count frames (PNG pixels), HW = roi_dim*roi_dim

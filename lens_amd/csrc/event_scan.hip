@@ -7,13 +7,14 @@
 // Sequences lie one behind the other in the rows; row seq_off[s] starts sequence s.
 //
 // A run of rows acts on the state that enters it as h -> f h + H, and two runs in a row act as one such pair again.  So the
-// rows are cut into tiles, a workgroup each, a tile into runs of 8 to 128 rows, a thread each (V channels), and there are
-// three launches:
-//   pairs   the pair of every run over its rows; those of a tile are joined in LDS to what is before each run, and the tile's
+// rows are cut into tiles, a workgroup each, a tile into runs, a thread each (V channels).  Bytes bound it, and where
+// they do the rows are read once: a thread keeps its 8 or 16 rows in registers until the pairs of the tiles before have arrived.
+// Where the arithmetic of the rows counts too, three launches take less:
+//   pairs   the pair of every run of 8 to 128 rows; those of a tile are joined in LDS to what is before each, and the tile's
 //   join    what is before every tile (a few tiles are joined by the next launch itself)
-//   states  the states, a row after the other from what enters the run
-// The rows are read twice.  The second time is in the other order, so that what was read last comes from the Infinity Cache.
-// The order of every composition is fixed by T and D alone: results do not depend on timing.
+//   states  the states, a row after the other from what enters the run; the tiles in the other order, so that what was read
+//           last comes from the Infinity Cache
+// The order of every composition is fixed by T, D and the types alone: results do not depend on timing.
 // A run with the start of a sequence in it does not depend on what enters: it is marked, and the state is selected, not
 // multiplied by zero (an infinity of one sequence must not reach the next).
 //
@@ -23,15 +24,16 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <type_traits>
+#include <cstdlib>
 
 #include "../../include/lens_amd.h"
 
 namespace {
 
-// Rows a thread loads at once (B below): 16 forward where x and gates are 64 registers then, else 8; backward 8, whose states
-// in 32 bits are 32 registers.
-constexpr int MARK_ROWS = 8;                       // rows between two marks: backward starts from one for every batch
-constexpr int MAX_RUN = 128;                       // rows of a run: 8, 16, .. 128
+// Rows a thread loads at once, and rows between two marks of the states: backward computes the states of a batch again from
+// the mark before it (32 registers in 32 bits).
+constexpr int B = 8;
+constexpr int NUM_CUS = 256;
 constexpr int FAR = 1 << 30;                       // rows from a tile's first to one that it never reaches
 constexpr int64_t MAX_THREADS = 0xffff0000ll;      // of a launch in one direction
 
@@ -122,20 +124,22 @@ struct ScanArgs {
     float2 *agg;                       // [tiles][D] pairs of the tiles, in the order in which they are joined
     float *entry;                      // [tiles][D] what enters them; NULL: few tiles, joined by those that need it
     float *pre;                        // [tiles][ts][2][D] pairs of what is before a run in its tile
+    uint64_t *words;                   // one pass: pairs of the tiles and of their groups (Chain)
+    unsigned *ticket;
     float *part;                       // [tiles][D] a tile's share of grad_rate
     int64_t T;
     int ldx, ldg, ldh, ld_grad, ld_gx, ld_gg;
-    int n_seq, D, cg, lanes, ts, run, fill, ny, tiles;
+    int n_seq, D, cg, lanes, ts, run, fill, ny, tiles, levels;
 };
 
 // ------------------------------------------------------------------------------------------ rows, tiles, sequences
-// How many of the n offsets are at most `row`: a wavefront asks for 64 at once.
+// How many of the n offsets are at most `row`: a wavefront asks for as many at once as it has lanes (the workgroup's last may have few).
 __device__ __forceinline__ int offsets_up_to(const int64_t *off, int n, int64_t row)
 {
-    const int lane = (int)threadIdx.x & 63;
+    const int lane = (int)threadIdx.x & 63, from_here = (int)blockDim.x - ((int)threadIdx.x & ~63), lanes = from_here < 64 ? from_here : 64;
     int lo = 0, hi = n;
     while (lo < hi) {
-        const int step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step - 1;
+        const int step = (hi - lo + lanes - 1) / lanes, at = lo + (lane + 1) * step - 1;
         const int found = __builtin_popcountll(__ballot(at < hi && off[at < hi ? at : hi - 1] <= row));
         lo += found * step;
         hi = lo + step - 1 < hi ? lo + step - 1 : hi;
@@ -266,7 +270,7 @@ __device__ __forceinline__ void as_loaded(T &v)
 __device__ __forceinline__ void pace() { __builtin_amdgcn_sched_barrier(0); }
 
 // B rows of an operand from row t on, as they are stored.
-template <int V, int B, typename T>
+template <int V, typename T>
 struct Raw {
     vec<T, V> r[B];
     __device__ __forceinline__ void load_rows(const T *base, int ld, int t, int c, const Tile &tile)
@@ -300,7 +304,6 @@ struct Rows {
 };
 
 // `w` is the place of row t, and moves on to row t + B.
-template <int B>
 __device__ __forceinline__ Rows rows_of(const ScanArgs &p, const Tile &tile, Place &w, int t, int *ids)
 {
     const int left = tile.left - t, n = left < B ? left : B;
@@ -384,11 +387,13 @@ struct Pair {
 };
 
 // Gates of B rows.  G = void: decays.
-template <int V, int B, typename G>
+template <int V, typename G>
 struct Gates {
-    Raw<V, B, G> g;
+    Raw<V, G> g;
     vec<float, V> a;                   // product over the rows so far
+    __device__ __forceinline__ Gates() : a(1.0f) {}
     __device__ __forceinline__ Gates(const ScanArgs &, int) : a(1.0f) {}
+    __device__ __forceinline__ void begin(const ScanArgs &, int) {}
     __device__ __forceinline__ void load_rows(const ScanArgs &p, int t, int c, const Tile &tile)
     {
         g.load_rows((const G *)p.gate, p.ldg, t, c, tile);
@@ -406,17 +411,21 @@ struct Gates {
 #pragma unroll
         for (int j = 0; j < B; ++j) a *= g[j];
     }
+    __device__ __forceinline__ void absorb(const Gates &n) { a *= n.a; }
     __device__ __forceinline__ vec<float, V> factor() const { return a; }
 };
 
-template <int V, int B>
-struct Gates<V, B, void> {
+template <int V>
+struct Gates<V, void> {
     float dt[B], sum;
     vec<float, V> rate;
     float fastest;
     bool near;                         // all of the thread's are: no exponentials
-    __device__ __forceinline__ Gates(const ScanArgs &p, int c) : sum(0.0f), rate(load<V>(p.rate + c)), fastest(0.0f)
+    __device__ __forceinline__ Gates() : sum(0.0f), rate(0.0f), fastest(0.0f) {}
+    __device__ __forceinline__ Gates(const ScanArgs &p, int c) : Gates() { begin(p, c); }
+    __device__ __forceinline__ void begin(const ScanArgs &p, int c)
     {
+        rate = load<V>(p.rate + c);
 #pragma unroll
         for (int i = 0; i < V; ++i) fastest = __builtin_fmaxf(fastest, __builtin_fabsf(rate[i]));
     }
@@ -455,9 +464,10 @@ struct Gates<V, B, void> {
     }
     __device__ __forceinline__ void add_rows()
     {
-#pragma unroll
-        for (int j = 0; j < B; ++j) sum += dt[j];
+        static_assert(B == 8, "");
+        sum += ((dt[0] + dt[1]) + (dt[2] + dt[3])) + ((dt[4] + dt[5]) + (dt[6] + dt[7]));      // errors of 128 rows: 3 + 15 roundings
     }
+    __device__ __forceinline__ void absorb(const Gates &n) { sum += n.sum; }
     __device__ __forceinline__ vec<float, V> factor() const
     {
         vec<float, V> f;
@@ -472,7 +482,7 @@ struct Gates<V, B, void> {
 template <int V>
 struct Lds {
     float *f, *h;                      // [ts][slots] pairs of the runs
-    int *ids;                          // [ts][16] sequences of the rows of a batch
+    int *ids;                          // [ts][B] sequences of the rows of a batch
     int slots;
     __device__ __forceinline__ Lds(const ScanArgs &p)
     {
@@ -482,7 +492,7 @@ struct Lds {
         h = f + p.ts * slots;
         ids = reinterpret_cast<int *>(h + p.ts * slots);
     }
-    static size_t bytes(int ts, int lanes) { return ((size_t)2 * ts * lanes * V + ts * 16) * 4; }
+    static size_t bytes(int ts, int lanes) { return ((size_t)2 * ts * lanes * V + ts * B) * 4; }
 };
 
 // The channel of a slot, -1: none.
@@ -613,16 +623,85 @@ __device__ __forceinline__ void put_pair(const Lds<V> &lds, const Own<V> &o, vec
 }
 
 // ------------------------------------------------------------------------------------------ forward
-template <int V, int B, typename X, typename G>
+// A sequence without rows ends as it began: `to` (if any) from `from` (zeros without).  Shared out over `of` workgroups.
+__device__ __forceinline__ void pass_on(const ScanArgs &p, const float *from, float *to, int index, int of)
+{
+    if (!p.off || !to) return;
+    for (int64_t s = index; s < p.n_seq; s += of)
+        if (p.off[s] == p.off[s + 1])
+            for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x) to[s * p.D + c] = from ? from[s * p.D + c] : 0.0f;
+}
+
+// Instead of everything else where there are no rows at all.
+__global__ void __launch_bounds__(256) k_scan_no_rows(const float *from, float *to, int64_t n, float *rate, int D)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n || i < D; i += (int64_t)gridDim.x * 256) {
+        if (to && i < n) to[i] = from ? from[i] : 0.0f;
+        if (rate && i < D) rate[i] = 0.0f;
+    }
+}
+
+// H behind the rows of a batch, from H before them.
+template <int V, typename X, typename G>
+__device__ __forceinline__ void forward_batch(const ScanArgs &p, const Own<V> &o, const Rows &r, const int *ids, const Raw<V, X> &x,
+                                              const Gates<V, G> &g, vec<float, V> &H)
+{
+    if (__all(r.plain && g.near)) {
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            H = g.template step<true>(j, H, x[j]);
+            pace();
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            if (r.starts >> j & 1) H = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+            H = g.template step<false>(j, H, x[j]);
+            pace();
+        }
+    }
+}
+
+// The states of a batch of rows from row t on, stored; st: the state before them, then behind them.  out: of the tile.
+template <int V, typename X, typename G>
+__device__ __forceinline__ void states_batch(const ScanArgs &p, const Tile &tile, const Own<V> &o, const Rows &r, const int *ids, int t,
+                                             const Raw<V, X> &x, const Gates<V, G> &g, X *out, vec<float, V> &st)
+{
+    float *mark = p.marks ? p.marks + (tile.row0 + t) / B * p.D + o.c : nullptr;
+    const uint32_t at = (uint32_t)(t * p.ldh + o.c);
+    if (__all(r.plain && g.near)) {
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            if (j == 0 && mark) store<V>(mark, st);
+            st = g.template step<true>(j, st, x[j]);
+            store_past<V>(behind(out, at + j * p.ldh), st);
+            pace();
+        }
+    } else {
+        const int n = tile.left - t;
+        const unsigned in = n < B ? (1u << n) - 1 : (1u << B) - 1, written = p.fill ? in : r.lives;
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            if (j == 0 && mark) store<V>(mark, st);
+            if (r.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+            st = g.template step<false>(j, st, x[j]);
+            if (written >> j & 1) store_past<V>(behind(out, at + j * p.ldh), r.lives >> j & 1 ? st : vec<float, V>(0.0f));
+            if (r.ends >> j & 1) store<V>(p.last + (int64_t)ids[j] * p.D + o.c, st);
+            pace();
+        }
+    }
+}
+
+template <int V, typename X, typename G>
 __global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
 {
     const Lds<V> lds(p);
     const int index = blockIdx.x, y = blockIdx.y;
     Tile tile(p, index);
     const Own<V> o(p, tile, y);
-    int *ids = lds.ids + o.ts * 16;
-    Gates<V, B, G> g(p, o.c);
-    Raw<V, B, X> x;
+    int *ids = lds.ids + o.ts * B;
+    Gates<V, G> g(p, o.c);
+    Raw<V, X> x;
     vec<float, V> H(0.0f);
     bool mark = false;
     auto load_batch = [&](int b) {
@@ -636,22 +715,9 @@ __global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
 #pragma unroll 1
         for (int b = 0; b < o.n; b += B) {
             if (b) load_batch(b);
-            const Rows r = rows_of<B>(p, tile, w, o.t0 + b, ids);
+            const Rows r = rows_of(p, tile, w, o.t0 + b, ids);
             mark |= r.starts != 0;
-            if (__all(r.plain && g.near)) {
-#pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    H = g.template step<true>(j, H, x[j]);
-                    pace();
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    if (r.starts >> j & 1) H = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-                    H = g.template step<false>(j, H, x[j]);
-                    pace();
-                }
-            }
+            forward_batch<V, X, G>(p, o, r, ids, x, g, H);
             g.again();
             g.add_rows();
         }
@@ -661,26 +727,17 @@ __global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
     join_runs<V, G, false>(p, lds, index, y, index);
 }
 
-template <int V, int B, typename X, typename G>
+template <int V, typename X, typename G>
 __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
 {
     const Lds<V> lds(p);
     const int index = p.tiles - 1 - (int)blockIdx.x, y = blockIdx.y;       // what the first pass read last
-    // a sequence without rows ends as it began
-    if (p.off && y == 0)
-        for (int64_t s = index; s < p.n_seq; s += p.tiles)
-            if (p.off[s] == p.off[s + 1])
-                for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x) p.last[s * p.D + c] = p.h0 ? p.h0[s * p.D + c] : 0.0f;
-    if (p.T == 0) {
-        if (!p.off && y == 0)
-            for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x) p.last[c] = p.h0 ? p.h0[c] : 0.0f;
-        return;
-    }
+    if (y == 0) pass_on(p, p.h0, p.last, index, p.tiles);
     Tile tile(p, index);
     const Own<V> o(p, tile, y);
-    int *ids = lds.ids + o.ts * 16;
-    Gates<V, B, G> g(p, o.c);
-    Raw<V, B, X> x;
+    int *ids = lds.ids + o.ts * B;
+    Gates<V, G> g(p, o.c);
+    Raw<V, X> x;
     auto load_batch = [&](int b) {
         x.load_rows((const X *)p.x, p.ldx, o.t0 + b, o.c, tile);
         g.load_rows(p, o.t0 + b, o.c, tile);
@@ -695,48 +752,350 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
     for (int b = 0; b < o.n; b += B) {
         const int t = o.t0 + b;
         if (b) load_batch(b);
-        const Rows r = rows_of<B>(p, tile, w, t, ids);
-        float *mark = p.marks ? p.marks + (tile.row0 + t) / MARK_ROWS * p.D + o.c : nullptr;
-        const uint32_t at = (uint32_t)(t * p.ldh + o.c);
-        if (__all(r.plain && g.near)) {
+        const Rows r = rows_of(p, tile, w, t, ids);
+        states_batch<V, X, G>(p, tile, o, r, ids, t, x, g, out, st);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ one pass
+// The rows stay in registers until what is before them is known.  What enters a tile: the tiles of a launch are numbered by a
+// ticket that every workgroup draws when it starts; a workgroup waits only for what workgroups with smaller tickets publish,
+// which run already and publish before they wait for anything larger, so every wait ends.  8 or 16 tiles are a group, as many
+// groups a group of the next level, and the last tile of a group publishes the group's pair from those below.  What enters tile
+// i are the pairs before it in its group, before that group in its own, and so on: 3.5 or 7.5 pairs a level, read at once
+// by a wavefront a level, always joined in the same order.  A word is the pair of one channel: 8 bytes, stored and read
+// whole, all ones until it is there (a lane a channel: 8 words in flight and few registers).
+// Scratch memory that another call uses at the same time could keep a wait from ending: it is given up after about a second,
+// all others of the launch then at once, and the results are NaN.
+//
+// One pass against reading twice, us a call:
+//   forward    1048573 x 128 bf16, bf16 gates  189 / 253     400009 x 200 bf16, decays  135 / 123     1501 x 200 f32, decays  17 / 19
+//              262144 x 128 f32, decays         72 / 78       30000 x 128 bf16, decays   20 / 22      30000 x 128 f32, f32 gates  18 / 23
+//   backward   524287 x 256 bf16, bf16 gates   317 / 357     400009 x 200 bf16, decays  228 / 193     1501 x 200 f32, decays  23 / 23
+//              262144 x 128 f32, decays        114 / 113      30000 x 128 bf16, decays   26 / 31      30000 x 128 f32, f32 gates  21 / 27
+// So 16-bit rows with decays -- the fewest bytes for the arithmetic of a row -- are read twice when there are many, by
+// workgroups that wait for nothing; all others go in one pass.
+constexpr uint64_t EMPTY = ~0ull;
+constexpr int MOST_TRIES = 1 << 20;
+
+// 16 tiles a group, for decays, whose pairs take more work to join, 8.
+template <typename G> constexpr int group_bits = 4;
+template <> constexpr int group_bits<void> = 3;
+
+template <int V>
+struct LdsOnce {
+    float *f, *h;                      // [ts][slots] pairs of the runs, then of what is before each of them
+    float *bf, *bh;                    // [levels][slots] what is before the tile, a level each
+    int *ids;                          // [ts][run] sequences of the rows
+    int slots;
+    __device__ __forceinline__ LdsOnce(const ScanArgs &p)
+    {
+        extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+        slots = p.lanes * V;
+        f = reinterpret_cast<float *>(smem);
+        h = f + p.ts * slots;
+        bf = h + p.ts * slots;
+        bh = bf + p.levels * slots;
+        ids = reinterpret_cast<int *>(bh + p.levels * slots);
+    }
+    static size_t bytes(int ts, int lanes, int levels, int run) { return ((size_t)(2 * ts + 2 * levels) * lanes * V + ts * run) * 4; }
+};
+
+template <int V, typename G>
+struct Chain {
+    static constexpr int GROUP_BITS = group_bits<G>, GROUP = 1 << GROUP_BITS;
+    uint64_t *words;
+    unsigned *ticket;                  // and behind it: a wait was given up
+    int tile, tiles, levels, ts, D, c0, slots, cg_left;      // c0, cg_left: of the workgroup's part of the channels
+    __device__ __forceinline__ Chain(const ScanArgs &p, int tile_, int y)
+        : words(p.words), ticket(p.ticket), tile(tile_), tiles(p.tiles), levels(p.levels), ts(p.ts), D(p.D), c0(y * p.lanes * V),
+          slots(p.lanes * V), cg_left((p.cg - y * p.lanes) * V) {}
+    static __device__ __forceinline__ uint64_t word_of(Pair<G> w) { return (uint64_t)bits(w.H) << 32 | bits(w.f); }
+    static __device__ __forceinline__ Pair<G> pair_of(uint64_t w) { return {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))}; }
+    // the words of a tile or group, and a slot's among them (-1: the slot has no channel)
+    __device__ __forceinline__ uint64_t *at(int level, int index) const
+    {
+        int64_t before = 0;
+        for (int l = 0; l < level; ++l) before += tiles >> (GROUP_BITS * l);
+        return words + (before + index) * D;
+    }
+    __device__ __forceinline__ int channel(int slot) const
+    {
+        if (slot >= slots || slot >= cg_left) return -1;
+        const int first = c0 + slot / V * V;
+        return (first < D - V ? first : D - V) + slot % V;
+    }
+    __device__ __forceinline__ void publish(int level, int slot, Pair<G> w) const
+    {
+        uint64_t *to = at(level, tile >> (GROUP_BITS * level));
+        const int c = channel(slot);
+        if (c >= 0) __hip_atomic_store(behind(to, c), word_of(w), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __device__ __forceinline__ bool give_up(int tries) const
+    {
+        if (tries == MOST_TRIES) __hip_atomic_store(ticket + 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return __hip_atomic_load(ticket + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
+    }
+    // the pairs before the tile on one level, as one; the level is the same for the whole wavefront
+    __device__ __forceinline__ Pair<G> before(int level, int slot) const
+    {
+        const int index = tile >> (GROUP_BITS * level), n = index & (GROUP - 1);
+        uint64_t *from = at(level, index & ~(GROUP - 1));
+        const int c = channel(slot);
+        Pair<G> w = Pair<G>::none();
+        if (c < 0 || n == 0) return w;
+#pragma unroll 1
+        for (int k0 = 0; k0 < n; k0 += 8) {
+            uint64_t v[8];
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
-                if (j % MARK_ROWS == 0 && mark) store<V>(mark + j / MARK_ROWS * p.D, st);
-                st = g.template step<true>(j, st, x[j]);
-                store_past<V>(behind(out, at + j * p.ldh), st);
-                pace();
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k < n) v[k] = __hip_atomic_load(behind(from, (k0 + k) * D + c), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)                   // only what is not there yet is asked for again, one word at a time
+                if (k0 + k < n) {
+                    for (int tries = 1; v[k] == EMPTY; ++tries) {
+                        if (tries % 256 == 0 && give_up(tries)) {
+                            v[k] = (uint64_t)QUIET << 32 | QUIET;
+                            break;
+                        }
+                        __builtin_amdgcn_s_sleep(8);
+                        v[k] = __hip_atomic_load(behind(from, (k0 + k) * D + c), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    }
+                    w = w.then(pair_of(v[k]));
+                }
+        }
+        return w;
+    }
+    // The runs' pairs of a tile in LDS -> what is before each of them, there; the tile's pair is published, and that of every
+    // group that it completes.  BACK: from the last run to the first.  The first wavefronts work, a lane a slot.
+    template <bool BACK>
+    __device__ __forceinline__ void runs(const LdsOnce<V> &lds) const
+    {
+        const int slot = (int)threadIdx.x;
+        if (slot >= slots) return;
+        Pair<G> w = Pair<G>::none();
+        for (int q0 = 0; q0 < ts; q0 += 8) {
+            Pair<G> n[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int q = q0 + i < ts ? q0 + i : ts - 1, k = (BACK ? ts - 1 - q : q) * slots + slot;
+                n[i] = {lds.f[k], lds.h[k]};
             }
-        } else {
-            const int n = tile.left - t;
-            const unsigned in = n < B ? (1u << n) - 1 : (1u << B) - 1, written = p.fill ? in : r.lives;
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
-                if (j % MARK_ROWS == 0 && mark && (in >> j & 1)) store<V>(mark + j / MARK_ROWS * p.D, st);
-                if (r.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-                st = g.template step<false>(j, st, x[j]);
-                if (written >> j & 1) store_past<V>(behind(out, at + j * p.ldh), r.lives >> j & 1 ? st : vec<float, V>(0.0f));
-                if (r.ends >> j & 1) store<V>(p.last + (int64_t)ids[j] * p.D + o.c, st);
-                pace();
+            for (int i = 0; i < 8; ++i)
+                if (q0 + i < ts) {
+                    const int k = (BACK ? ts - 1 - q0 - i : q0 + i) * slots + slot;
+                    lds.f[k] = w.f;
+                    lds.h[k] = w.H;
+                    w = w.then(n[i]);
+                }
+        }
+        if (tile + 1 < tiles) publish(0, slot, w);
+#pragma unroll 1
+        for (int l = 0; l + 1 < levels && ((tile >> (GROUP_BITS * l)) & (GROUP - 1)) == GROUP - 1; ++l) {
+            w = before(l, slot).then(w);
+            publish(l + 1, slot, w);
+        }
+    }
+    // What is before the tile -> LDS, a wavefront a level and 64 slots.  All threads call it, then a barrier.
+    __device__ __forceinline__ void gather(const LdsOnce<V> &lds) const
+    {
+        const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        const int waves = blockDim.x < 64 ? 1 : (int)blockDim.x >> 6;      // whole ones
+        const int per = (slots + 63) / 64, all = levels * per;
+#pragma unroll 1
+        for (int q = wave < waves ? wave : all; q < all; q += waves) {
+            const int l = q / per, slot = q % per * 64 + lane;
+            const Pair<G> b = before(l, slot);
+            if (slot < slots) {
+                lds.bf[l * slots + slot] = b.f;
+                lds.bh[l * slots + slot] = b.H;
             }
         }
     }
+    // the state that enters the tile, for a lane of the rows
+    __device__ __forceinline__ vec<float, V> entry(const LdsOnce<V> &lds, int lane) const
+    {
+        vec<float, V> st(0.0f);
+        for (int l = levels - 1; l >= 0; --l) {
+            const vec<float, V> f = lds_load<V>(lds.bf + l * slots + lane * V), H = lds_load<V>(lds.bh + l * slots + lane * V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) st[i] = Pair<G>{f[i], H[i]}.over(st[i]);
+        }
+        return st;
+    }
+};
+
+// Before every launch of one pass.
+__global__ void __launch_bounds__(256) k_scan_clear(uint4 *words, int64_t n, unsigned *ticket)
+{
+    if (blockIdx.x == 0 && threadIdx.x < 2) ticket[threadIdx.x] = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+        words[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+}
+
+// Workgroups of 512 threads; forward at most 128 registers each (two workgroups a CU), backward 256: with three operands and the
+// states it would spill.
+constexpr int ONCE = 512;
+
+template <int V, int NB, typename X, typename G>
+__global__ void __launch_bounds__(ONCE, 4) k_scan_once(const ScanArgs p)
+{
+    __shared__ unsigned mine;
+    if (threadIdx.x == 0) mine = p.tiles > 1 ? atomicAdd(p.ticket, 1u) : blockIdx.x;
+    const LdsOnce<V> lds(p);
+    pass_on(p, p.h0, p.last, blockIdx.x, gridDim.x);
+    __syncthreads();
+    const int ticket = __builtin_amdgcn_readfirstlane(mine), index = ticket / p.ny, y = ticket % p.ny;
+    if (ticket >= (int)gridDim.x) return;          // only where another call uses the scratch memory too
+    Tile tile(p, index);
+    const Own<V> o(p, tile, y);
+    int *ids = lds.ids + o.ts * (NB * B);
+    Raw<V, X> x[NB];
+    Gates<V, G> g[NB];
+    Rows r[NB];
+    if (o.n > 0)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            x[b].load_rows((const X *)p.x, p.ldx, o.t0 + b * B, o.c, tile);
+            g[b].begin(p, o.c);
+            g[b].load_rows(p, o.t0 + b * B, o.c, tile);
+        }
+    tile.find(p);
+    vec<float, V> H(0.0f);
+    bool mark = false;
+    if (o.n > 0) {
+        Place w = locate(p, tile, o.t0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            r[b] = rows_of(p, tile, w, o.t0 + b * B, ids + b * B);
+            mark |= r[b].starts != 0;
+            forward_batch<V, X, G>(p, o, r[b], ids + b * B, x[b], g[b], H);
+            g[b].again();
+            g[b].add_rows();
+            if (b) g[0].absorb(g[b]);
+        }
+    }
+    vec<float, V> f = g[0].factor();
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = mark ? __uint_as_float(MARK) : Pair<G>::quiet(f[i]);
+    lds_store<V>(lds.f + o.ts * lds.slots + o.lane * V, f);
+    lds_store<V>(lds.h + o.ts * lds.slots + o.lane * V, H);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        x[b].again();
+        if (!__is_same(G, void)) g[b].again();
+    }
+    const Chain<V, G> chain(p, index, y);
+    chain.template runs<false>(lds);
+    if (p.levels) chain.gather(lds);
+    __syncthreads();
+    if (!o.any || o.n == 0) return;
+    vec<float, V> st = chain.entry(lds, o.lane);
+    const vec<float, V> bf = lds_load<V>(lds.f + o.ts * lds.slots + o.lane * V), bh = lds_load<V>(lds.h + o.ts * lds.slots + o.lane * V);
+#pragma unroll
+    for (int i = 0; i < V; ++i) st[i] = Pair<G>{bf[i], bh[i]}.over(st[i]);
+    X *out = (X *)p.h + tile.row0 * p.ldh;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+        if (b * B < o.n) {
+            if (__is_same(G, void)) g[b].load_rows(p, o.t0 + b * B, o.c, tile);      // few bytes: not kept
+            states_batch<V, X, G>(p, tile, o, r[b], ids + b * B, o.t0 + b * B, x[b], g[b], out, st);
+        }
 }
 
 // ------------------------------------------------------------------------------------------
 // Backward.  With r_t = a_t g_t the message that row t sends back: g_t = dh_t + r_{t+1}, so a run of rows acts on the
 // message that enters from behind as r -> f r + U with the f of the forward direction.  The states before the rows are
-// computed again from the marks, MARK_ROWS rows at a time.
+// computed again from the marks, B rows at a time.
 // ------------------------------------------------------------------------------------------
-template <int V, int B, typename X, typename G>
+// The message before the rows of a batch, from U behind them.
+template <int V, typename X, typename G>
+__device__ __forceinline__ void backward_batch(const ScanArgs &p, const Own<V> &o, const Rows &r, const int *ids, const Raw<V, X> &d,
+                                               const Gates<V, G> &g, vec<float, V> &U)
+{
+    if (__all(r.plain && g.near)) {
+#pragma unroll
+        for (int j = B - 1; j >= 0; --j) {
+            U = g.template times<true>(j, U + d[j]);
+            pace();
+        }
+    } else {
+#pragma unroll
+        for (int j = B - 1; j >= 0; --j) {
+            if (r.ends >> j & 1) U = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
+            U = g.template times<false>(j, U + d[j]);
+            pace();
+        }
+    }
+}
+
+// The gradients of a batch of rows from row t on, stored; st: the state before them, r: the message behind them, then before them.
+// gx, gg: of the tile.
+template <int V, typename X, typename G>
+__device__ __forceinline__ void rows_batch(const ScanArgs &p, const Tile &tile, const Own<V> &o, const Rows &q, const int *ids, int t,
+                                           const Raw<V, X> &x, const Raw<V, X> &d, Gates<V, G> &g, X *gx, gate_or_char<G> *gg,
+                                           vec<float, V> st, vec<float, V> &r, vec<float, V> &share)
+{
+    const vec<float, V> zero(0.0f);
+    vec<float, V> before[B];
+    const uint32_t at_x = (uint32_t)(t * p.ld_gx + o.c), at_g = (uint32_t)(t * p.ld_gg + o.c);
+    if (__all(q.plain && g.near)) {
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            before[j] = st;
+            if (j + 1 < B) st = g.template step<true>(j, st, x[j]);
+            pace();
+        }
+        g.again();
+#pragma unroll
+        for (int j = B - 1; j >= 0; --j) {
+            const vec<float, V> gt = r + d[j];
+            r = g.template times<true>(j, gt);
+            store_past<V>(behind(gx, at_x + j * p.ld_gx), gt);
+            if constexpr (__is_same(G, void)) share = fma<V>(r * -g.dt[j], before[j], share);
+            else store_past<V>(behind(gg, at_g + j * p.ld_gg), gt * before[j]);
+            pace();
+        }
+    } else {
+        const int n = tile.left - t;
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            if (q.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+            before[j] = st;
+            st = g.template step<false>(j, st, x[j]);
+            pace();
+        }
+        g.again();
+#pragma unroll
+        for (int j = B - 1; j >= 0; --j) {
+            const bool live = q.lives >> j & 1;
+            if (q.ends >> j & 1) r = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
+            const vec<float, V> gt = r + d[j];
+            r = g.template times<false>(j, gt);
+            if (live && (q.starts >> j & 1) && p.grad_h0) store<V>(p.grad_h0 + (int64_t)ids[j] * p.D + o.c, r);
+            if (j < n) store_past<V>(behind(gx, at_x + j * p.ld_gx), live ? gt : zero);
+            if constexpr (__is_same(G, void)) {
+                if (live) share = fma<V>(r * -g.dt[j], before[j], share);
+            } else {
+                if (j < n) store_past<V>(behind(gg, at_g + j * p.ld_gg), live ? gt * before[j] : zero);
+            }
+            pace();
+        }
+    }
+}
+
+template <int V, typename X, typename G>
 __global__ void __launch_bounds__(256) k_scan_back_pairs(const ScanArgs p)
 {
     const Lds<V> lds(p);
     const int index = blockIdx.x, y = blockIdx.y;
     Tile tile(p, index);
     const Own<V> o(p, tile, y);
-    int *ids = lds.ids + o.ts * 16;
-    Gates<V, B, G> g(p, o.c);
-    Raw<V, B, X> d;
+    int *ids = lds.ids + o.ts * B;
+    Gates<V, G> g(p, o.c);
+    Raw<V, X> d;
     vec<float, V> U(0.0f);
     bool mark = false;
     auto load_batch = [&](int b) {
@@ -751,22 +1110,9 @@ __global__ void __launch_bounds__(256) k_scan_back_pairs(const ScanArgs p)
     for (int b = last; b >= 0; b -= B) {
         if (b != last) load_batch(b);
         Place w = locate(p, tile, o.t0 + b);
-        const Rows r = rows_of<B>(p, tile, w, o.t0 + b, ids);
+        const Rows r = rows_of(p, tile, w, o.t0 + b, ids);
         mark |= r.ends != 0;
-        if (__all(r.plain && g.near)) {
-#pragma unroll
-            for (int j = B - 1; j >= 0; --j) {
-                U = g.template times<true>(j, U + d[j]);
-                pace();
-            }
-        } else {
-#pragma unroll
-            for (int j = B - 1; j >= 0; --j) {
-                if (r.ends >> j & 1) U = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
-                U = g.template times<false>(j, U + d[j]);
-                pace();
-            }
-        }
+        backward_batch<V, X, G>(p, o, r, ids, d, g, U);
         g.again();
         g.add_rows();
     }
@@ -775,94 +1121,118 @@ __global__ void __launch_bounds__(256) k_scan_back_pairs(const ScanArgs p)
     join_runs<V, G, true>(p, lds, index, y, p.tiles - 1 - index);
 }
 
-template <int V, int B, typename X, typename G>
+template <int V, typename X, typename G>
 __global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
 {
     const Lds<V> lds(p);
     const int index = p.tiles - 1 - (int)blockIdx.x, y = blockIdx.y;       // what the first pass read last
-    const vec<float, V> zero(0.0f);
-    if (p.off && p.grad_h0 && y == 0)
-        for (int64_t s = index; s < p.n_seq; s += p.tiles)
-            if (p.off[s] == p.off[s + 1])
-                for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x)
-                    p.grad_h0[s * p.D + c] = p.grad_last ? p.grad_last[s * p.D + c] : 0.0f;
-    if (p.T == 0) {
-        for (int c = (int)threadIdx.x; c < p.D && y == 0; c += blockDim.x) {
-            if (!p.off && p.grad_h0) p.grad_h0[c] = p.grad_last ? p.grad_last[c] : 0.0f;
-            if (__is_same(G, void)) p.part[c] = 0.0f;
-        }
-        return;
-    }
+    if (y == 0) pass_on(p, p.grad_last, p.grad_h0, index, p.tiles);
     Tile tile(p, index);
     const Own<V> o(p, tile, y);
-    int *ids = lds.ids + o.ts * 16;
+    int *ids = lds.ids + o.ts * B;
     tile.find(p);
     vec<float, V> r = run_entry<V, G>(p, lds, o, index, y, p.tiles - 1 - index), share(0.0f);
-    Gates<V, B, G> g(p, o.c);
+    Gates<V, G> g(p, o.c);
     X *gx = (X *)p.grad_x + tile.row0 * p.ld_gx;
     gate_or_char<G> *gg = (gate_or_char<G> *)p.grad_gate + tile.row0 * p.ld_gg;
 #pragma unroll 1
     for (int b = o.any && o.n > 0 ? (o.n - 1) & ~(B - 1) : -1; b >= 0; b -= B) {
         const int t = o.t0 + b;
-        Raw<V, B, X> x, d;
-        vec<float, V> before[B];
+        Raw<V, X> x, d;
         g.load_rows(p, t, o.c, tile);
         x.load_rows((const X *)p.x, p.ldx, t, o.c, tile);
-        constexpr bool wide_rows = sizeof(X) == 4 && !__is_same(G, void);      // x, gates and gradient at once would not fit
-        auto load_d = [&]() {
-            if (p.grad) d.load_rows((const X *)p.grad, p.ld_grad, t, o.c, tile);
-            else d.zero();
-        };
-        if (!wide_rows) load_d();
-        vec<float, V> st = load<V>(p.marks_in + (tile.row0 + t) / MARK_ROWS * p.D + o.c);
+        if (p.grad) d.load_rows((const X *)p.grad, p.ld_grad, t, o.c, tile);
+        else d.zero();
+        vec<float, V> st = load<V>(p.marks_in + (tile.row0 + t) / B * p.D + o.c);
         Place w = locate(p, tile, t);
-        const Rows q = rows_of<B>(p, tile, w, t, ids);
-        const uint32_t at_x = (uint32_t)(t * p.ld_gx + o.c), at_g = (uint32_t)(t * p.ld_gg + o.c);
-        if (__all(q.plain && g.near)) {
-#pragma unroll
-            for (int j = 0; j < B; ++j) {
-                before[j] = st;
-                if (j + 1 < B) st = g.template step<true>(j, st, x[j]);
-                pace();
-            }
-            g.again();
-            if (wide_rows) load_d();
-#pragma unroll
-            for (int j = B - 1; j >= 0; --j) {
-                const vec<float, V> gt = r + d[j];
-                r = g.template times<true>(j, gt);
-                store_past<V>(behind(gx, at_x + j * p.ld_gx), gt);
-                if constexpr (__is_same(G, void)) share = fma<V>(r * -g.dt[j], before[j], share);
-                else store_past<V>(behind(gg, at_g + j * p.ld_gg), gt * before[j]);
-                pace();
-            }
-        } else {
-            const int n = tile.left - t;
-#pragma unroll
-            for (int j = 0; j < B; ++j) {
-                if (q.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-                before[j] = st;
-                st = g.template step<false>(j, st, x[j]);
-                pace();
-            }
-            g.again();
-            if (wide_rows) load_d();
-#pragma unroll
-            for (int j = B - 1; j >= 0; --j) {
-                const bool live = q.lives >> j & 1;
-                if (q.ends >> j & 1) r = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
-                const vec<float, V> gt = r + d[j];
-                r = g.template times<false>(j, gt);
-                if (live && (q.starts >> j & 1) && p.grad_h0) store<V>(p.grad_h0 + (int64_t)ids[j] * p.D + o.c, r);
-                if (j < n) store_past<V>(behind(gx, at_x + j * p.ld_gx), live ? gt : zero);
-                if constexpr (__is_same(G, void)) {
-                    if (live) share = fma<V>(r * -g.dt[j], before[j], share);
-                } else {
-                    if (j < n) store_past<V>(behind(gg, at_g + j * p.ld_gg), live ? gt * before[j] : zero);
-                }
-                pace();
-            }
+        const Rows q = rows_of(p, tile, w, t, ids);
+        rows_batch<V, X, G>(p, tile, o, q, ids, t, x, d, g, gx, gg, st, r, share);
+    }
+    if constexpr (__is_same(G, void)) {
+        __syncthreads();
+        lds_store<V>(lds.f + o.ts * lds.slots + o.lane * V, share);
+        __syncthreads();
+        if (o.ts == 0 && o.any) {
+            for (int k = 1; k < p.ts; ++k) share += lds_load<V>(lds.f + k * lds.slots + o.lane * V);
+            store<V>(p.part + (int64_t)index * p.D + o.c, share);
         }
+    }
+}
+
+template <int V, int NB, typename X, typename G>
+__global__ void __launch_bounds__(ONCE, 2) k_scan_back_once(const ScanArgs p)
+{
+    __shared__ unsigned mine;
+    if (threadIdx.x == 0) mine = p.tiles > 1 ? atomicAdd(p.ticket, 1u) : blockIdx.x;
+    const LdsOnce<V> lds(p);
+    pass_on(p, p.grad_last, p.grad_h0, blockIdx.x, gridDim.x);
+    __syncthreads();
+    const int ticket = __builtin_amdgcn_readfirstlane(mine), from_end = ticket / p.ny, y = ticket % p.ny;
+    if (ticket >= (int)gridDim.x) return;          // only where another call uses the scratch memory too
+    const int index = p.tiles - 1 - from_end;
+    Tile tile(p, index);
+    const Own<V> o(p, tile, y);
+    int *ids = lds.ids + o.ts * (NB * B);
+    Raw<V, X> d[NB];
+    Gates<V, G> g[NB];
+    Rows q[NB];
+    if (o.n > 0)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            g[b].begin(p, o.c);
+            g[b].load_rows(p, o.t0 + b * B, o.c, tile);
+            if (p.grad) d[b].load_rows((const X *)p.grad, p.ld_grad, o.t0 + b * B, o.c, tile);
+            else d[b].zero();
+        }
+    tile.find(p);
+    vec<float, V> U(0.0f);
+    bool mark = false;
+    if (o.n > 0) {
+        Place w = locate(p, tile, o.t0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) q[b] = rows_of(p, tile, w, o.t0 + b * B, ids + b * B);
+#pragma unroll
+        for (int b = NB - 1; b >= 0; --b) {
+            mark |= q[b].ends != 0;
+            backward_batch<V, X, G>(p, o, q[b], ids + b * B, d[b], g[b], U);
+            g[b].again();
+            g[b].add_rows();
+            if (b) g[0].absorb(g[b]);
+        }
+    }
+    vec<float, V> f = g[0].factor();
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = mark ? __uint_as_float(MARK) : Pair<G>::quiet(f[i]);
+    lds_store<V>(lds.f + o.ts * lds.slots + o.lane * V, f);
+    lds_store<V>(lds.h + o.ts * lds.slots + o.lane * V, U);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        d[b].again();
+        if (!__is_same(G, void)) g[b].again();
+    }
+    const Chain<V, G> chain(p, from_end, y);
+    chain.template runs<true>(lds);
+    if (p.levels) chain.gather(lds);
+    __syncthreads();
+    vec<float, V> share(0.0f);
+    if (o.any && o.n > 0) {
+        vec<float, V> r = chain.entry(lds, o.lane);
+        const vec<float, V> bf = lds_load<V>(lds.f + o.ts * lds.slots + o.lane * V), bh = lds_load<V>(lds.h + o.ts * lds.slots + o.lane * V);
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] = Pair<G>{bf[i], bh[i]}.over(r[i]);
+        X *gx = (X *)p.grad_x + tile.row0 * p.ld_gx;
+        gate_or_char<G> *gg = (gate_or_char<G> *)p.grad_gate + tile.row0 * p.ld_gg;
+#pragma unroll
+        for (int b = NB - 1; b >= 0; --b)
+            if (b * B < o.n) {
+                const int t = o.t0 + b * B;
+                Raw<V, X> x;
+                x.load_rows((const X *)p.x, p.ldx, t, o.c, tile);
+                if (__is_same(G, void)) g[b].load_rows(p, t, o.c, tile);      // few bytes: not kept
+                const vec<float, V> st = load<V>(p.marks_in + (tile.row0 + t) / B * p.D + o.c);
+                rows_batch<V, X, G>(p, tile, o, q[b], ids + b * B, t, x, d[b], g[b], gx, gg, st, r, share);
+            }
     }
     if constexpr (__is_same(G, void)) {
         __syncthreads();
@@ -951,46 +1321,131 @@ __global__ void __launch_bounds__(256) k_step(const StepArgs p)
 }
 
 // ------------------------------------------------------------------------------------------ launches
+// Workgroups of `threads` over the channels (ny parts of `lanes` lanes of V) and ts runs of rows.
 struct Shape {
-    int V, cg, ny, lanes, ts, run;
+    int V, cg, ny, lanes, ts;
 };
 
-// run: the longest that leaves 1024 workgroups (four a CU), the shortest where there is less
-Shape shape_of(int64_t T, int D)
+Shape shape_of(int D, int threads)
 {
     Shape s;
     s.V = D >= 4 ? 4 : 1;
     s.cg = (D + s.V - 1) / s.V;
     s.ny = (s.cg + 63) / 64;
     s.lanes = (s.cg + s.ny - 1) / s.ny;
-    s.ts = 256 / s.lanes;
-    if (s.ts > 32) s.ts = 32;
-    s.run = MAX_RUN;
-    while (s.run > 8 && T * s.ny < (int64_t)1024 * s.run * s.ts) s.run /= 2;
+    s.ts = threads / s.lanes < 32 ? threads / s.lanes : 32;
     return s;
 }
 
+int64_t tiles_of(int64_t T, int64_t rows) { return (T + rows - 1) / rows; }
+
+// Rows of a run where the rows are read twice: the most that leave 1024 workgroups (four a CU), the fewest where there are less.
+constexpr int MOST_RUN = 128;
+
+int run_of(int64_t T, const Shape &s)
+{
+    int run = MOST_RUN;
+    while (run > B && T * s.ny < (int64_t)1024 * run * s.ts) run /= 2;
+    return run;
+}
+
+// Tiles' pairs of at most this many tiles are joined by those that need them, without a launch.
 constexpr int FEW_TILES = 64;
 
+// Words of one pass: those of `tiles` tiles and of all complete groups above them; levels: how many that are.
+int64_t words_of(int64_t tiles, int D, int bits, int &levels)
+{
+    int64_t words = 0;
+    for (levels = 0; (tiles - 1) >> (bits * levels) > 0; ++levels) words += (tiles >> (bits * levels)) * D;
+    return words;
+}
+
+// Scratch: whichever way is taken, tiles as small as they get.  The parts of one way lie over those of the other.
 struct Scratch {
-    int64_t tiles;
-    size_t agg, entry, pre, part, bytes;
+    size_t agg, entry, pre;            // read twice
+    size_t ticket, words;              // one pass
+    size_t part, bytes;
 };
 
 Scratch scratch_of(int64_t T, int D, bool back)
 {
-    const Shape s = shape_of(T, D);
-    const int64_t rows = (int64_t)s.run * s.ts;
+    const Shape two = shape_of(D, 256), one = shape_of(D, ONCE);
+    const int64_t rows = (int64_t)run_of(T, two) * two.ts, tiles = tiles_of(T, rows), tiles_one = tiles_of(T, (int64_t)B * one.ts);
+    auto whole = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    int levels;
     Scratch r;
-    r.tiles = T > 0 ? (T + rows - 1) / rows : 1;
-    size_t at = 0;
-    auto take = [&](size_t n) { const size_t here = at; at += (n + 255) & ~(size_t)255; return here; };
-    r.agg = take((size_t)r.tiles * D * 8);
-    r.entry = take((size_t)r.tiles * D * 4);
-    r.pre = take((size_t)r.tiles * s.ts * 2 * D * 4);
-    r.part = back ? take((size_t)r.tiles * D * 4) : at;
-    r.bytes = at;
+    r.agg = 0;
+    r.entry = whole((size_t)tiles * D * 8);
+    r.pre = r.entry + whole((size_t)tiles * D * 4);
+    r.ticket = 0;
+    r.words = 256;
+    const size_t end_two = r.pre + whole((size_t)tiles * two.ts * 2 * D * 4);
+    const size_t end_one = r.words + whole((size_t)words_of(tiles_one, D, group_bits<void>, levels) * 8);
+    r.part = end_two > end_one ? end_two : end_one;
+    r.bytes = r.part + (back ? whole((size_t)(tiles > tiles_one ? tiles : tiles_one) * D * 4) : 0);
     return r;
+}
+
+// Whether 16-bit rows with decays are read twice, in three launches; all others take one pass (measured
+// above).  LENS_AMD_SCAN_LAUNCHES=1/3 forces the choice (tests; read at every call).
+constexpr int64_t MANY_ELEMENTS = 1 << 23;
+
+template <typename X, typename G> constexpr bool either_way = sizeof(X) == 2 && __is_same(G, void);
+
+bool read_twice(int64_t T, int D)
+{
+    const char *e = getenv("LENS_AMD_SCAN_LAUNCHES");
+    const int force = e ? atoi(e) : 0;
+    return force == 3 || (force != 1 && T * D >= MANY_ELEMENTS);
+}
+
+void put_shape(ScanArgs &p, const Shape &s, int run)
+{
+    p.cg = s.cg; p.ny = s.ny; p.lanes = s.lanes; p.ts = s.ts; p.run = run;
+    p.tiles = (int)tiles_of(p.T, (int64_t)run * s.ts);
+}
+
+// The grid of a pass of three launches / of one; 0 workgroups: more than a launch has.
+dim3 put_twice(ScanArgs &p, unsigned char *scratch, bool back)
+{
+    const Shape s = shape_of(p.D, 256);
+    const Scratch r = scratch_of(p.T, p.D, back);
+    put_shape(p, s, run_of(p.T, s));
+    p.agg = (float2 *)(scratch + r.agg);
+    p.entry = p.tiles > FEW_TILES ? (float *)(scratch + r.entry) : nullptr;
+    p.pre = (float *)(scratch + r.pre);
+    p.part = (float *)(scratch + r.part);
+    return dim3((int64_t)p.tiles * 256 > MAX_THREADS ? 0 : p.tiles, s.ny);
+}
+
+template <typename G>
+unsigned put_once(ScanArgs &p, unsigned char *scratch, bool back, int batches)
+{
+    const Shape s = shape_of(p.D, ONCE);
+    const Scratch r = scratch_of(p.T, p.D, back);
+    put_shape(p, s, batches * B);
+    p.ticket = (unsigned *)(scratch + r.ticket);
+    p.words = (uint64_t *)(scratch + r.words);
+    p.part = (float *)(scratch + r.part);
+    words_of(p.tiles, p.D, group_bits<G>, p.levels);
+    const int64_t n = (int64_t)p.tiles * s.ny;
+    return n * ONCE > MAX_THREADS ? 0 : (unsigned)n;
+}
+
+template <typename G>
+void launch_clear(const ScanArgs &p, hipStream_t st)
+{
+    int levels;
+    const int64_t n = (words_of(p.tiles, p.D, group_bits<G>, levels) + 1) / 2, blocks = (n + 1023) / 1024;
+    if (p.tiles > 1)
+        hipLaunchKernelGGL(k_scan_clear, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (uint4 *)p.words, n, p.ticket);
+}
+
+// Batches of a thread in one pass: two where their rows fit its registers, but one where two would leave a CU without a tile.
+int batches_of(const ScanArgs &p)
+{
+    const Shape s = shape_of(p.D, ONCE);
+    return tiles_of(p.T, 2 * B * s.ts) * s.ny < NUM_CUS ? 1 : 2;
 }
 
 template <typename G>
@@ -999,37 +1454,68 @@ void launch_join(const ScanArgs &p, hipStream_t st)
     if (p.entry) hipLaunchKernelGGL(k_scan_join<G>, dim3((p.D + 3) / 4), dim3(1024), 0, st, p.agg, p.entry, p.tiles, p.D);
 }
 
-template <int V, int B, typename X, typename G>
-void launch_forward_of(const ScanArgs &p, hipStream_t st)
+int launch_no_rows(const float *from, float *to, int64_t n, float *rate, int D, hipStream_t st)
 {
-    const dim3 grid(p.tiles, p.ny), block(p.lanes * p.ts);
-    const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
-    if (p.T > 0) {
-        hipLaunchKernelGGL((k_scan_pairs<V, B, X, G>), grid, block, lds, st, p);
-        launch_join<G>(p, st);
-    }
-    hipLaunchKernelGGL((k_scan_states<V, B, X, G>), grid, block, lds, st, p);
+    const int64_t most = n > D ? n : D, blocks = (most + 255) / 256;
+    hipLaunchKernelGGL(k_scan_no_rows, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st, from, to, n, rate, D);
+    return (int)hipGetLastError();
 }
 
-template <int V, typename X, typename G>
-int launch_forward(const ScanArgs &p, hipStream_t st)
+template <int V, int NB, typename X, typename G>
+int launch_once(ScanArgs &p, unsigned char *scratch, hipStream_t st)
 {
-    constexpr int B = 8;
-    if (p.run >= B) launch_forward_of<V, B, X, G>(p, st);
-    else launch_forward_of<V, 8, X, G>(p, st);
+    const unsigned grid = put_once<G>(p, scratch, false, NB);
+    if (!grid) return LENS_ERR_SIZE;
+    launch_clear<G>(p, st);
+    hipLaunchKernelGGL((k_scan_once<V, NB, X, G>), dim3(grid), dim3(p.lanes * p.ts), LdsOnce<V>::bytes(p.ts, p.lanes, p.levels, p.run), st, p);
     return (int)hipGetLastError();
 }
 
 template <int V, typename X, typename G>
-int launch_backward(const ScanArgs &p, hipStream_t st)
+int launch_forward(ScanArgs &p, unsigned char *scratch, hipStream_t st)
 {
-    const dim3 grid(p.tiles, p.ny), block(p.lanes * p.ts);
-    const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
-    if (p.T > 0) {
-        hipLaunchKernelGGL((k_scan_back_pairs<V, MARK_ROWS, X, G>), grid, block, lds, st, p);
-        launch_join<G>(p, st);
-    }
-    hipLaunchKernelGGL((k_scan_back<V, MARK_ROWS, X, G>), grid, block, lds, st, p);
+    if constexpr (either_way<X, G>)
+        if (read_twice(p.T, p.D)) {
+            const dim3 grid = put_twice(p, scratch, false), block(p.lanes * p.ts);
+            if (!grid.x) return LENS_ERR_SIZE;
+            const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
+            hipLaunchKernelGGL((k_scan_pairs<V, X, G>), grid, block, lds, st, p);
+            launch_join<G>(p, st);
+            hipLaunchKernelGGL((k_scan_states<V, X, G>), grid, block, lds, st, p);
+            return (int)hipGetLastError();
+        }
+    if constexpr (sizeof(X) + (__is_same(G, void) ? 0 : sizeof(gate_or_char<G>)) <= 4)
+        if (batches_of(p) == 2) return launch_once<V, 2, X, G>(p, scratch, st);
+    return launch_once<V, 1, X, G>(p, scratch, st);
+}
+
+template <int V, int NB, typename X, typename G>
+int launch_back_once(ScanArgs &p, unsigned char *scratch, hipStream_t st)
+{
+    const unsigned grid = put_once<G>(p, scratch, true, NB);
+    if (!grid) return LENS_ERR_SIZE;
+    launch_clear<G>(p, st);
+    hipLaunchKernelGGL((k_scan_back_once<V, NB, X, G>), dim3(grid), dim3(p.lanes * p.ts), LdsOnce<V>::bytes(p.ts, p.lanes, p.levels, p.run), st, p);
+    return (int)hipGetLastError();
+}
+
+template <int V, typename X, typename G>
+int launch_backward(ScanArgs &p, unsigned char *scratch, hipStream_t st)
+{
+    int status = 0;
+    bool done = false;
+    if constexpr (either_way<X, G>)
+        if (read_twice(p.T, p.D)) {
+            const dim3 grid = put_twice(p, scratch, true), block(p.lanes * p.ts);
+            if (!grid.x) return LENS_ERR_SIZE;
+            const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
+            hipLaunchKernelGGL((k_scan_back_pairs<V, X, G>), grid, block, lds, st, p);
+            launch_join<G>(p, st);
+            hipLaunchKernelGGL((k_scan_back<V, X, G>), grid, block, lds, st, p);
+            done = true;
+        }
+    if (!done) status = batches_of(p) == 2 ? launch_back_once<V, 2, X, G>(p, scratch, st) : launch_back_once<V, 1, X, G>(p, scratch, st);
+    if (status) return status;
     if (__is_same(G, void))
         hipLaunchKernelGGL(k_scan_rate, dim3((p.D + 15) / 16), dim3(1024), 0, st, p.part, p.grad_rate, p.tiles, p.D);
     return (int)hipGetLastError();
@@ -1064,13 +1550,13 @@ int by_types(int V, int x_type, bool gates, int gate_type, F f)
 }
 
 struct ForwardCall {
-    ScanArgs &p; hipStream_t st;
-    template <int V, typename X, typename G> int go() { return launch_forward<V, X, G>(p, st); }
+    ScanArgs &p; unsigned char *scratch; hipStream_t st;
+    template <int V, typename X, typename G> int go() { return launch_forward<V, X, G>(p, scratch, st); }
 };
 
 struct BackwardCall {
-    ScanArgs &p; hipStream_t st;
-    template <int V, typename X, typename G> int go() { return launch_backward<V, X, G>(p, st); }
+    ScanArgs &p; unsigned char *scratch; hipStream_t st;
+    template <int V, typename X, typename G> int go() { return launch_backward<V, X, G>(p, scratch, st); }
 };
 
 struct StepCall {
@@ -1110,7 +1596,7 @@ extern "C" {
 int lens_scan_mark_rows(int D)
 {
     if (D < 1 || D > LENS_SCAN_MAX_DIM) return 0;
-    return MARK_ROWS;
+    return B;
 }
 
 size_t lens_gated_scan_scratch_bytes(int64_t T, int D, int backward)
@@ -1128,18 +1614,12 @@ int lens_gated_scan(const void *d_x, int x_type, int64_t ldx, const void *d_gate
     if (!d_last || !d_scratch || (T > 0 && !d_h)) return LENS_ERR_NULL;
     if ((T > 1 && ldh < D) || ldh > LENS_SCAN_MAX_LD) return LENS_ERR_SIZE;
     if (off_element(d_h, x_type) || (((uintptr_t)d_last | (uintptr_t)d_marks) & 3) || ((uintptr_t)d_scratch & 15)) return LENS_ERR_ALIGN;
-    const Shape s = shape_of(T, D);
-    const Scratch r = scratch_of(T, D, false);
-    if (scratch_bytes < r.bytes) return LENS_ERR_SCRATCH;
-    if (r.tiles * 256 > MAX_THREADS) return LENS_ERR_SIZE;
-    unsigned char *base = (unsigned char *)d_scratch;
+    if (scratch_bytes < scratch_of(T, D, false).bytes) return LENS_ERR_SCRATCH;
+    if (T == 0) return launch_no_rows(d_h0, d_last, (int64_t)n_seq * D, nullptr, D, (hipStream_t)stream);
     ScanArgs p = {};
     p.x = d_x; p.gate = d_gate; p.dt = d_dt; p.rate = d_rate; p.off = d_seq_off; p.h0 = d_h0; p.h = d_h; p.last = d_last;
-    p.marks = d_marks; p.agg = (float2 *)(base + r.agg); p.pre = (float *)(base + r.pre);
-    p.entry = r.tiles > FEW_TILES ? (float *)(base + r.entry) : nullptr;
-    p.T = T; p.ldx = (int)ldx; p.ldg = (int)ldg; p.ldh = (int)ldh; p.n_seq = n_seq; p.D = D; p.cg = s.cg;
-    p.lanes = s.lanes; p.ts = s.ts; p.run = s.run; p.ny = s.ny; p.fill = fill; p.tiles = (int)r.tiles;
-    return by_types(s.V, x_type, d_rate == nullptr, gate_type, ForwardCall{p, (hipStream_t)stream});
+    p.marks = d_marks; p.T = T; p.ldx = (int)ldx; p.ldg = (int)ldg; p.ldh = (int)ldh; p.n_seq = n_seq; p.D = D; p.fill = fill;
+    return by_types(D >= 4 ? 4 : 1, x_type, d_rate == nullptr, gate_type, ForwardCall{p, (unsigned char *)d_scratch, (hipStream_t)stream});
 }
 
 int lens_gated_scan_grad(const void *d_grad_h, int64_t ld_grad, const float *d_grad_last, const void *d_x, int x_type, int64_t ldx,
@@ -1157,20 +1637,14 @@ int lens_gated_scan_grad(const void *d_grad_h, int64_t ld_grad, const float *d_g
     if ((((uintptr_t)d_grad_last | (uintptr_t)d_marks | (uintptr_t)d_grad_rate | (uintptr_t)d_grad_h0) & 3) ||
         ((uintptr_t)d_scratch & 15))
         return LENS_ERR_ALIGN;
-    const Shape s = shape_of(T, D);
-    const Scratch r = scratch_of(T, D, true);
-    if (scratch_bytes < r.bytes) return LENS_ERR_SCRATCH;
-    if (r.tiles * 256 > MAX_THREADS) return LENS_ERR_SIZE;
-    unsigned char *base = (unsigned char *)d_scratch;
+    if (scratch_bytes < scratch_of(T, D, true).bytes) return LENS_ERR_SCRATCH;
+    if (T == 0) return launch_no_rows(d_grad_last, d_grad_h0, (int64_t)n_seq * D, d_rate ? d_grad_rate : nullptr, D, (hipStream_t)stream);
     ScanArgs p = {};
     p.x = d_x; p.gate = d_gate; p.grad = d_grad_h; p.dt = d_dt; p.rate = d_rate; p.off = d_seq_off; p.h0 = d_h0;
     p.grad_last = d_grad_last; p.grad_x = d_grad_x; p.grad_gate = d_grad_gate; p.grad_h0 = d_grad_h0; p.grad_rate = d_grad_rate;
-    p.marks_in = d_marks; p.agg = (float2 *)(base + r.agg); p.pre = (float *)(base + r.pre);
-    p.entry = r.tiles > FEW_TILES ? (float *)(base + r.entry) : nullptr;
-    p.part = (float *)(base + r.part);
-    p.T = T; p.ldx = (int)ldx; p.ldg = (int)ldg; p.ld_grad = (int)ld_grad; p.ld_gx = (int)ld_gx; p.ld_gg = (int)ld_gg;
-    p.n_seq = n_seq; p.D = D; p.cg = s.cg; p.lanes = s.lanes; p.ts = s.ts; p.run = s.run; p.ny = s.ny; p.tiles = (int)r.tiles;
-    return by_types(s.V, x_type, d_rate == nullptr, gate_type, BackwardCall{p, (hipStream_t)stream});
+    p.marks_in = d_marks; p.T = T; p.ldx = (int)ldx; p.ldg = (int)ldg; p.ld_grad = (int)ld_grad; p.ld_gx = (int)ld_gx;
+    p.ld_gg = (int)ld_gg; p.n_seq = n_seq; p.D = D;
+    return by_types(D >= 4 ? 4 : 1, x_type, d_rate == nullptr, gate_type, BackwardCall{p, (unsigned char *)d_scratch, (hipStream_t)stream});
 }
 
 int lens_gated_step(const float *d_state, int64_t lds, const void *d_x, int x_type, int64_t ldx,

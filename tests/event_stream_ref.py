@@ -6,8 +6,9 @@ Lookup: scale * w and its product with the element round once each, the output o
 Table gradient: a sum of n terms, each fma rounding once, in any order and grouping: (n + 3) u times the sum of magnitudes.
 Scan: with S_t = |a_t| S_{t-1} + |x_t| every |h_t| <= S_t.  A step rounds its product and its sum, and a run of rows that is
 joined to another rounds the factor and the sum of its pair once a row: 8 u S_t covers these.  A decay a = exp(z), z = -dt rate:
-z is rounded (u |z|, relative in a), so is its product with log2 e (u |z|); the exponential is good to 2 u, the series below 1/16 to
-5 u of 1/16.  A run's z is a sum of at most 16 terms: 15 u more of it, shared out over its rows.  So (8 + 20 |z_t|) u S_t.
+z is rounded (u |z|, relative in a), so is its product with log2 e (u |z|); the exponential is good to 2 u, the polynomial below
+1/2 to 2.5 u of what it is there, 1/2 at most.  A run's z is a sum of at most 128 terms, 8 at a time in pairs (3 roundings) and these
+one after the other (15): 18 u more of it, shared out over its rows.  So (8 + 20 |z_t|) u S_t.
 Results below the normal numbers are rounded to a multiple of 2^-149, not relative to themselves: up to 2^-150 for each of a
 row's four roundings; and an exponential below 2^-126 is zero, which is 2^-126 of what it multiplies.
 An error made at a row decays as the state does: E_t = |a_t| E_{t-1} + (8 + 20 |z_t|) u S_t + 4 2^-150 + 2^-126 S_{t-1}.

@@ -220,6 +220,57 @@ def test_scan_many_sequences_of_every_length():
     run_scan(x, d, off, rnd(g, S, D), rnd(g, T, D), rnd(g, S, D))
 
 
+@pytest.mark.parametrize("launches", ["1", "3"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scan_of_16_bit_rows_both_ways(dtype, launches, monkeypatch):
+    """16-bit rows with decays go in one pass or, where there are many, are read twice: one shape through both."""
+    monkeypatch.setenv("LENS_AMD_SCAN_LAUNCHES", launches)
+    for D in (1, 3, 4, 63, 200, 259):
+        for T, off in ((0, None), (1, None), (8, [0, 8]), (79, None), (257, [3, 3, 100, 256, 256]), (700, [0, 1, 1, 300, 428, 428, 700]), (4001, None)):
+            g = gen(10 * D + T)
+            S = 1 if off is None else len(off) - 1
+            x, d = rnd(g, T, D, dtype=dtype), decays("time", T, D, dtype, g)
+            run_scan(x, d, off, rnd(g, S, D), rnd(g, T, D, dtype=dtype), rnd(g, S, D))
+
+
+def test_scan_of_no_rows():
+    h0, last = rnd(gen(15), 3, 70), rnd(gen(16), 3, 70)
+    off = torch.zeros(4, dtype=torch.int64, device="cuda")
+    x = torch.empty(0, 70, device="cuda")
+    for d in (dict(dt=torch.empty(0, device="cuda"), rate=torch.ones(70, device="cuda")), dict(gate=torch.empty(0, 70, device="cuda"))):
+        h, end, marks = E().gated_scan(x, seq_off=off, h0=h0, marks=True, **d)
+        gx, ga, g0 = E().gated_scan_grad(None, x, marks, seq_off=off, h0=h0, grad_last=last, **d)
+        assert h.shape == gx.shape == (0, 70) and torch.equal(end, h0) and torch.equal(g0, last) and not f64_any(ga)
+
+
+@pytest.mark.parametrize("kind,dtype,launches", [("time", torch.float32, "1"), ("gate", torch.float32, "1"), ("time", torch.bfloat16, "1"),
+                                                 ("time", torch.bfloat16, "3"), ("gate", torch.bfloat16, "1")])
+def test_scan_of_many_tiles(kind, dtype, launches, monkeypatch):
+    """Groups of groups of tiles; more than 256 sequences, most of them of no row, and a long one."""
+    monkeypatch.setenv("LENS_AMD_SCAN_LAUNCHES", launches)
+    g = gen(17)
+    T, D = 70001, 1
+    x, d = rnd(g, T, D, dtype=dtype), decays(kind, T, D, dtype, g)
+    if kind == "time":
+        d["dt"] *= 1e-4
+    run_scan(x, d, None, rnd(g, 1, D), rnd(g, T, D, dtype=dtype), rnd(g, 1, D))
+    cuts = sorted(torch.randint(0, 30000, (300,), generator=g, device="cuda").tolist()) + [30000] * 100 + [T - 2]
+    run_scan(x, d, cuts, rnd(g, len(cuts) - 1, D), rnd(g, T, D, dtype=dtype), None)
+
+
+@pytest.mark.parametrize("kind", ["time", "gate", "gate32"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,D", [(2017, 4096), (2100, 4096), (8401, 1001)])
+def test_scan_of_many_elements(dtype, kind, T, D):
+    """On both sides of 2^23 elements, enough of them for two batches a thread."""
+    g = gen(T)
+    x, d = rnd(g, T, D, dtype=dtype), decays(kind, T, D, dtype, g)
+    if kind == "time":
+        d["dt"] *= 1e-2
+    off = [0, 700, 700, T - 1]
+    run_scan(x, d, off, rnd(g, 3, D), rnd(g, T, D, dtype=dtype), rnd(g, 3, D))
+
+
 def test_scan_without_gradient_of_states_and_expanded_rows():
     g = gen(10)
     T, D = 300, 96
