@@ -43,9 +43,17 @@ __device__ __forceinline__ void store_past(T *p, vec<float, V> v)
     __builtin_nontemporal_store(r, reinterpret_cast<U *>(p));
 }
 
-__device__ __forceinline__ int64_t token_at(const void *tokens, int wide_tokens, int64_t i)
+// The tokens at i, i + step, .. of a list of n, at most its last: their loads are in flight together.
+template <int U>
+__device__ __forceinline__ void tokens_at(const void *tokens, int wide_tokens, int64_t i, int64_t step, int64_t n, int64_t (&k)[U])
 {
-    return wide_tokens ? ((const int64_t *)tokens)[i] : (int64_t)((const int32_t *)tokens)[i];
+    if (wide_tokens) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = ((const int64_t *)tokens)[i + u * step < n ? i + u * step : n - 1];
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = ((const int32_t *)tokens)[i + u * step < n ? i + u * step : n - 1];
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -74,22 +82,24 @@ __global__ void __launch_bounds__(256) k_embed(const EmbedArgs p)
     const int64_t i0 = (int64_t)blockIdx.x * p.rows * EMBED_U + row;
     vec<X, V> v[EMBED_U];
     float f[EMBED_U];
+    int64_t k[EMBED_U];
     bool ok[EMBED_U];
+    tokens_at(p.tokens, p.wide_tokens, i0, p.rows, p.T, k);
+#pragma unroll
+    for (int u = 0; u < EMBED_U; ++u) f[u] = p.scale;
+    if (p.weight)
+#pragma unroll
+        for (int u = 0; u < EMBED_U; ++u) f[u] *= p.weight[i0 + u * p.rows < p.T ? i0 + u * p.rows : p.T - 1];
 #pragma unroll
     for (int u = 0; u < EMBED_U; ++u) {
-        const int64_t i = i0 + u * p.rows;
-        ok[u] = false;
-        if (i >= p.T) continue;
-        const int64_t k = token_at(p.tokens, p.wide_tokens, i);
-        ok[u] = k >= 0 && k < p.V_rows;
-        if (!ok[u] && k != -1 && p.first_bad && cc == 0) atomicMin(p.first_bad, (unsigned long long)i);
-        if (ok[u]) v[u] = load<V>((const X *)p.table + k * p.ld_table + c);
-        f[u] = p.weight ? p.scale * p.weight[i] : p.scale;
+        ok[u] = k[u] >= 0 && k[u] < p.V_rows;
+        if (ok[u]) v[u] = load<V>((const X *)p.table + k[u] * p.ld_table + c);
     }
 #pragma unroll
     for (int u = 0; u < EMBED_U; ++u) {
         const int64_t i = i0 + u * p.rows;
         if (i >= p.T) continue;
+        if (!ok[u] && k[u] != -1 && p.first_bad && cc == 0) atomicMin(p.first_bad, (unsigned long long)i);
         store_past<V>((X *)p.out + i * p.ld_out + c, ok[u] ? wide<V, X>(v[u]) * f[u] : vec<float, V>(0.0f));
     }
 }
@@ -98,11 +108,11 @@ __global__ void __launch_bounds__(256) k_embed(const EmbedArgs p)
 // Sort: stable, least significant digit first, digits of at most SORT_BITS bits.  An element is token << 32 | position, so the
 // sorted list holds both.  A pass counts the digits of every block, adds the counts up for every digit over the blocks,
 // and moves the elements, through LDS in the order of their digits (elements of one digit leave side by side: 32 bytes
-// and more a digit at once instead of 8).  A short list has smaller blocks, and those add the counts up themselves.
+// and more a digit at once instead of 8).
 // Tokens that name no row get the key V_rows and end behind all others.
 // ------------------------------------------------------------------------------------------
 constexpr int SORT_BITS = 9, SORT_THREADS = 256, SORT_WAVES = SORT_THREADS / 64;
-constexpr int SORT_EACH = 16, SORT_EACH_SHORT = 4;           // elements a thread; a short list has more blocks
+constexpr int SORT_EACH = 16;        // elements a thread
 
 struct SortArgs {
     const void *tokens;              // first pass: the caller's; else NULL
@@ -114,19 +124,22 @@ struct SortArgs {
     int wide_tokens, shift, bits, blocks;
 };
 
-__device__ __forceinline__ uint32_t sort_key(const SortArgs &p, int64_t i)
+// The elements at i, i + step, .., the list's last for those behind it.
+template <int U>
+__device__ __forceinline__ void sort_elements(const SortArgs &p, int64_t i, int64_t step, uint64_t (&e)[U])
 {
-    if (!p.tokens) return (uint32_t)(p.from[i] >> 32);
-    const int64_t k = token_at(p.tokens, p.wide_tokens, i);
-    return (uint32_t)(k >= 0 && k < p.V_rows ? k : p.V_rows);
+    if (p.tokens) {
+        int64_t k[U];
+        tokens_at(p.tokens, p.wide_tokens, i, step, p.T, k);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            e[u] = (uint64_t)(uint32_t)(k[u] >= 0 && k[u] < p.V_rows ? k[u] : p.V_rows) << 32 | (uint64_t)(uint32_t)(i + u * step);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) e[u] = p.from[i + u * step < p.T ? i + u * step : p.T - 1];
+    }
 }
 
-__device__ __forceinline__ uint64_t sort_element(const SortArgs &p, int64_t i)
-{
-    return p.tokens ? (uint64_t)sort_key(p, i) << 32 | (uint64_t)i : p.from[i];
-}
-
-template <int SORT_EACH>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_count(const SortArgs p)
 {
     __shared__ int n[1 << SORT_BITS];
@@ -134,12 +147,11 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_count(const SortArgs p)
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) n[d] = 0;
     __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * SORT_THREADS * SORT_EACH + threadIdx.x;
-    uint32_t key[SORT_EACH];
-#pragma unroll
-    for (int r = 0; r < SORT_EACH; ++r) key[r] = base + r * SORT_THREADS < p.T ? sort_key(p, base + r * SORT_THREADS) : 0;
+    uint64_t e[SORT_EACH];
+    sort_elements(p, base, SORT_THREADS, e);
 #pragma unroll
     for (int r = 0; r < SORT_EACH; ++r)
-        if (base + r * SORT_THREADS < p.T) atomicAdd(&n[(key[r] >> p.shift) & (digits - 1)], 1);
+        if (base + r * SORT_THREADS < p.T) atomicAdd(&n[(int)(e[r] >> (32 + p.shift)) & (digits - 1)], 1);
     __syncthreads();
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) p.count[(int64_t)d * p.blocks + blockIdx.x] = n[d];
 }
@@ -181,10 +193,23 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_add(int32_t *__restrict__
     if (threadIdx.x == 0) total[blockIdx.x] = before;
 }
 
-template <int EACH, bool SHORT>
+// The lanes that have the same digit and are `in`.
+__device__ __forceinline__ uint64_t lanes_of(int d, int bits, bool in)
+{
+    const uint64_t all = __ballot(in);
+    uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
+    for (int b = 0; b < bits; ++b) {
+        const uint32_t mine = (uint32_t)(d << (31 - b) >> 31);        // the bit, in every place
+        const uint64_t on = __ballot(mine != 0);
+        lo &= ~((uint32_t)on ^ mine);
+        hi &= ~((uint32_t)(on >> 32) ^ mine);
+    }
+    return (uint64_t)hi << 32 | lo;
+}
+
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
 {
-    constexpr int BLOCK = SORT_THREADS * EACH;
+    constexpr int EACH = SORT_EACH, BLOCK = SORT_THREADS * EACH;
     __shared__ volatile int n[SORT_WAVES][1 << SORT_BITS];   // a wavefront's elements of a digit so far; then where they start
     __shared__ int start[1 << SORT_BITS], goes[1 << SORT_BITS];   // a digit's elements: where they start in the block, in the list
     __shared__ uint64_t sorted[BLOCK];
@@ -192,45 +217,19 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
     const int digits = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t first = (int64_t)blockIdx.x * BLOCK;
     const int here = p.T - first < BLOCK ? (int)(p.T - first) : BLOCK;
-    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) {
+    for (int d = threadIdx.x; d < digits; d += SORT_THREADS)
         for (int k = 0; k < SORT_WAVES; ++k) n[k][d] = 0;
-        start[d] = goes[d] = 0;
-    }
     __syncthreads();
-    if (SHORT) {                                             // start: all elements of a digit; goes: those of earlier blocks
-        for (int d = threadIdx.x; d < digits; d += SORT_THREADS) {
-            const int32_t *row = p.count + (int64_t)d * p.blocks;
-            int all = 0, earlier = 0;
-            for (int k0 = 0; k0 < p.blocks; k0 += 8) {
-                int v[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = row[k0 + k < p.blocks ? k0 + k : p.blocks - 1];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    all += k0 + k < p.blocks ? v[k] : 0;
-                    earlier += k0 + k < (int)blockIdx.x ? v[k] : 0;
-                }
-            }
-            start[d] = all;
-            goes[d] = earlier;
-        }
-        __syncthreads();
-    }
     // every wavefront takes 64 x EACH elements that follow each other, 64 at a time: their order is the list's
     const int base = wave * (64 * EACH) + lane;
     uint64_t e[EACH];
     int rank[EACH];
-#pragma unroll
-    for (int r = 0; r < EACH; ++r) e[r] = base + r * 64 < here ? sort_element(p, first + base + r * 64) : 0;
+    sort_elements(p, first + base, 64, e);
 #pragma unroll
     for (int r = 0; r < EACH; ++r) {
         const bool in = base + r * 64 < here;
         const int d = (int)(e[r] >> (32 + p.shift)) & (digits - 1);
-        uint64_t same = __ballot(in);
-        for (int b = 0; b < p.bits; ++b) {
-            const uint64_t on = __ballot((d >> b) & 1);
-            same &= ((d >> b) & 1) ? on : ~on;
-        }
+        const uint64_t same = lanes_of(d, p.bits, in);
         const int below = __builtin_popcountll(same & ((1ull << lane) - 1));
         int at = 0;
         if (in) at = n[wave][d];
@@ -247,10 +246,10 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
         int mine = 0, all, all_here;
         if (d < digits)
             for (int k = 0; k < SORT_WAVES; ++k) mine += n[k][d];
-        const int list = sum_before(d < digits ? (SHORT ? start[d] : p.total[d]) : 0, part, all);
+        const int list = sum_before(d < digits ? p.total[d] : 0, part, all);
         const int block = sum_before(mine, part, all_here);
         if (d < digits) {
-            goes[d] = before + list + (SHORT ? goes[d] : p.count[(int64_t)d * p.blocks + blockIdx.x]);
+            goes[d] = before + list + p.count[(int64_t)d * p.blocks + blockIdx.x];
             start[d] = before_here + block;
             int at = before_here + block;
             for (int k = 0; k < SORT_WAVES; ++k) {
@@ -271,6 +270,171 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
         const uint64_t v = sorted[i];
         const int d = (int)(v >> (32 + p.shift)) & (digits - 1);
         p.to[(int64_t)goes[d] + (i - start[d])] = v;
+    }
+}
+
+// A list of at most SORT_FEW tokens, in one launch: a workgroup for every `span` rows reads all tokens (240 KB for 30 K events:
+// from L2), counts the smaller ones, picks its own and sorts them by counting their digits -- one pass, unless it has more than
+// 1024 rows.  Against the launches above, us a list of int32 tokens of 32768 rows (of 179920):
+//   500 events  8 / 30 (10 / 35)     5000  9 / 35 (10 / 41)     30011  16 / 37 (17 / 42)     65536  25 / 37 (27 / 42)
+// What a workgroup picks it sorts alone: half of the events at one row cost 41 / 41 (45 / 46) at 30011, 83 / 41 (93 / 46) at
+// 65536, and two rows with all 57 / 41 (64 / 46) and 117 / 41 (132 / 46).  So up to 32 K, where that costs little.
+constexpr int FEW_THREADS = 1024, FEW_WAVES = FEW_THREADS / 64, FEW_GROUPS = 256, FEW_U = 8, FEW_EACH = 8;
+constexpr int FEW_BITS = 10;                                 // of a digit at most: a thread a digit
+constexpr int64_t SORT_FEW = 32 * FEW_THREADS;
+
+// The keys of the tokens at i, i + 64, .., the list's last for those behind it.
+__device__ __forceinline__ void few_keys(const SortArgs &p, int i, uint32_t (&key)[FEW_U])
+{
+    const uint32_t last = (uint32_t)p.T - 1, rows = (uint32_t)p.V_rows;
+    uint32_t at[FEW_U];
+#pragma unroll
+    for (int u = 0; u < FEW_U; ++u) at[u] = (uint32_t)(i + u * 64) < last ? i + u * 64 : last;
+    if (p.wide_tokens) {
+        uint64_t k[FEW_U];
+#pragma unroll
+        for (int u = 0; u < FEW_U; ++u) k[u] = ((const uint64_t *)p.tokens)[at[u]];
+#pragma unroll
+        for (int u = 0; u < FEW_U; ++u) key[u] = k[u] >> 32 ? rows : (uint32_t)k[u];
+    } else {
+#pragma unroll
+        for (int u = 0; u < FEW_U; ++u) key[u] = ((const uint32_t *)p.tokens)[at[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < FEW_U; ++u) key[u] = key[u] < rows ? key[u] : rows;
+}
+
+__global__ void __launch_bounds__(FEW_THREADS) k_sort_few(const SortArgs p, uint64_t *other, uint32_t span, int passes)
+{
+    __shared__ int picked[FEW_WAVES], smaller[FEW_WAVES], part[(1 << FEW_BITS) / 64];
+    __shared__ int goes[1 << FEW_BITS];                     // where the next element of a digit goes
+    __shared__ volatile int n_wave[FEW_WAVES][1 << FEW_BITS];   // a wavefront's elements of a digit so far; then where they go
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int T = (int)p.T, rounds = (T + FEW_THREADS - 1) / FEW_THREADS, first = wave * rounds * 64 + lane;
+    const int end = (wave + 1) * rounds * 64 < T ? (wave + 1) * rounds * 64 : T;
+    const uint32_t lo = blockIdx.x * span;
+    const uint64_t lower = (1ull << lane) - 1;
+    uint64_t mine = 0;                                       // lane k: the lanes whose token of round k is picked
+    int n_mine = 0, n_smaller = 0;
+    for (int r = 0; r < rounds; r += FEW_U) {
+        uint32_t key[FEW_U];
+        few_keys(p, first + r * 64, key);
+#pragma unroll
+        for (int u = 0; u < FEW_U; ++u) {
+            const bool there = first + (r + u) * 64 < end;
+            const uint64_t in = __ballot(there && key[u] - lo < span);
+            n_smaller += __builtin_popcountll(__ballot(there && key[u] < lo));
+            n_mine += __builtin_popcountll(in);
+            if (lane == r + u) mine = in;
+        }
+    }
+    if (lane == 0) {
+        picked[wave] = n_mine;
+        smaller[wave] = n_smaller;
+    }
+    __syncthreads();
+    int start = 0, at = 0, n = 0;
+    for (int k = 0; k < FEW_WAVES; ++k) {
+        start += smaller[k];
+        at += k < wave ? picked[k] : 0;
+        n += picked[k];
+    }
+    if (n == 0) return;
+    // the picked ones in the list's order, where an odd number of passes leads from there to p.to
+    uint64_t *list = (passes & 1 ? other : p.to) + start, *next = (passes & 1 ? p.to : other) + start;
+    for (int r = 0; r < rounds; r += FEW_U) {
+        uint64_t in[FEW_U], any = 0;
+        uint32_t key[FEW_U];
+#pragma unroll
+        for (int u = 0; u < FEW_U; ++u) any |= in[u] = r + u < rounds ? __shfl(mine, r + u, 64) : 0;
+        if (!any) continue;
+        few_keys(p, first + r * 64, key);
+#pragma unroll
+        for (int u = 0; u < FEW_U; ++u) {
+            if (in[u] >> lane & 1) list[at + __builtin_popcountll(in[u] & lower)] = (uint64_t)key[u] << 32 | (uint32_t)(first + (r + u) * 64);
+            at += __builtin_popcountll(in[u]);
+        }
+    }
+    // passes over the digits, in chunks of FEW_EACH elements a thread; a wavefront's follow each other
+    constexpr int CHUNK = FEW_THREADS * FEW_EACH;
+    const int digits = 1 << p.bits;
+    for (int pass = 0; pass < passes; ++pass) {
+        auto digit = [&](uint64_t e) { return (int)(((uint32_t)(e >> 32) - lo) >> (pass * p.bits)) & (digits - 1); };
+        for (int d = threadIdx.x; d < digits; d += FEW_THREADS) goes[d] = 0;
+        __syncthreads();
+        if (n > CHUNK) {                                     // else the only chunk's counts are those of all
+            for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < n; i0 += CHUNK) {
+                uint64_t e[FEW_EACH];
+#pragma unroll
+                for (int r = 0; r < FEW_EACH; ++r) e[r] = list[i0 + r * FEW_THREADS < n ? i0 + r * FEW_THREADS : n - 1];
+#pragma unroll
+                for (int r = 0; r < FEW_EACH; ++r)
+                    if (i0 + r * FEW_THREADS < n) atomicAdd(&goes[digit(e[r])], 1);
+            }
+            __syncthreads();
+        }
+        for (int c0 = 0; c0 < n; c0 += CHUNK) {
+            const int here = n - c0 < CHUNK ? n - c0 : CHUNK, per = (here + FEW_THREADS - 1) / FEW_THREADS;
+            const int base = wave * 64 * per + lane;
+            uint64_t e[FEW_EACH];
+            int rank[FEW_EACH];
+            for (int d = threadIdx.x; d < FEW_WAVES << p.bits; d += FEW_THREADS) n_wave[d >> p.bits][d & (digits - 1)] = 0;
+#pragma unroll
+            for (int r = 0; r < FEW_EACH; ++r) e[r] = r < per ? list[c0 + (base + r * 64 < here ? base + r * 64 : here - 1)] : 0;
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < FEW_EACH; ++r) {
+                if (r >= per) break;
+                const bool in = base + r * 64 < here;
+                const int d = digit(e[r]);
+                const uint64_t same = lanes_of(d, p.bits, in);
+                const int below = __builtin_popcountll(same & lower);
+                int before = 0;
+                if (in) before = n_wave[wave][d];
+                __builtin_amdgcn_wave_barrier();
+                if (in && below == 0) n_wave[wave][d] = before + __builtin_popcountll(same);
+                __builtin_amdgcn_wave_barrier();
+                rank[r] = before + below;
+            }
+            __syncthreads();
+            const int mine_d = threadIdx.x;                  // a thread a digit: where its elements go, of every wavefront
+            if (c0 == 0) {
+                int c = 0, s = 0;
+                if (mine_d < digits) {
+                    if (n > CHUNK) c = goes[mine_d];
+                    else
+                        for (int k = 0; k < FEW_WAVES; ++k) c += n_wave[k][mine_d];
+                }
+                s = c;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int o = __shfl_up(s, d, 64);
+                    if (lane >= d) s += o;
+                }
+                if (lane == 63) part[wave] = s;
+                __syncthreads();
+                if (mine_d < digits) {
+                    for (int k = 0; k < wave; ++k) s += part[k];
+                    goes[mine_d] = s - c;
+                }
+            }
+            if (mine_d < digits) {
+                int to = goes[mine_d];
+                for (int k = 0; k < FEW_WAVES; ++k) {
+                    const int m = n_wave[k][mine_d];
+                    n_wave[k][mine_d] = to;
+                    to += m;
+                }
+                goes[mine_d] = to;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < FEW_EACH; ++r)
+                if (r < per && base + r * 64 < here) next[n_wave[wave][digit(e[r])] + rank[r]] = e[r];
+            __syncthreads();
+        }
+        uint64_t *const was = list;
+        list = next;
+        next = was;
     }
 }
 
@@ -346,7 +510,7 @@ __device__ __forceinline__ int channel(int k, int lane, int D, int &skip)
 template <int V, int NV, int G, typename X, bool WEIGHTS>
 __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
 {
-    constexpr int NG = 256 / G;
+    constexpr int NG = 256 / G, U = NV < 4 ? GRAD_U : GRAD_U / 2;
     __shared__ int32_t keys[NG * GRAD_ITEMS], index[NG * GRAD_ITEMS];
     __shared__ int64_t ends[2];
     __shared__ int32_t before_first;                 // the key before the workgroup's first token, -1: none
@@ -388,7 +552,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     int64_t r = r0;
     const bool begun0 = (t0 > 0 ? keys[t0 - 1] : before_first) == r0;     // the row begins before this group
     bool begun = begun0;
-    Row<V, NV> acc, head, row;
+    Row<V, NV> acc, head;
     acc.zero();
     head.zero();
     auto end_row = [&]() {
@@ -403,20 +567,25 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
         acc.zero();
         ++r;
     };
-    int64_t held = -1;               // row of the table that `row` holds
-    for (int t = t0; t < t1; t += GRAD_U) {
-        vec<X, V> g[GRAD_U][NV];
-        float f[GRAD_U];
+    for (int t = t0; t < t1; t += U) {
+        vec<X, V> g[U][NV], w[WEIGHTS ? U : 1][NV];         // w: of the table
+        float f[U];
 #pragma unroll
-        for (int u = 0; u < GRAD_U; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int tt = t + u < t1 ? t + u : t1 - 1;
             const int64_t i = index[tt];
             f[u] = p.weight ? p.scale * p.weight[i] : p.scale;
 #pragma unroll
             for (int k = 0; k < NV; ++k) g[u][k] = load<V>((const X *)p.grad + i * p.ld_grad + c[k]);
+            if constexpr (WEIGHTS) {
+                const int64_t v = keys[tt] < p.V_rows ? keys[tt] : p.V_rows - 1;
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+                    if (v >= 0) w[u][k] = load<V>((const X *)p.table + v * p.ld_table + c[k]);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < GRAD_U; ++u) {
+        for (int u = 0; u < U; ++u) {
             if (t + u >= t1) break;
             const int key = keys[t + u];
             while (r < key) end_row();
@@ -425,17 +594,12 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
                 continue;
             }
             if constexpr (WEIGHTS) {
-                if (held != r) {
-#pragma unroll
-                    for (int k = 0; k < NV; ++k) row.v[k] = wide<V, X>(load<V>((const X *)p.table + r * p.ld_table + c[k]));
-                    held = r;
-                }
                 float dot = 0.0f;
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
 #pragma unroll
                     for (int i = 0; i < V; ++i)
-                        if (i >= skip[k]) dot = __builtin_fmaf((float)g[u][k][i], row.v[k][i], dot);
+                        if (i >= skip[k]) dot = __builtin_fmaf((float)g[u][k][i], (float)w[u][k][i], dot);
 #pragma unroll
                 for (int m = G / 2; m > 0; m >>= 1) dot += __shfl_xor(dot, m, G);
                 if (lane == 0) p.grad_weight[index[t + u]] = p.scale * dot;
@@ -568,10 +732,9 @@ Width width_of(int type, int D)
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// A list of this many tokens at most is short (64 blocks, whose counts every block adds up: 256 bytes a digit).
-constexpr int64_t SORT_SHORT = 64 * SORT_THREADS * SORT_EACH_SHORT;
-
 struct SortPlan {
+    bool few;                        // in one launch
+    uint32_t span;                   // then: rows of a workgroup
     int bits, passes, blocks;
     size_t other, count, total, bytes;
 };
@@ -579,16 +742,17 @@ struct SortPlan {
 SortPlan sort_plan(int64_t T, int64_t V_rows)
 {
     SortPlan s;
+    s.few = T <= SORT_FEW;
+    s.span = (uint32_t)((V_rows + FEW_GROUPS) / FEW_GROUPS);      // V_rows and the key of tokens without a row
     int bits = 1;
-    while (bits < 31 && (V_rows >> bits) != 0) ++bits;
-    s.passes = (bits + SORT_BITS - 1) / SORT_BITS;
+    while (bits < 31 && ((s.few ? (int64_t)s.span - 1 : V_rows) >> bits) != 0) ++bits;
+    s.passes = s.few ? (bits + FEW_BITS - 1) / FEW_BITS : (bits + SORT_BITS - 1) / SORT_BITS;
     s.bits = (bits + s.passes - 1) / s.passes;
-    const int64_t block = (int64_t)SORT_THREADS * (T <= SORT_SHORT ? SORT_EACH_SHORT : SORT_EACH);
-    s.blocks = (int)((T + block - 1) / block);
+    s.blocks = (int)((T + SORT_THREADS * SORT_EACH - 1) / (SORT_THREADS * SORT_EACH));
     s.other = 0;
     s.count = up((size_t)T * 8);
-    s.total = s.count + up((size_t)s.blocks * 4 << s.bits);
-    s.bytes = s.total + up((size_t)4 << s.bits);
+    s.total = s.count + (s.few ? 0 : up((size_t)s.blocks * 4 << s.bits));
+    s.bytes = s.total + (s.few ? 0 : up((size_t)4 << s.bits));
     return s;
 }
 
@@ -699,20 +863,21 @@ int lens_sort_tokens(const void *d_tokens, int token_bytes, int64_t T, int64_t n
     p.T = T; p.V_rows = n_rows; p.wide_tokens = token_bytes == 8; p.bits = s.bits; p.blocks = s.blocks;
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid(s.blocks), block(SORT_THREADS);
+    if (s.few) {
+        p.tokens = d_tokens;
+        p.to = list[1];
+        hipLaunchKernelGGL(k_sort_few, dim3((unsigned)((n_rows + s.span) / s.span)), dim3(FEW_THREADS), 0, st, p, list[0], s.span, s.passes);
+        return (int)hipGetLastError();
+    }
     for (int i = 0; i < s.passes; ++i) {
         const int to = (s.passes - 1 - i) & 1 ? 0 : 1;                 // the last pass writes the caller's list
         p.tokens = i == 0 ? d_tokens : nullptr;
         p.from = list[to ^ 1];
         p.to = list[to];
         p.shift = i * s.bits;
-        if (T <= SORT_SHORT) {
-            hipLaunchKernelGGL(k_sort_count<SORT_EACH_SHORT>, grid, block, 0, st, p);
-            hipLaunchKernelGGL((k_sort_move<SORT_EACH_SHORT, true>), grid, block, 0, st, p);
-        } else {
-            hipLaunchKernelGGL(k_sort_count<SORT_EACH>, grid, block, 0, st, p);
-            hipLaunchKernelGGL(k_sort_add, dim3(1 << s.bits), block, 0, st, p.count, p.total, s.blocks);
-            hipLaunchKernelGGL((k_sort_move<SORT_EACH, false>), grid, block, 0, st, p);
-        }
+        hipLaunchKernelGGL(k_sort_count, grid, block, 0, st, p);
+        hipLaunchKernelGGL(k_sort_add, dim3(1 << s.bits), block, 0, st, p.count, p.total, s.blocks);
+        hipLaunchKernelGGL(k_sort_move, grid, block, 0, st, p);
     }
     return (int)hipGetLastError();
 }

@@ -100,6 +100,18 @@ def test_sort_is_stable(T, V):
         assert torch.equal(keys, want) and torch.equal(index, at)
 
 
+@pytest.mark.parametrize("T,V", [(1, 5000000), (30000, 5000000), (65536, 100000000), (65537, 100000000), (2000, 2147483000)])
+def test_sort_of_large_tables_and_few_tokens(T, V):
+    """More rows than a digit has, a list of one token, of two, and one that is sorted the other way."""
+    g = gen(T + V)
+    wide = torch.randint(0, V, (T,), generator=g, device="cuda")
+    one = torch.full((T,), V - 1, device="cuda")
+    two = torch.where(torch.rand(T, generator=g, device="cuda") < 0.5, one, one - 1)
+    for tok in (wide, one, two, torch.arange(T, device="cuda").flip(0) % V, two.int()):
+        want, at = torch.sort(tok.long(), stable=True)
+        assert torch.equal(E().sort_events(tok, V), want << 32 | at)
+
+
 def skewed(T, V, g, dev="cuda"):
     """A tenth of the events at one row, a stretch of rows without any, padding and tokens outside."""
     tok = torch.randint(0, V, (T,), generator=g, device=dev)
