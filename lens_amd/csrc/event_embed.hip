@@ -111,8 +111,10 @@ __global__ void __launch_bounds__(256) k_embed(const EmbedArgs p)
 // and more a digit at once instead of 8).
 // Tokens that name no row get the key V_rows and end behind all others.
 // ------------------------------------------------------------------------------------------
-constexpr int SORT_BITS = 9, SORT_THREADS = 256, SORT_WAVES = SORT_THREADS / 64;
-constexpr int SORT_EACH = 16;        // elements a thread
+// Latency and the issue of a digit's ballots bound it.  2000000 tokens of 179920 rows (16000000), us, by threads x elements of a
+// thread:  512 x 8  49 (273)   512 x 4  61 (355)   512 x 6  62 (313)   256 x 16  58 (311)   1024 x 8  51 (279)
+constexpr int SORT_BITS = 9, SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64;
+constexpr int SORT_EACH = 8;         // elements a thread
 
 struct SortArgs {
     const void *tokens;              // first pass: the caller's; else NULL
@@ -276,9 +278,9 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
 // A list of at most SORT_FEW tokens, in one launch: a workgroup for every `span` rows reads all tokens (240 KB for 30 K events:
 // from L2), counts the smaller ones, picks its own and sorts them by counting their digits -- one pass, unless it has more than
 // 1024 rows.  Against the launches above, us a list of int32 tokens of 32768 rows (of 179920):
-//   500 events  8 / 30 (10 / 35)     5000  9 / 35 (10 / 41)     30011  16 / 37 (17 / 42)     65536  25 / 37 (27 / 42)
-// What a workgroup picks it sorts alone: half of the events at one row cost 41 / 41 (45 / 46) at 30011, 83 / 41 (93 / 46) at
-// 65536, and two rows with all 57 / 41 (64 / 46) and 117 / 41 (132 / 46).  So up to 32 K, where that costs little.
+//   500 events  8 / 25 (10 / 26)     5000  9 / 27 (10 / 30)     30011  16 / 30 (17 / 31)     65536  25 / 30 (27 / 31)
+// What a workgroup picks it sorts alone: half of the events at one row cost 41 / 33 (45 / 35) at 30011, 83 / 34 (93 / 35) at
+// 65536, and two rows with all 57 / 34 (64 / 35) and 117 / 34 (132 / 35).  So up to 32 K, where that costs little.
 constexpr int FEW_THREADS = 1024, FEW_WAVES = FEW_THREADS / 64, FEW_GROUPS = 256, FEW_U = 8, FEW_EACH = 8;
 constexpr int FEW_BITS = 10;                                 // of a digit at most: a thread a digit
 constexpr int64_t SORT_FEW = 32 * FEW_THREADS;
