@@ -104,6 +104,29 @@ def frames_from_events(t, x, y, timebin_ms, roi_dim, t_unit_s=1e-6, t0=None, dev
     return frames, win
 
 
+def event_tokens(t, x, y, p, height, width, t_unit_s=1e-6, device="cuda", one_based=True):
+    """The events of a recording as engine.embed_events and engine.gated_scan take them, on `device`:
+    tokens int32 [T], (polarity * height + y) * width + x with y and x from 0 -- rows of a table of 2 * height * width --
+    and -1 (padding) for events outside of the sensor; dt float32 [T], the seconds since the event before (0 for the first).
+    p > 0 is polarity 1.  window_events gives the offsets that cut them into sequences."""
+    t = np.asarray(t, dtype=np.float64)
+    x, y, p = (np.asarray(v, dtype=np.int64) for v in (x, y, p))
+    if not t.ndim == 1 or not t.shape == x.shape == y.shape == p.shape:
+        raise ValueError("t, x, y and p must be of one length")
+    height, width = int(height), int(width)
+    if height < 1 or width < 1 or 2 * height * width > 2 ** 31 - 1:
+        raise ValueError("2 * height * width must be positive and fit 32 bits")
+    dt = np.diff(t, prepend=t[:1]) * float(t_unit_s)
+    if np.any(dt < 0):
+        raise ValueError("event timestamps must be non-decreasing")
+    if one_based:
+        x, y = x - 1, y - 1
+    inside = (x >= 0) & (x < width) & (y >= 0) & (y < height)
+    tokens = np.where(inside, ((p > 0) * height + y) * width + x, -1).astype(np.int32)
+    dev = torch.device(device)
+    return torch.from_numpy(tokens).to(dev), torch.from_numpy(dt.astype(np.float32)).to(dev)
+
+
 def save_frames(frames, folder, start_index=0):
     """`frame_%05d.png` like collect_data.py:198 (8-bit greyscale)."""
     from PIL import Image

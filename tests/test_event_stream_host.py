@@ -160,3 +160,17 @@ def test_reference_gradients_are_the_differences():
             up = loss(*args)
             args[which][at] -= 2 * e
             assert abs((up - loss(*args)) / (2 * e) - got[at]) < 1e-7 * (1 + abs(got[at]))
+
+
+def test_event_tokens_of_a_recording():
+    from lens_amd.events import event_tokens
+    t, x, y, p = [10.0, 12.0, 12.0, 2012.0, 5000.0], [1, 4, 5, 4, 0], [1, 3, 1, 3, 2], [0, 1, 1, -1, 1]
+    tok, dt = event_tokens(t, x, y, p, height=3, width=4, device="cpu")
+    assert tok.dtype == torch.int32 and tok.tolist() == [0, 23, -1, 11, -1]
+    assert dt.dtype == torch.float32 and dt.tolist() == [np.float32(v) for v in (0, 2e-6, 0, 2e-3, 2.988e-3)]
+    tok, dt = event_tokens(t, x, y, p, 3, 6, t_unit_s=1.0, device="cpu", one_based=False)
+    assert tok.tolist() == [7, -1, 29, -1, 30] and dt.tolist() == [0, 2, 0, 2000, 2988]
+    assert [v.numel() for v in event_tokens([], [], [], [], 3, 4, device="cpu")] == [0, 0]
+    for bad in ((t[::-1], x, y, p, 3, 4), (t, x[:4], y, p, 3, 4), (t, x, y, p, 0, 4), (t, x, y, p, 2 ** 15, 2 ** 15)):
+        with pytest.raises(ValueError):
+            event_tokens(*bad, device="cpu")

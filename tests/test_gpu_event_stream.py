@@ -516,3 +516,28 @@ def test_encoder_pass_in_a_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, want))
         assert torch.equal(state, expect)
+
+
+def test_recording_to_states_and_one_by_one():
+    """Events as a sensor records them -> tokens -> lookup -> states; and the same events one at a time, state carried."""
+    from lens_amd.events import event_tokens, window_events
+    rng = np.random.default_rng(3)
+    T, H, W, D = 300, 12, 16, 40
+    t = np.cumsum(rng.integers(0, 400, T)).astype(np.float64)
+    x, y, p = rng.integers(0, W + 2, T), rng.integers(1, H + 1, T), rng.integers(0, 2, T)
+    off, _ = window_events(t, 10.0)
+    tok, dt = event_tokens(t, x, y, p, H, W)
+    g = gen(50)
+    table, rate = rnd(g, 2 * H * W, D), torch.exp(rnd(g, D) * 2 + 4)
+    rows = E().embed_events(table, tok, scale=0.25)
+    seq = torch.from_numpy(off).cuda()
+    h, last = E().gated_scan(rows, dt=dt, rate=rate, seq_off=seq)
+    a = R.gates(None, dt, rate)
+    want = R.scan(rows, a, off.tolist(), None)
+    R.check(h, want[0], want[3])
+    R.check(last, want[1], want[4])
+    assert (tok == -1).any() and len(off) > 4
+    state = torch.zeros(1, D, device="cuda")
+    for i in range(off[1]):
+        E().event_step(state, table, tok[i:i + 1], scale=0.25, dt=dt[i:i + 1], rate=rate)
+        R.check(state[0], want[0][i], want[3][i])           # scale 1/4 is exact: the same x
