@@ -418,8 +418,8 @@ int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const 
  * d_h       x_type [T][ldh], the states.  Rows of no sequence: zeros where `fill` is not 0, else left as they were.
  * d_last    float [n_seq][D], the last state of every sequence (h0 for one without rows), in 32 bits
  * d_marks   float [ceil(T / lens_scan_mark_rows(D))][D], optional: what lens_gated_scan_grad needs of the states
- * d_h must not overlap the inputs.  |a| <= 1 is assumed to the extent that the product of the gates over some hundred rows
- * must not overflow.  Scratch: lens_gated_scan_scratch_bytes(T, D, 0).
+ * d_h must not overlap the inputs.  |a| <= 1 is assumed to the extent that the product of the gates over the rows of a
+ * sequence must not overflow: products over runs of rows are formed.  Scratch: lens_gated_scan_scratch_bytes(T, D, 0).
  */
 int lens_scan_mark_rows(int D);
 size_t lens_gated_scan_scratch_bytes(int64_t T, int D, int backward);

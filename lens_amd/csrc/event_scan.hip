@@ -67,7 +67,7 @@ __device__ __forceinline__ void store_past(T *p, vec<float, V> v)
 template <typename T>
 __device__ __forceinline__ T *behind(T *base, uint32_t at)
 {
-    return reinterpret_cast<T *>((uintptr_t)base + (uintptr_t)(at * (uint32_t)sizeof(T)));
+    return reinterpret_cast<T *>(reinterpret_cast<std::conditional_t<std::is_const_v<T>, const char, char> *>(base) + at * (uint32_t)sizeof(T));
 }
 
 template <int V, typename T>
@@ -130,6 +130,7 @@ struct ScanArgs {
     int64_t T;
     int ldx, ldg, ldh, ld_grad, ld_gx, ld_gg;
     int n_seq, D, cg, lanes, ts, run, fill, ny, tiles, levels;
+    int few_ends;                      // sequences without rows are seen to by the passes (pass_on)
 };
 
 // ------------------------------------------------------------------------------------------ rows, tiles, sequences
@@ -155,8 +156,10 @@ struct Tile {
     int64_t row0;
     int left;                          // rows from there to the end, FAR at most
     int s_lo, s_hi;
+    bool in_lds;
     const int64_t *off;
-    __device__ __forceinline__ Tile(const ScanArgs &p, int index) : s_lo(1), s_hi(1), off(p.off)
+    const __attribute__((address_space(3))) int64_t *lds;
+    __device__ __forceinline__ Tile(const ScanArgs &p, int index) : s_lo(1), s_hi(1), in_lds(false), off(p.off), lds(nullptr)
     {
         row0 = (int64_t)index * (p.ts * p.run);
         const int64_t n = p.T - row0;
@@ -170,7 +173,8 @@ struct Tile {
         if (!p.off) return;
         if (p.n_seq < FEW_OFFSETS) {
             for (int i = (int)threadIdx.x; i <= p.n_seq; i += blockDim.x) few[i] = p.off[i];
-            off = few;
+            in_lds = true;
+            lds = (const __attribute__((address_space(3))) int64_t *)few;
             s_lo = 0;
             s_hi = p.n_seq + 1;
             __syncthreads();
@@ -185,6 +189,9 @@ struct Tile {
         s_lo = __builtin_amdgcn_readfirstlane(found[0]);
         s_hi = __builtin_amdgcn_readfirstlane(found[1]);
     }
+    // Each memory by its own instruction.  One pointer to either would be a flat address, whose memory the hardware tells by
+    // the base before the instruction's offset is added: a base just before the array is not in LDS.
+    __device__ __forceinline__ int64_t at(int i) const { return in_lds ? lds[i] : off[i]; }
     __device__ __forceinline__ int rel(int64_t row) const
     {
         const int64_t d = row - row0;
@@ -192,31 +199,38 @@ struct Tile {
     }
 };
 
-// Where a row lies.  s: its sequence (-1: before the first, n_seq: behind the last), next: where the following one starts.
+// Where a row lies.  k: how many sequences start at or before it (its own is k - 1; none: 0, or behind the last), next: where
+// the following one starts.
 struct Place {
-    int s, next;
+    int k, next;
     bool live, start;
 };
 
-__device__ __forceinline__ Place locate(const ScanArgs &p, const Tile &tile, int t)
+// How many of offsets lo .. hi - 1 and those before are at most `row`.
+__device__ __forceinline__ int started(const Tile &tile, int lo, int hi, int64_t row)
 {
-    if (!p.off) return {0, tile.left, true, tile.row0 + t == 0};
-    const int64_t row = tile.row0 + t;
-    int lo = tile.s_lo, hi = tile.s_hi;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (tile.off[mid] <= row) lo = mid + 1; else hi = mid;
+        if (tile.at(mid) <= row) lo = mid + 1; else hi = mid;
     }
-    const int s = lo - 1;
-    return {s, s < p.n_seq ? tile.rel(tile.off[s + 1]) : FAR, s >= 0 && s < p.n_seq, s >= 0 && tile.off[s] == row};
+    return lo;
+}
+
+__device__ __forceinline__ Place locate(const ScanArgs &p, const Tile &tile, int t)
+{
+    if (!p.off) return {1, tile.left, true, tile.row0 + t == 0};
+    const int64_t row = tile.row0 + t;
+    const int k = started(tile, tile.s_lo, tile.s_hi, row);
+    return {k, k <= p.n_seq ? tile.rel(tile.at(k)) : FAR, k >= 1 && k <= p.n_seq, k >= 1 && tile.at(k - 1) == row};
 }
 
 __device__ __forceinline__ void advance(const ScanArgs &p, const Tile &tile, Place &w, int t)      // t == w.next
 {
-    ++w.s;
-    while (w.s < p.n_seq && tile.off[w.s + 1] <= tile.row0 + t) ++w.s;                                // sequences without rows
-    w.live = w.s < p.n_seq;
-    w.next = w.live ? tile.rel(tile.off[w.s + 1]) : FAR;
+    const int64_t row = tile.row0 + t;
+    ++w.k;
+    if (w.k <= p.n_seq && tile.at(w.k) <= row) w.k = started(tile, w.k + 1, tile.s_hi, row);       // sequences without rows
+    w.live = w.k <= p.n_seq;
+    w.next = w.live ? tile.rel(tile.at(w.k)) : FAR;
 }
 
 template <int V>
@@ -321,7 +335,7 @@ __device__ __forceinline__ Rows rows_of(const ScanArgs &p, const Tile &tile, Pla
             r.starts |= (start ? 1u : 0u) << j;
             r.ends |= (t + j + 1 == w.next ? 1u : 0u) << j;
         }
-        ids[j] = w.s;                                      // the same from every lane of the rows
+        ids[j] = w.k - 1;                                      // the same from every lane of the rows
         start = false;
     }
     w.start = false;
@@ -623,13 +637,26 @@ __device__ __forceinline__ void put_pair(const Lds<V> &lds, const Own<V> &o, vec
 }
 
 // ------------------------------------------------------------------------------------------ forward
-// A sequence without rows ends as it began: `to` (if any) from `from` (zeros without).  Shared out over `of` workgroups.
+// A sequence without rows ends as it began: `to` (if any) from `from` (zeros without).  A few sequences are shared out over the
+// threads of a pass, workgroup `index` of `of`.
+constexpr int PASS_ON = 4;             // elements a thread at most
+
 __device__ __forceinline__ void pass_on(const ScanArgs &p, const float *from, float *to, int index, int of)
 {
-    if (!p.off || !to) return;
-    for (int64_t s = index; s < p.n_seq; s += of)
-        if (p.off[s] == p.off[s + 1])
-            for (int c = (int)threadIdx.x; c < p.D; c += blockDim.x) to[s * p.D + c] = from ? from[s * p.D + c] : 0.0f;
+    if (!p.few_ends || !to) return;
+    const uint32_t n = (uint32_t)p.n_seq * (uint32_t)p.D;
+    for (uint32_t i = (uint32_t)index * blockDim.x + threadIdx.x; i < n; i += (uint32_t)of * blockDim.x) {
+        const uint32_t s = i / (uint32_t)p.D;
+        if (p.off[s] == p.off[s + 1]) to[i] = from ? from[i] : 0.0f;
+    }
+}
+
+// Many: a wavefront each.
+__global__ void __launch_bounds__(256) k_scan_pass_on(const int64_t *off, int64_t n_seq, const float *from, float *to, int D)
+{
+    for (int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); s < n_seq; s += (int64_t)gridDim.x * 4)
+        if (off[s] == off[s + 1])
+            for (int c = (int)threadIdx.x & 63; c < D; c += 64) to[s * D + c] = from ? from[s * D + c] : 0.0f;
 }
 
 // Instead of everything else where there are no rows at all.
@@ -1448,6 +1475,16 @@ int batches_of(const ScanArgs &p)
     return tiles_of(p.T, 2 * B * s.ts) * s.ny < NUM_CUS ? 1 : 2;
 }
 
+// Before a pass of `threads` threads.
+void launch_pass_on(ScanArgs &p, const float *from, float *to, int64_t threads, hipStream_t st)
+{
+    if (!p.off || !to) return;
+    p.few_ends = (int64_t)p.n_seq * p.D <= PASS_ON * threads;
+    if (p.few_ends) return;
+    const int64_t blocks = ((int64_t)p.n_seq + 3) / 4;
+    hipLaunchKernelGGL(k_scan_pass_on, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st, p.off, (int64_t)p.n_seq, from, to, p.D);
+}
+
 template <typename G>
 void launch_join(const ScanArgs &p, hipStream_t st)
 {
@@ -1467,6 +1504,7 @@ int launch_once(ScanArgs &p, unsigned char *scratch, hipStream_t st)
     const unsigned grid = put_once<G>(p, scratch, false, NB);
     if (!grid) return LENS_ERR_SIZE;
     launch_clear<G>(p, st);
+    launch_pass_on(p, p.h0, p.last, (int64_t)grid * p.lanes * p.ts, st);
     hipLaunchKernelGGL((k_scan_once<V, NB, X, G>), dim3(grid), dim3(p.lanes * p.ts), LdsOnce<V>::bytes(p.ts, p.lanes, p.levels, p.run), st, p);
     return (int)hipGetLastError();
 }
@@ -1479,6 +1517,7 @@ int launch_forward(ScanArgs &p, unsigned char *scratch, hipStream_t st)
             const dim3 grid = put_twice(p, scratch, false), block(p.lanes * p.ts);
             if (!grid.x) return LENS_ERR_SIZE;
             const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
+            launch_pass_on(p, p.h0, p.last, (int64_t)p.tiles * block.x, st);
             hipLaunchKernelGGL((k_scan_pairs<V, X, G>), grid, block, lds, st, p);
             launch_join<G>(p, st);
             hipLaunchKernelGGL((k_scan_states<V, X, G>), grid, block, lds, st, p);
@@ -1495,6 +1534,7 @@ int launch_back_once(ScanArgs &p, unsigned char *scratch, hipStream_t st)
     const unsigned grid = put_once<G>(p, scratch, true, NB);
     if (!grid) return LENS_ERR_SIZE;
     launch_clear<G>(p, st);
+    launch_pass_on(p, p.grad_last, p.grad_h0, (int64_t)grid * p.lanes * p.ts, st);
     hipLaunchKernelGGL((k_scan_back_once<V, NB, X, G>), dim3(grid), dim3(p.lanes * p.ts), LdsOnce<V>::bytes(p.ts, p.lanes, p.levels, p.run), st, p);
     return (int)hipGetLastError();
 }
@@ -1509,6 +1549,7 @@ int launch_backward(ScanArgs &p, unsigned char *scratch, hipStream_t st)
             const dim3 grid = put_twice(p, scratch, true), block(p.lanes * p.ts);
             if (!grid.x) return LENS_ERR_SIZE;
             const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
+            launch_pass_on(p, p.grad_last, p.grad_h0, (int64_t)p.tiles * block.x, st);
             hipLaunchKernelGGL((k_scan_back_pairs<V, X, G>), grid, block, lds, st, p);
             launch_join<G>(p, st);
             hipLaunchKernelGGL((k_scan_back<V, X, G>), grid, block, lds, st, p);

@@ -660,7 +660,7 @@ def gated_scan(x, gate=None, dt=None, rate=None, seq_off=None, h0=None, out=None
 
     x       [T, D] float32 / bfloat16 / float16, the rows of all sequences one behind the other
     gate    [T, D] the a_t (x's type or float32), or dt float32 [T] and rate float32 [D]: a_t = exp(-dt_t rate_d), dt the time
-            since the previous event
+            since the previous event.  Gates above 1 are taken as long as their product over a sequence does not overflow.
     seq_off int64 [S + 1]: rows of sequence s are [seq_off[s], seq_off[s + 1]), possibly none; None: one sequence.  On the device
             it is trusted (non-decreasing, the last at most T); in host memory it is checked, and copied.
     h0      float32 [S, D], the state before every sequence's first row; None: zeros

@@ -107,6 +107,7 @@ def test_sort_of_large_tables_and_few_tokens(T, V):
     wide = torch.randint(0, V, (T,), generator=g, device="cuda")
     one = torch.full((T,), V - 1, device="cuda")
     two = torch.where(torch.rand(T, generator=g, device="cuda") < 0.5, one, one - 1)
+    assert torch.equal(E().sort_events(one, 0), torch.arange(T, device="cuda"))
     for tok in (wide, one, two, torch.arange(T, device="cuda").flip(0) % V, two.int()):
         want, at = torch.sort(tok.long(), stable=True)
         assert torch.equal(E().sort_events(tok, V), want << 32 | at)
@@ -243,6 +244,19 @@ def test_scan_of_16_bit_rows_both_ways(dtype, launches, monkeypatch):
             S = 1 if off is None else len(off) - 1
             x, d = rnd(g, T, D, dtype=dtype), decays("time", T, D, dtype, g)
             run_scan(x, d, off, rnd(g, S, D), rnd(g, T, D, dtype=dtype), rnd(g, S, D))
+
+
+@pytest.mark.parametrize("kind,launches", [("time", "1"), ("time", "3"), ("gate", "1")])
+def test_scan_of_many_sequences_and_few_rows(kind, launches, monkeypatch):
+    """Thousands of streams of which few had an event, and not the first or last ones."""
+    monkeypatch.setenv("LENS_AMD_SCAN_LAUNCHES", launches)
+    g = gen(18)
+    for S, T, D in ((5000, 150, 7), (300, 40, 200), (70001, 9, 3)):
+        at = torch.sort(torch.randint(S // 9, S - S // 9, (T,), generator=g, device="cuda")).values      # the stream of every row
+        off = torch.searchsorted(at, torch.arange(S + 1, device="cuda")).tolist()
+        x, d = rnd(g, T, D, dtype=torch.bfloat16), decays(kind, T, D, torch.bfloat16, g)
+        run_scan(x, d, off, rnd(g, S, D), rnd(g, T, D, dtype=torch.bfloat16), rnd(g, S, D))
+        run_scan(x, d, off, None, None, rnd(g, S, D))
 
 
 def test_scan_of_no_rows():
