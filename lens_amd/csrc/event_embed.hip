@@ -58,7 +58,9 @@ __device__ __forceinline__ void tokens_at(const void *tokens, int wide_tokens, i
 
 // ------------------------------------------------------------------------------------------
 // Lookup.  A workgroup of `rows` x `lanes` threads; every thread reads V channels of EMBED_U rows at once (the rows are
-// anywhere in the table: what hides their latency is the number of loads in flight).
+// anywhere in the table: what hides their latency is the number of loads in flight).  Bytes bound it: 1000003 events of
+// 179920 x 128 bf16 with weights 67 us, 4.6 TB/s of the 310 MB of rows, tokens and weights in and states out; with stores
+// through the caches 87 us.  500 events x 100 f32 are 4 us of latency.
 // ------------------------------------------------------------------------------------------
 constexpr int EMBED_U = 4;
 
@@ -445,6 +447,8 @@ __global__ void __launch_bounds__(FEW_THREADS) k_sort_few(const SortArgs p, uint
 // list: token t stands at place t + key[t], the end of row r behind the last token of r.  A workgroup takes `items` places
 // a group, a group is `G` lanes that hold one row of the table's width, NV vectors each.
 // A row that begins in one group and ends in a later one is joined in LDS, over workgroups by k_grad_join.
+// Bytes bound a large one: 2000000 x 256 bf16 to 179920 rows 260 us, 4.7 TB/s, and 16 us to join; latency a small one: 30011 x 63
+// f32 to 32768 rows, weights too, 14 and 5 us.
 // ------------------------------------------------------------------------------------------
 constexpr int GRAD_ITEMS = 64, GRAD_U = 4;
 
@@ -758,7 +762,8 @@ SortPlan sort_plan(int64_t T, int64_t V_rows)
     return s;
 }
 
-// Places a group of k_grad: as many as leave 1024 workgroups, 8 at least.
+// Places a group of k_grad: as many as leave 1024 workgroups, 8 at least.  By this rule / 64 always / 8 always, us with the
+// sort:  30011 x 63 to 32768 rows  34 / 74 / 35    2000 x 128 to 32768  22 / 27 / 21    2000000 x 256 bf16 to 179920  330 / 329 / 421
 int grad_items(int64_t T, int64_t V_rows, int G)
 {
     int items = GRAD_ITEMS;

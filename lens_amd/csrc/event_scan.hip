@@ -11,7 +11,7 @@
 // they do the rows are read once: a thread keeps its 8 or 16 rows in registers until the pairs of the tiles before have arrived.
 // Where the arithmetic of the rows counts too, three launches take less:
 //   pairs   the pair of every run of 8 to 128 rows; those of a tile are joined in LDS to what is before each, and the tile's
-//   join    what is before every tile (a few tiles are joined by the next launch itself)
+//   join    what is before every tile
 //   states  the states, a row after the other from what enters the run; the tiles in the other order, so that what was read
 //           last comes from the Infinity Cache
 // The order of every composition is fixed by T, D and the types alone: results do not depend on timing.
@@ -122,7 +122,7 @@ struct ScanArgs {
     float *last, *marks, *grad_h0, *grad_rate;
     const float *marks_in;
     float2 *agg;                       // [tiles][D] pairs of the tiles, in the order in which they are joined
-    float *entry;                      // [tiles][D] what enters them; NULL: few tiles, joined by those that need it
+    float *entry;                      // [tiles][D] what enters them
     float *pre;                        // [tiles][ts][2][D] pairs of what is before a run in its tile
     uint64_t *words;                   // one pass: pairs of the tiles and of their groups (Chain)
     unsigned *ticket;
@@ -549,7 +549,8 @@ __device__ __forceinline__ void join_runs(const ScanArgs &p, const Lds<V> &lds, 
 }
 
 // Tiles' pairs -> what enters every tile.  A workgroup holds 4 channels x 256 runs of up to JOIN tiles at once: every thread joins
-// its run, the 16 runs of a wavefront are joined by shuffles, the 16 wavefronts through LDS.
+// its run, the 16 runs of a wavefront are joined by shuffles, the 16 wavefronts through LDS.  Latency: 7 us for 1042 tiles of 200
+// channels.
 constexpr int JOIN = 8;
 
 template <typename G>
@@ -595,32 +596,13 @@ __global__ void __launch_bounds__(1024) k_scan_join(const float2 *__restrict__ a
     }
 }
 
-// What enters a thread's run.  All threads call it.  order: the tile's place among those that are joined.
+// What enters a thread's run.  order: the tile's place among those that are joined.
 template <int V, typename G>
-__device__ __forceinline__ vec<float, V> run_entry(const ScanArgs &p, const Lds<V> &lds, const Own<V> &o, int tile, int y, int order)
+__device__ __forceinline__ vec<float, V> run_entry(const ScanArgs &p, const Own<V> &o, int tile, int order)
 {
     const float *from = p.pre + ((int64_t)tile * p.ts + o.ts) * 2 * p.D + o.c;
     const vec<float, V> f = load<V>(from), H = load<V>(from + p.D);
-    vec<float, V> st;
-    if (p.entry) {
-        st = load<V>(p.entry + (int64_t)order * p.D + o.c);
-    } else {
-        const int slot = (int)threadIdx.x, c = slot < lds.slots ? slot_channel<V>(p, y, slot) : -1;
-        if (c >= 0) {
-            float h = 0.0f;
-            for (int b = 0; b < order; b += 16) {
-                float2 v[16];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = p.agg[(int64_t)(b + k < order ? b + k : order - 1) * p.D + c];
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    if (b + k < order) h = Pair<G>{v[k].x, v[k].y}.over(h);
-            }
-            lds.f[slot] = h;
-        }
-        __syncthreads();
-        st = lds_load<V>(lds.f + o.lane * V);
-    }
+    vec<float, V> st = load<V>(p.entry + (int64_t)order * p.D + o.c);
 #pragma unroll
     for (int i = 0; i < V; ++i) st[i] = Pair<G>{f[i], H[i]}.over(st[i]);
     return st;
@@ -719,6 +701,7 @@ __device__ __forceinline__ void states_batch(const ScanArgs &p, const Tile &tile
     }
 }
 
+// 400009 x 200 bf16 with decays: pairs 39 us, 4.1 TB/s of the rows; states 75 us, 4.3 TB/s of the rows in and out.
 template <int V, typename X, typename G>
 __global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
 {
@@ -771,7 +754,7 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
     };
     if (o.n > 0) load_batch(0);
     tile.find(p);
-    vec<float, V> st = run_entry<V, G>(p, lds, o, index, y, index);
+    vec<float, V> st = run_entry<V, G>(p, o, index, index);
     if (!o.any || o.n == 0) return;
     Place w = locate(p, tile, o.t0);
     X *out = (X *)p.h + tile.row0 * p.ldh;
@@ -795,13 +778,20 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
 // Scratch memory that another call uses at the same time could keep a wait from ending: it is given up after about a second,
 // all others of the launch then at once, and the results are NaN.
 //
-// One pass against reading twice, us a call:
-//   forward    1048573 x 128 bf16, bf16 gates  189 / 253     400009 x 200 bf16, decays  135 / 123     1501 x 200 f32, decays  17 / 19
-//              262144 x 128 f32, decays         72 / 78       30000 x 128 bf16, decays   20 / 22      30000 x 128 f32, f32 gates  18 / 23
-//   backward   524287 x 256 bf16, bf16 gates   317 / 357     400009 x 200 bf16, decays  228 / 193     1501 x 200 f32, decays  23 / 23
-//              262144 x 128 f32, decays        114 / 113      30000 x 128 bf16, decays   26 / 31      30000 x 128 f32, f32 gates  21 / 27
-// So 16-bit rows with decays -- the fewest bytes for the arithmetic of a row -- are read twice when there are many, by
+// One pass against reading twice, us a call (backward: scan and gradients):
+//   gates                 1048573 x 128 bf16, bf16 gates 189 / 253     30000 x 128 f32, f32 gates 18 / 23
+//   gates, backward        524287 x 256 bf16, bf16 gates 317 / 357 (the backward launches)
+//   f32 rows, decays       262144 x 128  72 / 78     1501 x 200  17 / 19     backward  114 / 113  and  23 / 23 (the backward launches)
+//   16-bit rows, decays   of 128 channels, 4 sequences:  16384  20 / 21    32768  22 / 24    65536  26 / 31    131072  35 / 37
+//                         262144  61 / 56    524288  102 / 87     400009 x 200, 37 sequences  135 / 117
+//            backward     16384  46 / 47    32768  50 / 52    65536  60 / 71    131072  89 / 89    262144  160 / 144    524288  281 / 236
+//                         400009 x 200  364 / 296
+// So 16-bit rows with decays -- the fewest bytes for the arithmetic of a row -- are read twice from 16 M elements on, by
 // workgroups that wait for nothing; all others go in one pass.
+//
+// What it reaches: 1048573 x 128 bf16 with gates 186 us, 4.3 TB/s of the 805 MB that have to move (torch's copy of 1 GB:
+// 5.0); 262144 x 128 f32 with decays 72 us, 3.7 TB/s: two rounds of workgroups, each of which loads, waits and stores in step.
+// Outputs past the caches: 185 / 192 us with / without, forward and backward of 262144 x 128 f32 197 / 216.
 constexpr uint64_t EMPTY = ~0ull;
 constexpr int MOST_TRIES = 1 << 20;
 
@@ -1035,7 +1025,8 @@ __global__ void __launch_bounds__(ONCE, 4) k_scan_once(const ScanArgs p)
 // ------------------------------------------------------------------------------------------
 // Backward.  With r_t = a_t g_t the message that row t sends back: g_t = dh_t + r_{t+1}, so a run of rows acts on the
 // message that enters from behind as r -> f r + U with the f of the forward direction.  The states before the rows are
-// computed again from the marks, B rows at a time.
+// computed again from the marks, B rows at a time.  Bytes bound it: 524287 x 256 bf16 with gates 315 us, 4.5 TB/s of the 1.4 GB of
+// x, gates, gradient and marks in and both gradients out; 262144 x 128 f32 with decays 108 us, 3.9 TB/s of 420 MB.
 // ------------------------------------------------------------------------------------------
 // The message before the rows of a batch, from U behind them.
 template <int V, typename X, typename G>
@@ -1158,7 +1149,7 @@ __global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
     const Own<V> o(p, tile, y);
     int *ids = lds.ids + o.ts * B;
     tile.find(p);
-    vec<float, V> r = run_entry<V, G>(p, lds, o, index, y, p.tiles - 1 - index), share(0.0f);
+    vec<float, V> r = run_entry<V, G>(p, o, index, p.tiles - 1 - index), share(0.0f);
     Gates<V, G> g(p, o.c);
     X *gx = (X *)p.grad_x + tile.row0 * p.ld_gx;
     gate_or_char<G> *gg = (gate_or_char<G> *)p.grad_gate + tile.row0 * p.ld_gg;
@@ -1300,7 +1291,9 @@ __global__ void __launch_bounds__(1024) k_scan_rate(const float *__restrict__ pa
 }
 
 // ------------------------------------------------------------------------------------------
-// Single steps of carried states: out = a * state + x, x a row of its own or w * scale * table[token].
+// Single steps of carried states: out = a * state + x, x a row of its own or w * scale * table[token].  A thread 4 channels of a
+// state; everything is the latency of one load behind another (token, row): 2.2 us for one state of 200 channels, of which
+// a call from Python shows 8.5.
 // ------------------------------------------------------------------------------------------
 struct StepArgs {
     const float *state;
@@ -1367,6 +1360,8 @@ Shape shape_of(int D, int threads)
 int64_t tiles_of(int64_t T, int64_t rows) { return (T + rows - 1) / rows; }
 
 // Rows of a run where the rows are read twice: the most that leave 1024 workgroups (four a CU), the fewest where there are less.
+// bf16 rows with decays, us by this rule / 8 always / 128 always:  400009 x 200  116 / 161 / 127, with gradients 297 / 400 / 325;
+// 70001 x 128  33 / 33 / 58, with gradients 75 / 73 / 151.
 constexpr int MOST_RUN = 128;
 
 int run_of(int64_t T, const Shape &s)
@@ -1375,9 +1370,6 @@ int run_of(int64_t T, const Shape &s)
     while (run > B && T * s.ny < (int64_t)1024 * run * s.ts) run /= 2;
     return run;
 }
-
-// Tiles' pairs of at most this many tiles are joined by those that need them, without a launch.
-constexpr int FEW_TILES = 64;
 
 // Words of one pass: those of `tiles` tiles and of all complete groups above them; levels: how many that are.
 int64_t words_of(int64_t tiles, int D, int bits, int &levels)
@@ -1415,7 +1407,7 @@ Scratch scratch_of(int64_t T, int D, bool back)
 
 // Whether 16-bit rows with decays are read twice, in three launches; all others take one pass (measured
 // above).  LENS_AMD_SCAN_LAUNCHES=1/3 forces the choice (tests; read at every call).
-constexpr int64_t MANY_ELEMENTS = 1 << 23;
+constexpr int64_t MANY_ELEMENTS = 1 << 24;
 
 template <typename X, typename G> constexpr bool either_way = sizeof(X) == 2 && __is_same(G, void);
 
@@ -1423,7 +1415,7 @@ bool read_twice(int64_t T, int D)
 {
     const char *e = getenv("LENS_AMD_SCAN_LAUNCHES");
     const int force = e ? atoi(e) : 0;
-    return force == 3 || (force != 1 && T * D >= MANY_ELEMENTS);
+    return force == 3 || (force != 1 && T * D > MANY_ELEMENTS);
 }
 
 void put_shape(ScanArgs &p, const Shape &s, int run)
@@ -1439,7 +1431,7 @@ dim3 put_twice(ScanArgs &p, unsigned char *scratch, bool back)
     const Scratch r = scratch_of(p.T, p.D, back);
     put_shape(p, s, run_of(p.T, s));
     p.agg = (float2 *)(scratch + r.agg);
-    p.entry = p.tiles > FEW_TILES ? (float *)(scratch + r.entry) : nullptr;
+    p.entry = (float *)(scratch + r.entry);
     p.pre = (float *)(scratch + r.pre);
     p.part = (float *)(scratch + r.part);
     return dim3((int64_t)p.tiles * 256 > MAX_THREADS ? 0 : p.tiles, s.ny);
@@ -1469,6 +1461,8 @@ void launch_clear(const ScanArgs &p, hipStream_t st)
 }
 
 // Batches of a thread in one pass: two where their rows fit its registers, but one where two would leave a CU without a tile.
+// One / two, us:  1501 x 200 f32 decays 17.5 / 23.1, 30000 x 128 bf16 gates 17.0 / 17.6;  1048573 x 128 bf16 gates 243 / 184, with
+// gradients 262144 x 128 f32 decays 239 / 199, 524287 x 256 bf16 gates 640 / 507.
 int batches_of(const ScanArgs &p)
 {
     const Shape s = shape_of(p.D, ONCE);
@@ -1488,7 +1482,7 @@ void launch_pass_on(ScanArgs &p, const float *from, float *to, int64_t threads, 
 template <typename G>
 void launch_join(const ScanArgs &p, hipStream_t st)
 {
-    if (p.entry) hipLaunchKernelGGL(k_scan_join<G>, dim3((p.D + 3) / 4), dim3(1024), 0, st, p.agg, p.entry, p.tiles, p.D);
+    hipLaunchKernelGGL(k_scan_join<G>, dim3((p.D + 3) / 4), dim3(1024), 0, st, p.agg, p.entry, p.tiles, p.D);
 }
 
 int launch_no_rows(const float *from, float *to, int64_t n, float *rate, int D, hipStream_t st)

@@ -284,11 +284,10 @@ def test_scan_of_many_tiles(kind, dtype, launches, monkeypatch):
     run_scan(x, d, cuts, rnd(g, len(cuts) - 1, D), rnd(g, T, D, dtype=dtype), None)
 
 
-@pytest.mark.parametrize("kind", ["time", "gate", "gate32"])
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("T,D", [(2017, 4096), (2100, 4096), (8401, 1001)])
+@pytest.mark.parametrize("T,D,dtype,kind", [(t, d, y, k) for t, d in ((2017, 4096), (8401, 1001)) for y in (torch.float32, torch.bfloat16)
+                                            for k in ("time", "gate", "gate32")] + [(4101, 4096, torch.bfloat16, "time")])
 def test_scan_of_many_elements(dtype, kind, T, D):
-    """On both sides of 2^23 elements, enough of them for two batches a thread."""
+    """Enough of them for two batches a thread; more than 2^24, where 16-bit rows with decays are read twice."""
     g = gen(T)
     x, d = rnd(g, T, D, dtype=dtype), decays(kind, T, D, dtype, g)
     if kind == "time":
