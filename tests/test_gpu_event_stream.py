@@ -554,3 +554,74 @@ def test_recording_to_states_and_one_by_one():
     for i in range(off[1]):
         E().event_step(state, table, tok[i:i + 1], scale=0.25, dt=dt[i:i + 1], rate=rate)
         R.check(state[0], want[0][i], want[3][i])           # scale 1/4 is exact: the same x
+
+
+@pytest.mark.parametrize("dtype,kind,launches", [(torch.bfloat16, "time", "1"), (torch.bfloat16, "time", "3"), (torch.bfloat16, "gate", "1"),
+                                                 (torch.float16, "gate32", "1")])
+def test_scan_in_a_graph(dtype, kind, launches, monkeypatch):
+    """Two graphs of different lengths, replayed in turn with eager calls between them."""
+    monkeypatch.setenv("LENS_AMD_SCAN_LAUNCHES", launches)
+    D, calls = 100, []
+    for T, S in ((5003, 3), (801, 700)):
+        g = gen(T)
+        x, d, grad, h0, last = rnd(g, T, D, dtype=dtype), decays(kind, T, D, dtype, g), rnd(g, T, D, dtype=dtype), rnd(g, S, D), rnd(g, S, D)
+        off = torch.sort(torch.randint(0, T, (S + 1,), generator=g, device="cuda")).values
+
+        def run(x=x, d=d, grad=grad, h0=h0, last=last, off=off):
+            h, end, marks = E().gated_scan(x, seq_off=off, h0=h0, marks=True, **d)
+            return (h, end, *E().gated_scan_grad(grad, x, marks, seq_off=off, h0=h0, grad_last=last, **d))
+        run()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            out = run()
+        calls.append((run, graph, out, x, grad, off, g))
+    for _ in range(4):
+        for run, graph, out, x, grad, off, g in calls:
+            x.normal_(generator=g)
+            grad.normal_(generator=g)
+            off.copy_(torch.sort(torch.randint(0, x.shape[0], off.shape, generator=g, device="cuda")).values)
+            want = run()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_offsets_past_32_bits():
+    """Operands of more than 2^32 bytes and 2^31 elements; what lies at their ends against the same in 64 bits."""
+    g = gen(60)
+    T, D, tail = 8400011, 256, 700
+    x = torch.empty(T, D, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    off = torch.tensor([0, 5, T - tail, T - 3], device="cuda")
+    h0, rate = rnd(g, 3, D), torch.exp(rnd(g, D) + 4)
+    for d in (dict(dt=torch.rand(T, generator=g, device="cuda") * 1e-2, rate=rate), dict(gate=torch.sigmoid(x))):
+        h, last, marks = E().gated_scan(x, seq_off=off, h0=h0, marks=True, **d)
+        grad = E().gated_scan_grad(x, x, marks, seq_off=off, h0=h0, **d)
+        s = slice(T - tail, T)
+        a = R.gates(d["gate"][s], None, None) if "gate" in d else R.gates(None, d["dt"][s], rate)
+        want = R.scan(x[s], a, [0, tail - 3], h0[2:])
+        R.check(h[s], want[0], want[3])
+        R.check(last[2:], want[1], want[4])
+        gx, ga, g0, Eg, Ea, E0 = R.scan_grad(x[s], None, x[s], a, d["dt"][s] if "dt" in d else None, [0, tail - 3], h0[2:])
+        R.check(grad[0][s], gx, Eg)
+        R.check(grad[2][2:], g0, E0)
+        if "gate" in d:
+            R.check(grad[1][s], ga, Ea)
+        del h, marks, grad, d
+    at = torch.arange(T - 1, -1, -1, device="cuda")
+    rows = E().embed_events(x, at, check=False)                              # a long table, a long output
+    assert all(torch.equal(rows[i:i + 1000], x[T - 1000 - i:T - i].flip(0)) for i in (0, T // 2, T - 1000))
+    del rows
+    n = 65536
+    gt, _ = E().embed_events_grad(x, at % n, n)                              # long rows in; events from the last to the first
+    exact, mag = torch.zeros(n, D, dtype=torch.float64, device="cuda"), torch.zeros(n, D, dtype=torch.float64, device="cuda")
+    for part in x.flip(0).split(n):
+        exact[:len(part)] += part.double()
+        mag[:len(part)] += part.double().abs()
+    R.check(gt, exact.cpu().numpy(), ((T // n + 4) * R.U * mag).cpu().numpy())
+    V = T // 2 + 1                                                           # a long gradient of the table
+    few = torch.tensor([V - 1, 0, V - 1], device="cuda")
+    gt, _ = E().embed_events_grad(x[:3], few, V)
+    assert torch.equal(gt[V - 1], x[0].float() + x[2].float()) and torch.equal(gt[0], x[1].float()) and not f64_any(gt[1:V - 1])
