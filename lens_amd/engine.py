@@ -494,7 +494,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # LENS_F32,
 def _call(name, dev, *args):
     """One entry point on the current stream of device `dev` (an index; it need not be the current device)."""
     fn = getattr(_lib.lib(), name)
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
