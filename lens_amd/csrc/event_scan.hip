@@ -650,6 +650,18 @@ __global__ void __launch_bounds__(256) k_scan_no_rows(const float *from, float *
     }
 }
 
+// f(true) where no decay of the wavefront's rows needs an exponential, else f(false).
+template <typename G, typename GATES, typename F>
+__device__ __forceinline__ void by_distance(const GATES &g, F f)
+{
+    if constexpr (__is_same(G, void)) {
+        if (__all(g.near)) f(std::true_type{});
+        else f(std::false_type{});
+    } else {
+        f(std::true_type{});
+    }
+}
+
 // H behind the rows of a batch, from H before them.
 template <int V, typename X, typename G>
 __device__ __forceinline__ void forward_batch(const ScanArgs &p, const Own<V> &o, const Rows &r, const int *ids, const Raw<V, X> &x,
@@ -662,12 +674,15 @@ __device__ __forceinline__ void forward_batch(const ScanArgs &p, const Own<V> &o
             pace();
         }
     } else {
+        by_distance<G>(g, [&](auto nearby) {
+            constexpr bool NEARBY = nearby;
 #pragma unroll
-        for (int j = 0; j < B; ++j) {
-            if (r.starts >> j & 1) H = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-            H = g.template step<false>(j, H, x[j]);
-            pace();
-        }
+            for (int j = 0; j < B; ++j) {
+                if (r.starts >> j & 1) H = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+                H = g.template step<NEARBY>(j, H, x[j]);
+                pace();
+            }
+        });
     }
 }
 
@@ -687,17 +702,20 @@ __device__ __forceinline__ void states_batch(const ScanArgs &p, const Tile &tile
             pace();
         }
     } else {
-        const int n = tile.left - t;
-        const unsigned in = n < B ? (1u << n) - 1 : (1u << B) - 1, written = p.fill ? in : r.lives;
+        by_distance<G>(g, [&](auto nearby) {
+            constexpr bool NEARBY = nearby;
+            const int n = tile.left - t;
+            const unsigned in = n < B ? (1u << n) - 1 : (1u << B) - 1, written = p.fill ? in : r.lives;
 #pragma unroll
-        for (int j = 0; j < B; ++j) {
-            if (j == 0 && mark) store<V>(mark, st);
-            if (r.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-            st = g.template step<false>(j, st, x[j]);
-            if (written >> j & 1) store_past<V>(behind(out, at + j * p.ldh), r.lives >> j & 1 ? st : vec<float, V>(0.0f));
-            if (r.ends >> j & 1) store<V>(p.last + (int64_t)ids[j] * p.D + o.c, st);
-            pace();
-        }
+            for (int j = 0; j < B; ++j) {
+                if (j == 0 && mark) store<V>(mark, st);
+                if (r.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+                st = g.template step<NEARBY>(j, st, x[j]);
+                if (written >> j & 1) store_past<V>(behind(out, at + j * p.ldh), r.lives >> j & 1 ? st : vec<float, V>(0.0f));
+                if (r.ends >> j & 1) store<V>(p.last + (int64_t)ids[j] * p.D + o.c, st);
+                pace();
+            }
+        });
     }
 }
 
@@ -1040,12 +1058,15 @@ __device__ __forceinline__ void backward_batch(const ScanArgs &p, const Own<V> &
             pace();
         }
     } else {
+        by_distance<G>(g, [&](auto nearby) {
+            constexpr bool NEARBY = nearby;
 #pragma unroll
-        for (int j = B - 1; j >= 0; --j) {
-            if (r.ends >> j & 1) U = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
-            U = g.template times<false>(j, U + d[j]);
-            pace();
-        }
+            for (int j = B - 1; j >= 0; --j) {
+                if (r.ends >> j & 1) U = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
+                U = g.template times<NEARBY>(j, U + d[j]);
+                pace();
+            }
+        });
     }
 }
 
@@ -1077,30 +1098,33 @@ __device__ __forceinline__ void rows_batch(const ScanArgs &p, const Tile &tile, 
             pace();
         }
     } else {
-        const int n = tile.left - t;
+        by_distance<G>(g, [&](auto nearby) {
+            constexpr bool NEARBY = nearby;
+            const int n = tile.left - t;
 #pragma unroll
-        for (int j = 0; j < B; ++j) {
-            if (q.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
-            before[j] = st;
-            st = g.template step<false>(j, st, x[j]);
-            pace();
-        }
-        g.again();
-#pragma unroll
-        for (int j = B - 1; j >= 0; --j) {
-            const bool live = q.lives >> j & 1;
-            if (q.ends >> j & 1) r = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
-            const vec<float, V> gt = r + d[j];
-            r = g.template times<false>(j, gt);
-            if (live && (q.starts >> j & 1) && p.grad_h0) store<V>(p.grad_h0 + (int64_t)ids[j] * p.D + o.c, r);
-            if (j < n) store_past<V>(behind(gx, at_x + j * p.ld_gx), live ? gt : zero);
-            if constexpr (__is_same(G, void)) {
-                if (live) share = fma<V>(r * -g.dt[j], before[j], share);
-            } else {
-                if (j < n) store_past<V>(behind(gg, at_g + j * p.ld_gg), live ? gt * before[j] : zero);
+            for (int j = 0; j < B; ++j) {
+                if (q.starts >> j & 1) st = row_or_zero<V>(p.h0, ids[j], p.D, o.c);
+                before[j] = st;
+                st = g.template step<NEARBY>(j, st, x[j]);
+                pace();
             }
-            pace();
-        }
+            g.again();
+#pragma unroll
+            for (int j = B - 1; j >= 0; --j) {
+                const bool live = q.lives >> j & 1;
+                if (q.ends >> j & 1) r = row_or_zero<V>(p.grad_last, ids[j], p.D, o.c);
+                const vec<float, V> gt = r + d[j];
+                r = g.template times<NEARBY>(j, gt);
+                if (live && (q.starts >> j & 1) && p.grad_h0) store<V>(p.grad_h0 + (int64_t)ids[j] * p.D + o.c, r);
+                if (j < n) store_past<V>(behind(gx, at_x + j * p.ld_gx), live ? gt : zero);
+                if constexpr (__is_same(G, void)) {
+                    if (live) share = fma<V>(r * -g.dt[j], before[j], share);
+                } else {
+                    if (j < n) store_past<V>(behind(gg, at_g + j * p.ld_gg), live ? gt * before[j] : zero);
+                }
+                pace();
+            }
+        });
     }
 }
 
