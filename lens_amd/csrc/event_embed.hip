@@ -447,8 +447,8 @@ __global__ void __launch_bounds__(FEW_THREADS) k_sort_few(const SortArgs p, uint
 // list: token t stands at place t + key[t], the end of row r behind the last token of r.  A workgroup takes `items` places
 // a group, a group is `G` lanes that hold one row of the table's width, NV vectors each.
 // A row that begins in one group and ends in a later one is joined in LDS, over workgroups by k_grad_join.
-// Bytes bound a large one: 2000000 x 256 bf16 to 179920 rows 260 us, 4.7 TB/s, and 16 us to join; latency a small one: 30011 x 63
-// f32 to 32768 rows, weights too, 14 and 5 us.
+// Bytes bound a large one: 2000000 x 256 bf16 to 179920 rows 260 us, 4.7 TB/s, and 9 us to join; latency a small one: 30011 x 63
+// f32 to 32768 rows, weights too, 14 and 6 us.
 // ------------------------------------------------------------------------------------------
 constexpr int GRAD_ITEMS = 64, GRAD_U = 4;
 
@@ -462,7 +462,7 @@ struct GradArgs {
     int32_t *open;                   // [workgroups] the row behind the last begins here, or there is none
     int64_t T, V_rows, ld_grad, ld_table;
     float scale;
-    int D, items;
+    int D, items, blocks;            // blocks: workgroups of k_grad
 };
 
 // A sorted token and its event, kept inside the table and the list whatever order the caller passed.
@@ -666,50 +666,67 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     }
 }
 
-// Rows that begin in one workgroup of k_grad and end in a later one: a workgroup here for each of its, the tails shared out
-// over its groups in runs.
+// Rows that begin in one workgroup of k_grad and end in a later one: a group here for each of its.  Where that is the workgroup
+// behind, the group adds the two shares; else all groups share out the tails between, in runs.
 template <int V, int NV, int G>
 __global__ void __launch_bounds__(256) k_grad_join(const GradArgs p)
 {
     constexpr int NG = 256 / G;
     __shared__ vec<float, V> part[NV][256];
     __shared__ int nearest;
-    const int lane = (int)threadIdx.x % G, group = (int)threadIdx.x / G, block = blockIdx.x;
-    const int64_t r = p.first_row[block];
-    if (r < 0) return;
-    int b0 = -1;                                                      // where the row begins: the nearest earlier one that is open
-    for (int top = block - 1; top >= 0 && b0 < 0; top -= 256) {
-        if (threadIdx.x == 0) nearest = -1;
-        __syncthreads();
-        const int q = top - (int)threadIdx.x;
-        if (q >= 0 && p.open[q]) atomicMax(&nearest, q);
-        __syncthreads();
-        b0 = nearest;
-        __syncthreads();
-    }
-    if (b0 < 0) b0 = 0;
-    const int n = block - b0, each = (n + NG - 1) / NG;
-    const int q0 = b0 + group * each < block ? b0 + group * each : block, q1 = q0 + each < block ? q0 + each : block;
-    vec<float, V> sum[NV];
+    __shared__ int64_t rest[NG];                                      // rows that begin further in front, -1: none
+    const int lane = (int)threadIdx.x % G, group = (int)threadIdx.x / G;
     int c[NV], skip[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        c[k] = channel<V, G>(k, lane, p.D, skip[k]);
-        sum[k] = vec<float, V>(0.0f);
+    for (int k = 0; k < NV; ++k) c[k] = channel<V, G>(k, lane, p.D, skip[k]);
+    {
+        const int block = blockIdx.x * NG + group, at = block < p.blocks ? block : p.blocks - 1;
+        const int64_t r = p.first_row[at];
+        const bool begins = p.open[at > 0 ? at - 1 : 0], ends = block < p.blocks && r >= 0, next = ends && at > 0 && begins;
+        if (lane == 0) rest[group] = ends && !next ? r : -1;
+        if (next)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const vec<float, V> v = load<V>(p.tail + (int64_t)(block - 1) * p.D + c[k]) + load<V>(p.head + (int64_t)block * p.D + c[k]);
+                if (skip[k] < V) store<V>(p.out + r * p.D + c[k], v);
+            }
     }
-#pragma unroll 4
-    for (int64_t q = q0; q < q1; ++q)
-#pragma unroll
-        for (int k = 0; k < NV; ++k) sum[k] += load<V>(p.tail + q * p.D + c[k]);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) part[k][threadIdx.x] = sum[k];
     __syncthreads();
-    if (group != 0) return;
+    for (int g = 0; g < NG; ++g) {
+        const int64_t r = rest[g];
+        if (r < 0) continue;
+        const int block = blockIdx.x * NG + g;
+        int b0 = -1;                                                  // where the row begins: the nearest earlier one that is open
+        for (int top = block - 1; top >= 0 && b0 < 0; top -= 256) {
+            if (threadIdx.x == 0) nearest = -1;
+            __syncthreads();
+            const int q = top - (int)threadIdx.x;
+            if (q >= 0 && p.open[q]) atomicMax(&nearest, q);
+            __syncthreads();
+            b0 = nearest;
+            __syncthreads();
+        }
+        if (b0 < 0) b0 = 0;
+        const int n = block - b0, each = (n + NG - 1) / NG;
+        const int q0 = b0 + group * each < block ? b0 + group * each : block, q1 = q0 + each < block ? q0 + each : block;
+        vec<float, V> sum[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        for (int q = 1; q < NG; ++q) sum[k] += part[k][q * G + lane];
-        sum[k] += load<V>(p.head + (int64_t)block * p.D + c[k]);
-        if (skip[k] < V) store<V>(p.out + r * p.D + c[k], sum[k]);
+        for (int k = 0; k < NV; ++k) sum[k] = vec<float, V>(0.0f);
+#pragma unroll 4
+        for (int64_t q = q0; q < q1; ++q)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) sum[k] += load<V>(p.tail + q * p.D + c[k]);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) part[k][threadIdx.x] = sum[k];
+        __syncthreads();
+        if (group == 0)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                for (int q = 1; q < NG; ++q) sum[k] += part[k][q * G + lane];
+                sum[k] += load<V>(p.head + (int64_t)block * p.D + c[k]);
+                if (skip[k] < V) store<V>(p.out + r * p.D + c[k], sum[k]);
+            }
+        __syncthreads();
     }
 }
 
@@ -783,7 +800,7 @@ int launch_grad(const GradArgs &p, hipStream_t st)
     const dim3 grid((unsigned)grad_blocks(p.T, p.V_rows, G)), block(256);
     if (p.grad_weight) hipLaunchKernelGGL((k_grad<V, NV, G, X, true>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((k_grad<V, NV, G, X, false>), grid, block, 0, st, p);
-    hipLaunchKernelGGL((k_grad_join<V, NV, G>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((k_grad_join<V, NV, G>), dim3((p.blocks + 256 / G - 1) / (256 / G)), block, 0, st, p);
     return (int)hipGetLastError();
 }
 
@@ -923,6 +940,7 @@ int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const 
     p.grad_weight = d_grad_weight; p.head = (float *)base; p.tail = (float *)(base + up(blocks * D * 4));
     p.first_row = (int64_t *)(base + 2 * up(blocks * D * 4)); p.open = (int32_t *)(base + 2 * up(blocks * D * 4) + up(blocks * 8));
     p.items = grad_items(T, n_rows, w.G);
+    p.blocks = (int)blocks;
     p.T = T; p.V_rows = n_rows; p.ld_grad = ld_grad; p.ld_table = ld_table; p.scale = scale; p.D = D;
     hipStream_t st = (hipStream_t)stream;
     if (type == LENS_F32) return w.V == 4 ? grad_by_width<4, float>(w, p, st) : grad_by_width<1, float>(w, p, st);
