@@ -666,8 +666,10 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     }
 }
 
-// Rows that begin in one workgroup of k_grad and end in a later one: a group here for each of its.  Where that is the workgroup
-// behind, the group adds the two shares; else all groups share out the tails between, in runs.
+// Rows that begin in one workgroup of k_grad and end in a later one: a group here for each of its.  Where they begin at most
+// JOIN_NEAR workgroups in front the group adds the shares; else all groups share out the tails between, in runs.
+constexpr int JOIN_NEAR = 4;
+
 template <int V, int NV, int G>
 __global__ void __launch_bounds__(256) k_grad_join(const GradArgs p)
 {
@@ -682,13 +684,23 @@ __global__ void __launch_bounds__(256) k_grad_join(const GradArgs p)
     {
         const int block = blockIdx.x * NG + group, at = block < p.blocks ? block : p.blocks - 1;
         const int64_t r = p.first_row[at];
-        const bool begins = p.open[at > 0 ? at - 1 : 0], ends = block < p.blocks && r >= 0, next = ends && at > 0 && begins;
-        if (lane == 0) rest[group] = ends && !next ? r : -1;
-        if (next)
+        int far = 0;                                                  // how many workgroups in front the row begins, 0: more
+        bool begins[JOIN_NEAR];
+#pragma unroll
+        for (int d = 0; d < JOIN_NEAR; ++d) begins[d] = p.open[at > d ? at - d - 1 : 0] && at > d;
+#pragma unroll
+        for (int d = JOIN_NEAR; d > 0; --d) far = begins[d - 1] ? d : far;
+        const bool ends = block < p.blocks && r >= 0;
+        if (lane == 0) rest[group] = ends && far == 0 ? r : -1;
+        if (ends && far > 0)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const vec<float, V> v = load<V>(p.tail + (int64_t)(block - 1) * p.D + c[k]) + load<V>(p.head + (int64_t)block * p.D + c[k]);
-                if (skip[k] < V) store<V>(p.out + r * p.D + c[k], v);
+                vec<float, V> v = load<V>(p.head + (int64_t)block * p.D + c[k]), sum(0.0f);
+#pragma unroll
+                for (int d = JOIN_NEAR; d > 0; --d)
+                    if (d <= far) sum += load<V>(p.tail + (int64_t)(block - d) * p.D + c[k]);
+                sum += v;
+                if (skip[k] < V) store<V>(p.out + r * p.D + c[k], sum);
             }
     }
     __syncthreads();
