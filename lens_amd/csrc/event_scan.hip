@@ -788,34 +788,34 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
 // ------------------------------------------------------------------------------------------ one pass
 // The rows stay in registers until what is before them is known.  What enters a tile: the tiles of a launch are numbered by a
 // ticket that every workgroup draws when it starts; a workgroup waits only for what workgroups with smaller tickets publish,
-// which run already and publish before they wait for anything larger, so every wait ends.  8 or 16 tiles are a group, as many
+// which run already and publish before they wait for anything larger, so every wait ends.  8 tiles are a group, 8
 // groups a group of the next level, and the last tile of a group publishes the group's pair from those below.  What enters tile
-// i are the pairs before it in its group, before that group in its own, and so on: 3.5 or 7.5 pairs a level, read at once
-// by a wavefront a level, always joined in the same order.  A word is the pair of one channel: 8 bytes, stored and read
-// whole, all ones until it is there (a lane a channel: 8 words in flight and few registers).
+// i are the pairs before it in its group, before that group in its own, and so on: 3.5 pairs a level, read by
+// a wavefront a level, always joined in the same order.  A word is the pair of one channel: 8 bytes, stored and read
+// whole, all ones until it is there (a lane a channel: 4 words in flight and few registers, while the rows wait in theirs;
+// 8 in flight spill, 262144 x 128 f32 with decays 82 us instead of 75).
 // Scratch memory that another call uses at the same time could keep a wait from ending: it is given up after about a second,
 // all others of the launch then at once, and the results are NaN.
 //
 // One pass against reading twice, us a call (backward: scan and gradients):
-//   gates                 1048573 x 128 bf16, bf16 gates 189 / 253     30000 x 128 f32, f32 gates 18 / 23
+//   gates                 1048573 x 128 bf16, bf16 gates 184 / 253     30000 x 128 f32, f32 gates 18 / 23
 //   gates, backward        524287 x 256 bf16, bf16 gates 317 / 357 (the backward launches)
-//   f32 rows, decays       262144 x 128  72 / 78     1501 x 200  17 / 19     backward  114 / 113  and  23 / 23 (the backward launches)
-//   16-bit rows, decays   of 128 channels, 4 sequences:  16384  20 / 21    32768  22 / 24    65536  26 / 31    131072  35 / 37
-//                         262144  61 / 56    524288  102 / 87     400009 x 200, 37 sequences  135 / 117
-//            backward     16384  46 / 47    32768  50 / 52    65536  60 / 71    131072  89 / 89    262144  160 / 144    524288  281 / 236
-//                         400009 x 200  364 / 296
+//   f32 rows, decays      262144 x 128  75 / 77    1501 x 200  16 / 18       with gradients  186 / 197  and  40 / 47
+//   16-bit rows, decays   of 128 channels, 4 sequences:  16384  19 / 19    32768  21 / 22    65536  25 / 31    131072  35 / 34
+//                         262144  59 / 56    524288  101 / 87     400009 x 200, 37 sequences  134 / 115
+//       with gradients    16384  42 / 46    32768  48 / 48    65536  59 / 68    131072  86 / 85    262144  155 / 141    524288  277 / 233
+//                         400009 x 200  355 / 292
 // So 16-bit rows with decays -- the fewest bytes for the arithmetic of a row -- are read twice from 16 M elements on, by
 // workgroups that wait for nothing; all others go in one pass.
 //
-// What it reaches: 1048573 x 128 bf16 with gates 186 us, 4.3 TB/s of the 805 MB that have to move (torch's copy of 1 GB:
-// 5.0); 262144 x 128 f32 with decays 72 us, 3.7 TB/s: two rounds of workgroups, each of which loads, waits and stores in step.
+// What it reaches: 1048573 x 128 bf16 with gates 184 us, 4.4 TB/s of the 805 MB that have to move (torch's copy of 1 GB:
+// 5.0); 262144 x 128 f32 with decays 75 us, 3.6 TB/s: two rounds of workgroups, each of which loads, waits and stores in step.
 // Outputs past the caches: 185 / 192 us with / without, forward and backward of 262144 x 128 f32 197 / 216.
 constexpr uint64_t EMPTY = ~0ull;
 constexpr int MOST_TRIES = 1 << 20;
 
-// 16 tiles a group, for decays, whose pairs take more work to join, 8.
-template <typename G> constexpr int group_bits = 4;
-template <> constexpr int group_bits<void> = 3;
+constexpr int GROUP_BITS = 3, GROUP = 1 << GROUP_BITS;       // 8 tiles a group
+constexpr int WORDS = 4;                                     // asked for at once
 
 template <int V>
 struct LdsOnce {
@@ -838,7 +838,6 @@ struct LdsOnce {
 
 template <int V, typename G>
 struct Chain {
-    static constexpr int GROUP_BITS = group_bits<G>, GROUP = 1 << GROUP_BITS;
     uint64_t *words;
     unsigned *ticket;                  // and behind it: a wait was given up
     int tile, tiles, levels, ts, D, c0, slots, cg_left;      // c0, cg_left: of the workgroup's part of the channels
@@ -880,13 +879,13 @@ struct Chain {
         Pair<G> w = Pair<G>::none();
         if (c < 0 || n == 0) return w;
 #pragma unroll 1
-        for (int k0 = 0; k0 < n; k0 += 8) {
-            uint64_t v[8];
+        for (int k0 = 0; k0 < n; k0 += WORDS) {
+            uint64_t v[WORDS];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int k = 0; k < WORDS; ++k)
                 if (k0 + k < n) v[k] = __hip_atomic_load(behind(from, (k0 + k) * D + c), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)                   // only what is not there yet is asked for again, one word at a time
+            for (int k = 0; k < WORDS; ++k)                   // only what is not there yet is asked for again, one word at a time
                 if (k0 + k < n) {
                     for (int tries = 1; v[k] == EMPTY; ++tries) {
                         if (tries % 256 == 0 && give_up(tries)) {
@@ -1396,10 +1395,10 @@ int run_of(int64_t T, const Shape &s)
 }
 
 // Words of one pass: those of `tiles` tiles and of all complete groups above them; levels: how many that are.
-int64_t words_of(int64_t tiles, int D, int bits, int &levels)
+int64_t words_of(int64_t tiles, int D, int &levels)
 {
     int64_t words = 0;
-    for (levels = 0; (tiles - 1) >> (bits * levels) > 0; ++levels) words += (tiles >> (bits * levels)) * D;
+    for (levels = 0; (tiles - 1) >> (GROUP_BITS * levels) > 0; ++levels) words += (tiles >> (GROUP_BITS * levels)) * D;
     return words;
 }
 
@@ -1423,7 +1422,7 @@ Scratch scratch_of(int64_t T, int D, bool back)
     r.ticket = 0;
     r.words = 256;
     const size_t end_two = r.pre + whole((size_t)tiles * two.ts * 2 * D * 4);
-    const size_t end_one = r.words + whole((size_t)words_of(tiles_one, D, group_bits<void>, levels) * 8);
+    const size_t end_one = r.words + whole((size_t)words_of(tiles_one, D, levels) * 8);
     r.part = end_two > end_one ? end_two : end_one;
     r.bytes = r.part + (back ? whole((size_t)(tiles > tiles_one ? tiles : tiles_one) * D * 4) : 0);
     return r;
@@ -1461,7 +1460,6 @@ dim3 put_twice(ScanArgs &p, unsigned char *scratch, bool back)
     return dim3((int64_t)p.tiles * 256 > MAX_THREADS ? 0 : p.tiles, s.ny);
 }
 
-template <typename G>
 unsigned put_once(ScanArgs &p, unsigned char *scratch, bool back, int batches)
 {
     const Shape s = shape_of(p.D, ONCE);
@@ -1470,16 +1468,15 @@ unsigned put_once(ScanArgs &p, unsigned char *scratch, bool back, int batches)
     p.ticket = (unsigned *)(scratch + r.ticket);
     p.words = (uint64_t *)(scratch + r.words);
     p.part = (float *)(scratch + r.part);
-    words_of(p.tiles, p.D, group_bits<G>, p.levels);
+    words_of(p.tiles, p.D, p.levels);
     const int64_t n = (int64_t)p.tiles * s.ny;
     return n * ONCE > MAX_THREADS ? 0 : (unsigned)n;
 }
 
-template <typename G>
 void launch_clear(const ScanArgs &p, hipStream_t st)
 {
     int levels;
-    const int64_t n = (words_of(p.tiles, p.D, group_bits<G>, levels) + 1) / 2, blocks = (n + 1023) / 1024;
+    const int64_t n = (words_of(p.tiles, p.D, levels) + 1) / 2, blocks = (n + 1023) / 1024;
     if (p.tiles > 1)
         hipLaunchKernelGGL(k_scan_clear, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (uint4 *)p.words, n, p.ticket);
 }
@@ -1519,9 +1516,9 @@ int launch_no_rows(const float *from, float *to, int64_t n, float *rate, int D, 
 template <int V, int NB, typename X, typename G>
 int launch_once(ScanArgs &p, unsigned char *scratch, hipStream_t st)
 {
-    const unsigned grid = put_once<G>(p, scratch, false, NB);
+    const unsigned grid = put_once(p, scratch, false, NB);
     if (!grid) return LENS_ERR_SIZE;
-    launch_clear<G>(p, st);
+    launch_clear(p, st);
     launch_pass_on(p, p.h0, p.last, (int64_t)grid * p.lanes * p.ts, st);
     hipLaunchKernelGGL((k_scan_once<V, NB, X, G>), dim3(grid), dim3(p.lanes * p.ts), LdsOnce<V>::bytes(p.ts, p.lanes, p.levels, p.run), st, p);
     return (int)hipGetLastError();
@@ -1549,9 +1546,9 @@ int launch_forward(ScanArgs &p, unsigned char *scratch, hipStream_t st)
 template <int V, int NB, typename X, typename G>
 int launch_back_once(ScanArgs &p, unsigned char *scratch, hipStream_t st)
 {
-    const unsigned grid = put_once<G>(p, scratch, true, NB);
+    const unsigned grid = put_once(p, scratch, true, NB);
     if (!grid) return LENS_ERR_SIZE;
-    launch_clear<G>(p, st);
+    launch_clear(p, st);
     launch_pass_on(p, p.grad_last, p.grad_h0, (int64_t)grid * p.lanes * p.ts, st);
     hipLaunchKernelGGL((k_scan_back_once<V, NB, X, G>), dim3(grid), dim3(p.lanes * p.ts), LdsOnce<V>::bytes(p.ts, p.lanes, p.levels, p.run), st, p);
     return (int)hipGetLastError();
