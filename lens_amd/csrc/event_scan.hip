@@ -719,7 +719,7 @@ __device__ __forceinline__ void states_batch(const ScanArgs &p, const Tile &tile
     }
 }
 
-// 400009 x 200 bf16 with decays: pairs 39 us, 4.1 TB/s of the rows; states 75 us, 4.3 TB/s of the rows in and out.
+// 400009 x 200 bf16 with decays: pairs 38 us, 4.2 TB/s of the rows; states 73 us, 4.4 TB/s of the rows in and out.
 template <int V, typename X, typename G>
 __global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
 {
@@ -810,7 +810,7 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
 //
 // What it reaches: 1048573 x 128 bf16 with gates 184 us, 4.4 TB/s of the 805 MB that have to move (torch's copy of 1 GB:
 // 5.0); 262144 x 128 f32 with decays 75 us, 3.6 TB/s: two rounds of workgroups, each of which loads, waits and stores in step.
-// Outputs past the caches: 185 / 192 us with / without, forward and backward of 262144 x 128 f32 197 / 216.
+// Outputs past the caches: 184 / 192 us with / without, forward and backward of 262144 x 128 f32 186 / 216.
 constexpr uint64_t EMPTY = ~0ull;
 constexpr int MOST_TRIES = 1 << 20;
 
@@ -1042,7 +1042,7 @@ __global__ void __launch_bounds__(ONCE, 4) k_scan_once(const ScanArgs p)
 // ------------------------------------------------------------------------------------------
 // Backward.  With r_t = a_t g_t the message that row t sends back: g_t = dh_t + r_{t+1}, so a run of rows acts on the
 // message that enters from behind as r -> f r + U with the f of the forward direction.  The states before the rows are
-// computed again from the marks, B rows at a time.  Bytes bound it: 524287 x 256 bf16 with gates 315 us, 4.5 TB/s of the 1.4 GB of
+// computed again from the marks, B rows at a time.  Bytes bound it: 524287 x 256 bf16 with gates 320 us, 4.4 TB/s of the 1.4 GB of
 // x, gates, gradient and marks in and both gradients out; 262144 x 128 f32 with decays 108 us, 3.9 TB/s of 420 MB.
 // ------------------------------------------------------------------------------------------
 // The message before the rows of a batch, from U behind them.
@@ -1483,7 +1483,7 @@ void launch_clear(const ScanArgs &p, hipStream_t st)
 
 // Batches of a thread in one pass: two where their rows fit its registers, but one where two would leave a CU without a tile.
 // One / two, us:  1501 x 200 f32 decays 17.5 / 23.1, 30000 x 128 bf16 gates 17.0 / 17.6;  1048573 x 128 bf16 gates 243 / 184, with
-// gradients 262144 x 128 f32 decays 239 / 199, 524287 x 256 bf16 gates 640 / 507.
+// gradients 262144 x 128 f32 decays 239 / 186, 524287 x 256 bf16 gates 640 / 512.
 int batches_of(const ScanArgs &p)
 {
     const Shape s = shape_of(p.D, ONCE);
