@@ -317,7 +317,8 @@ struct Rows {
     bool plain;
 };
 
-// `w` is the place of row t, and moves on to row t + B.
+// `w` is the place of row t, and moves on to row t + B.  ids: of these rows alone -- a run's lanes may lie in two wavefronts, and the
+// faster one is batches ahead.  Only rows of a sequence have one.
 __device__ __forceinline__ Rows rows_of(const ScanArgs &p, const Tile &tile, Place &w, int t, int *ids)
 {
     const int left = tile.left - t, n = left < B ? left : B;
@@ -334,8 +335,8 @@ __device__ __forceinline__ Rows rows_of(const ScanArgs &p, const Tile &tile, Pla
             r.lives |= 1u << j;
             r.starts |= (start ? 1u : 0u) << j;
             r.ends |= (t + j + 1 == w.next ? 1u : 0u) << j;
+            ids[j] = w.k - 1;                                  // the same from every lane of the rows
         }
-        ids[j] = w.k - 1;                                      // the same from every lane of the rows
         start = false;
     }
     w.start = false;
@@ -496,7 +497,7 @@ struct Gates<V, void> {
 template <int V>
 struct Lds {
     float *f, *h;                      // [ts][slots] pairs of the runs
-    int *ids;                          // [ts][B] sequences of the rows of a batch
+    int *ids;                          // [ts][run] sequences of the rows
     int slots;
     __device__ __forceinline__ Lds(const ScanArgs &p)
     {
@@ -506,7 +507,7 @@ struct Lds {
         h = f + p.ts * slots;
         ids = reinterpret_cast<int *>(h + p.ts * slots);
     }
-    static size_t bytes(int ts, int lanes) { return ((size_t)2 * ts * lanes * V + ts * B) * 4; }
+    static size_t bytes(int ts, int lanes, int run) { return ((size_t)2 * ts * lanes * V + ts * run) * 4; }
 };
 
 // The channel of a slot, -1: none.
@@ -727,7 +728,7 @@ __global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
     const int index = blockIdx.x, y = blockIdx.y;
     Tile tile(p, index);
     const Own<V> o(p, tile, y);
-    int *ids = lds.ids + o.ts * B;
+    int *ids = lds.ids + o.ts * p.run;
     Gates<V, G> g(p, o.c);
     Raw<V, X> x;
     vec<float, V> H(0.0f);
@@ -743,9 +744,9 @@ __global__ void __launch_bounds__(256) k_scan_pairs(const ScanArgs p)
 #pragma unroll 1
         for (int b = 0; b < o.n; b += B) {
             if (b) load_batch(b);
-            const Rows r = rows_of(p, tile, w, o.t0 + b, ids);
+            const Rows r = rows_of(p, tile, w, o.t0 + b, ids + b);
             mark |= r.starts != 0;
-            forward_batch<V, X, G>(p, o, r, ids, x, g, H);
+            forward_batch<V, X, G>(p, o, r, ids + b, x, g, H);
             g.again();
             g.add_rows();
         }
@@ -763,7 +764,7 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
     if (y == 0) pass_on(p, p.h0, p.last, index, p.tiles);
     Tile tile(p, index);
     const Own<V> o(p, tile, y);
-    int *ids = lds.ids + o.ts * B;
+    int *ids = lds.ids + o.ts * p.run;
     Gates<V, G> g(p, o.c);
     Raw<V, X> x;
     auto load_batch = [&](int b) {
@@ -780,8 +781,8 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
     for (int b = 0; b < o.n; b += B) {
         const int t = o.t0 + b;
         if (b) load_batch(b);
-        const Rows r = rows_of(p, tile, w, t, ids);
-        states_batch<V, X, G>(p, tile, o, r, ids, t, x, g, out, st);
+        const Rows r = rows_of(p, tile, w, t, ids + b);
+        states_batch<V, X, G>(p, tile, o, r, ids + b, t, x, g, out, st);
     }
 }
 
@@ -1134,7 +1135,7 @@ __global__ void __launch_bounds__(256) k_scan_back_pairs(const ScanArgs p)
     const int index = blockIdx.x, y = blockIdx.y;
     Tile tile(p, index);
     const Own<V> o(p, tile, y);
-    int *ids = lds.ids + o.ts * B;
+    int *ids = lds.ids + o.ts * p.run;
     Gates<V, G> g(p, o.c);
     Raw<V, X> d;
     vec<float, V> U(0.0f);
@@ -1151,9 +1152,9 @@ __global__ void __launch_bounds__(256) k_scan_back_pairs(const ScanArgs p)
     for (int b = last; b >= 0; b -= B) {
         if (b != last) load_batch(b);
         Place w = locate(p, tile, o.t0 + b);
-        const Rows r = rows_of(p, tile, w, o.t0 + b, ids);
+        const Rows r = rows_of(p, tile, w, o.t0 + b, ids + b);
         mark |= r.ends != 0;
-        backward_batch<V, X, G>(p, o, r, ids, d, g, U);
+        backward_batch<V, X, G>(p, o, r, ids + b, d, g, U);
         g.again();
         g.add_rows();
     }
@@ -1170,7 +1171,7 @@ __global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
     if (y == 0) pass_on(p, p.grad_last, p.grad_h0, index, p.tiles);
     Tile tile(p, index);
     const Own<V> o(p, tile, y);
-    int *ids = lds.ids + o.ts * B;
+    int *ids = lds.ids + o.ts * p.run;
     tile.find(p);
     vec<float, V> r = run_entry<V, G>(p, o, index, p.tiles - 1 - index), share(0.0f);
     Gates<V, G> g(p, o.c);
@@ -1186,8 +1187,8 @@ __global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
         else d.zero();
         vec<float, V> st = load<V>(p.marks_in + (tile.row0 + t) / B * p.D + o.c);
         Place w = locate(p, tile, t);
-        const Rows q = rows_of(p, tile, w, t, ids);
-        rows_batch<V, X, G>(p, tile, o, q, ids, t, x, d, g, gx, gg, st, r, share);
+        const Rows q = rows_of(p, tile, w, t, ids + b);
+        rows_batch<V, X, G>(p, tile, o, q, ids + b, t, x, d, g, gx, gg, st, r, share);
     }
     if constexpr (__is_same(G, void)) {
         __syncthreads();
@@ -1531,7 +1532,7 @@ int launch_forward(ScanArgs &p, unsigned char *scratch, hipStream_t st)
         if (read_twice(p.T, p.D)) {
             const dim3 grid = put_twice(p, scratch, false), block(p.lanes * p.ts);
             if (!grid.x) return LENS_ERR_SIZE;
-            const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
+            const size_t lds = Lds<V>::bytes(p.ts, p.lanes, p.run);
             launch_pass_on(p, p.h0, p.last, (int64_t)p.tiles * block.x, st);
             hipLaunchKernelGGL((k_scan_pairs<V, X, G>), grid, block, lds, st, p);
             launch_join<G>(p, st);
@@ -1563,7 +1564,7 @@ int launch_backward(ScanArgs &p, unsigned char *scratch, hipStream_t st)
         if (read_twice(p.T, p.D)) {
             const dim3 grid = put_twice(p, scratch, true), block(p.lanes * p.ts);
             if (!grid.x) return LENS_ERR_SIZE;
-            const size_t lds = Lds<V>::bytes(p.ts, p.lanes);
+            const size_t lds = Lds<V>::bytes(p.ts, p.lanes, p.run);
             launch_pass_on(p, p.grad_last, p.grad_h0, (int64_t)p.tiles * block.x, st);
             hipLaunchKernelGGL((k_scan_back_pairs<V, X, G>), grid, block, lds, st, p);
             launch_join<G>(p, st);

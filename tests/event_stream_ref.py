@@ -140,3 +140,118 @@ def check(got, want, bound, name=""):
         off = np.abs(got - want) - room
     bad = ~(off <= 0)
     assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.size} off, first at {np.argwhere(bad)[0].tolist()}: got {got[bad][0]!r}, want {want[bad][0]!r}, room {np.broadcast_to(room, bad.shape)[bad][0]!r}"
+
+
+# ---- the same for many rows in short sequences: torch in 64 bits on x's device, all sequences side by side, one row of each at a time
+def _walk_rows(off, backward=False):
+    """(sequences, their rows) of every step."""
+    start, n = off[:-1], off[1:] - off[:-1]
+    for j in range(int(n.max())):
+        s = (n > j).nonzero()[:, 0]
+        yield s, (start[s] + j if not backward else off[1:][s] - 1 - j)
+
+
+def _gate_rows(gate, dt, rate, t):
+    """a of the rows t, and (8 + 20 |z|) u of them as step_loss has it."""
+    a = gate[t].double() if gate is not None else torch.exp(-dt[t].double()[:, None] * rate.double())
+    z = torch.where(a > 0, a.clamp(min=1e-300).log().abs().clamp(max=700), 0.0)
+    return a, (8 + 20 * z) * U
+
+
+def scan_side_by_side(x, off, h0, gate=None, dt=None, rate=None):
+    """What scan returns, off an int64 tensor."""
+    T, D = x.shape
+    h, before, E, Eb = (torch.zeros(T, D, dtype=torch.float64, device=x.device) for _ in range(4))
+    v = h0.double().clone()
+    m, e = v.abs(), torch.zeros_like(v)
+    for s, t in _walk_rows(off):
+        a, c = _gate_rows(gate, dt, rate, t)
+        before[t], Eb[t] = v[s], e[s]
+        v[s] = a * v[s] + x[t].double()
+        e[s] = a.abs() * e[s] + 4 * TINY + FLUSHED * m[s]
+        m[s] = a.abs() * m[s] + x[t].double().abs()
+        e[s] += c * m[s]
+        h[t], E[t] = v[s], e[s]
+    return h, v, before, E, e, Eb
+
+
+def scan_grad_side_by_side(grad_h, grad_last, x, before, Eb, off, gate=None, dt=None, rate=None, sum_terms=None):
+    """What scan_grad returns; before, Eb: of scan_side_by_side.  sum_terms: roundings of a sum over all rows (T + 4)."""
+    T, D = x.shape
+    g, Eg = (torch.zeros(T, D, dtype=torch.float64, device=x.device) for _ in range(2))
+    ga, Ea = (torch.zeros_like(g), torch.zeros_like(g)) if gate is not None else (None, None)
+    r = grad_last.double().clone()
+    m, e = r.abs(), torch.zeros_like(r)
+    total, bound, mag = (torch.zeros(D, dtype=torch.float64, device=x.device) for _ in range(3))
+    for s, t in _walk_rows(off, True):
+        a, c = _gate_rows(gate, dt, rate, t)
+        d = grad_h[t].double()
+        gt = d + r[s]
+        mm = m[s] + d.abs()
+        eg = e[s] + 2 * U * mm
+        g[t], Eg[t] = gt, eg
+        if gate is not None:
+            ga[t] = gt * before[t]
+            Ea[t] = eg * before[t].abs() + Eb[t] * gt.abs() + eg * Eb[t] + U * (gt * before[t]).abs()
+        rr = a * gt
+        ee = a.abs() * eg + 4 * TINY + FLUSHED * mm
+        mm = a.abs() * mm
+        ee = ee + c * mm
+        r[s], m[s], e[s] = rr, mm, ee
+        if gate is None:
+            w = dt[t].double()[:, None]
+            total -= (w * rr * before[t]).sum(0)
+            mag += (w * rr * before[t]).abs().sum(0)
+            bound += (w.abs() * (ee * before[t].abs() + Eb[t] * rr.abs() + ee * Eb[t])).sum(0)
+    if gate is not None:
+        return g, ga, r, Eg, Ea, e
+    return g, total, r, Eg, bound + (T + 4 if sum_terms is None else sum_terms) * U * mag, e
+
+
+def check_all(got, want, bound, name=""):
+    """check, on the tensors' device."""
+    room = bound + half_step(got.dtype) * (want.abs() + bound) + least(got.dtype)
+    bad = ~((got.double() - want).abs() <= room)
+    if bool(bad.any()):
+        at = tuple(bad.nonzero()[0].tolist())
+        raise AssertionError(f"{name}: {int(bad.sum())} of {bad.numel()} off, first at {at}: got {float(got[at])!r}, want {float(want[at])!r}, "
+                             f"room {float(room[at])!r}")
+
+
+# Scans that are read twice, (D, T, dtype): by the rule of event_scan.hip (plan_twice below) a thread walks `run` rows in several batches of 8,
+# and the lanes of one run lie in two wavefronts.
+MANY_BATCHES = [(200, 81957, torch.bfloat16, 16), (100, 163845, torch.float16, 16), (300, 49163, torch.bfloat16, 16), (3, 524297, torch.float16, 16),
+                (200, 327683, torch.bfloat16, 64), (3, 4194319, torch.bfloat16, 128)]
+
+
+def plan_twice(T, D):
+    """lanes and runs of a workgroup, rows of a run, and the scratch bytes of a forward scan, as the library chooses them."""
+    def shape(threads):
+        cg = -(-D // (4 if D >= 4 else 1))
+        ny = -(-cg // 64)
+        lanes = -(-cg // ny)
+        return ny, lanes, min(threads // lanes, 32)
+
+    def whole(n):
+        return -(-n // 256) * 256
+    ny, lanes, ts = shape(256)
+    run = 128
+    while run > 8 and T * ny < 1024 * run * ts:
+        run //= 2
+    tiles, tiles_one = -(-T // (run * ts)), -(-T // (8 * shape(512)[2]))
+    words, level = 0, 0
+    while (tiles_one - 1) >> (3 * level) > 0:
+        words, level = words + (tiles_one >> (3 * level)) * D, level + 1
+    two = whole(tiles * D * 8) + whole(tiles * D * 4) + whole(tiles * ts * 2 * D * 4)
+    return lanes, ts, run, max(two, 256 + whole(words * 8))
+
+
+def ragged_offsets(T, seed):
+    """Sequences that end at multiples of 8 rows and anywhere, several within 8 rows, some without a row; rows of no sequence at both ends."""
+    rng = np.random.default_rng(seed)
+    n = rng.choice([0, 1, 2, 3, 5, 8, 8, 16, 16, 24, 40, 61], size=T // 8)
+    off = 11 + np.concatenate([[0], np.cumsum(n)])
+    # half of the places are moved to a multiple of 8
+    off = np.maximum.accumulate(np.where(rng.random(off.size) < 0.5, off // 8 * 8, off))
+    off = off[off <= T - 13]
+    return torch.from_numpy(np.ascontiguousarray(off))

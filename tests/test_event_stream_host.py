@@ -174,3 +174,33 @@ def test_event_tokens_of_a_recording():
     for bad in ((t[::-1], x, y, p, 3, 4), (t, x[:4], y, p, 3, 4), (t, x, y, p, 0, 4), (t, x, y, p, 2 ** 15, 2 ** 15)):
         with pytest.raises(ValueError):
             event_tokens(*bad, device="cpu")
+
+
+@pytest.mark.parametrize("kind", ["time", "gate"])
+def test_reference_side_by_side_is_the_reference_row_by_row(kind):
+    g = torch.Generator().manual_seed(3)
+    T, D = 257, 5
+    off = R.ragged_offsets(T, 4)
+    S = off.numel() - 1
+    x, gh = torch.randn(T, D, generator=g), torch.randn(T, D, generator=g)
+    h0, gl = torch.randn(S, D, generator=g), torch.randn(S, D, generator=g)
+    d = dict(dt=torch.rand(T, generator=g), rate=torch.rand(D, generator=g)) if kind == "time" else dict(gate=torch.rand(T, D, generator=g) * 2 - 1)
+    a = R.gates(d.get("gate"), d.get("dt"), d.get("rate"))
+    rows, ends = R.scan(x, a, off.tolist(), h0), R.scan_grad(gh, gl, x, a, d.get("dt"), off.tolist(), h0)
+    mine = R.scan_side_by_side(x, off, h0, **d)
+    back = R.scan_grad_side_by_side(gh, gl, x, mine[2], mine[5], off, **d)
+    for got, want in zip((*mine, *back), (*rows, *ends)):
+        np.testing.assert_allclose(got.numpy(), want, rtol=1e-12, atol=1e-300)
+
+
+def test_shapes_of_many_batches_have_them(L):
+    """The scans that the GPU tests read twice: several batches of 8 rows a run, lanes of one run in two wavefronts, and offsets at
+    multiples of 8 inside of runs whose neighbouring batches have starts or ends too.  The scratch memory that the library asks for
+    tells its plan."""
+    for D, T, _, rows in R.MANY_BATCHES:
+        lanes, ts, run, scratch = R.plan_twice(T, D)
+        assert scratch == L.lens_gated_scan_scratch_bytes(T, D, 0), (D, T)
+        assert run == rows > 8 and any(k * lanes // 64 != ((k + 1) * lanes - 1) // 64 for k in range(ts)), (D, T)
+        off = R.ragged_offsets(T, D)
+        inside = off[(off % 8 == 0) & (off % run != 0)]
+        assert inside.numel() > 500 and int(off[0]) > 0 and int(off[-1]) < T and bool((off[1:] == off[:-1]).any())

@@ -625,3 +625,88 @@ def test_offsets_past_32_bits():
     few = torch.tensor([V - 1, 0, V - 1], device="cuda")
     gt, _ = E().embed_events_grad(x[:3], few, V)
     assert torch.equal(gt[V - 1], x[0].float() + x[2].float()) and torch.equal(gt[0], x[1].float()) and not f64_any(gt[1:V - 1])
+
+
+# ---------------------------------------------------------------------------------- scans of many rows that are read twice
+def guarded(*shape):
+    """A float32 buffer of this shape between rows of sevens, and a check that these are still there."""
+    buf = torch.full((shape[0] + 4, *shape[1:]), 7.0, device="cuda")
+    return buf[2:-2], lambda: bool((buf[:2] == 7.0).all()) and bool((buf[-2:] == 7.0).all())
+
+
+def scan_both_ways_guarded(x, d, off, h0, grad, grad_last):
+    """Forward and backward through the C entry points, `last` and `grad_h0` between guard rows."""
+    from lens_amd import _lib
+    (T, D), S, dev = x.shape, off.numel() - 1, x.get_device()
+    L, size = _lib.lib(), E()._TYPES[x.dtype]
+    h, gx, gr = torch.empty_like(x), torch.empty_like(x), torch.empty(D, device="cuda")
+    marks = torch.empty(-(-T // L.lens_scan_mark_rows(D)), D, device="cuda")
+    last, last_ok = guarded(S, D)
+    g0, g0_ok = guarded(S, D)
+    need = L.lens_gated_scan_scratch_bytes(T, D, 0)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    E()._call("lens_gated_scan", dev, x.data_ptr(), size, D, None, 0, 0, d["dt"].data_ptr(), d["rate"].data_ptr(), off.data_ptr(), S,
+              h0.data_ptr(), T, D, h.data_ptr(), D, 1, last.data_ptr(), marks.data_ptr(), scratch.data_ptr(), need)
+    need = L.lens_gated_scan_scratch_bytes(T, D, 1)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    E()._call("lens_gated_scan_grad", dev, grad.data_ptr(), D, grad_last.data_ptr(), x.data_ptr(), size, D, None, 0, 0, d["dt"].data_ptr(),
+              d["rate"].data_ptr(), off.data_ptr(), S, h0.data_ptr(), marks.data_ptr(), T, D, gx.data_ptr(), D, None, D, gr.data_ptr(),
+              g0.data_ptr(), scratch.data_ptr(), need)
+    assert last_ok() and g0_ok(), "rows in front of or behind the last states, or the gradients of the first, were written"
+    return h, last, gx, gr, g0
+
+
+@pytest.mark.parametrize("D,T,dtype,run", R.MANY_BATCHES)
+def test_scan_of_several_batches_a_run(D, T, dtype, run, monkeypatch):
+    """Runs of several batches whose lanes lie in two wavefronts, sequences that end where batches do and within them, rows of no
+    sequence at both ends: every output, and the same bits again."""
+    monkeypatch.setenv("LENS_AMD_SCAN_LAUNCHES", "3")
+    g = gen(D + T)
+    off = R.ragged_offsets(T, D).cuda()
+    S = off.numel() - 1
+    x, grad, h0, gl = rnd(g, T, D, dtype=dtype), rnd(g, T, D, dtype=dtype), rnd(g, S, D), rnd(g, S, D)
+    d = decays("time", T, D, dtype, g)
+    first = scan_both_ways_guarded(x, d, off, h0, grad, gl)
+    h, last, before, Eh, El, Eb = R.scan_side_by_side(x, off, h0, **d)
+    R.check_all(first[0], h, Eh, "h")
+    R.check_all(first[1], last, El, "last")
+    del h, Eh
+    gx, gr, g0, Eg, Er, E0 = R.scan_grad_side_by_side(grad, gl, x, before, Eb, off, **d)
+    R.check_all(first[2], gx, Eg, "grad_x")
+    R.check_all(first[3], gr, Er, "grad_rate")
+    R.check_all(first[4], g0, E0, "grad_h0")
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(scan_both_ways_guarded(x, d, off, h0, grad, gl), first))
+
+
+@pytest.mark.parametrize("launches", ["1", "3"])
+@pytest.mark.parametrize("T,D", [(700, 64), (81957, 200)])
+def test_scan_of_16_bit_rows_keeps_infinities_in_their_sequence(T, D, launches, monkeypatch):
+    monkeypatch.setenv("LENS_AMD_SCAN_LAUNCHES", launches)
+    g = gen(70)
+    off = [0, 100, 101, 400, 401, T - 50]
+    x, d = rnd(g, T, D, dtype=torch.bfloat16), decays("time", T, D, torch.bfloat16, g)
+    grad, gl, h0 = rnd(g, T, D, dtype=torch.bfloat16), rnd(g, 5, D), rnd(g, 5, D)
+    seq = torch.tensor(off, device="cuda")
+
+    def both():
+        h, last, marks = E().gated_scan(x, seq_off=seq, h0=h0, marks=True, **d)
+        gx, _, g0 = E().gated_scan_grad(grad, x, marks, seq_off=seq, h0=h0, grad_last=gl, **d)
+        return [h, gx], [last, g0]
+    clean = both()
+    for s, bad in ((0, float("inf")), (2, float("nan")), (4, float("-inf")), (None, float("nan"))):
+        i, j = (T - 50, T) if s is None else (off[s], off[s + 1])
+        kept = [t.clone() for t in (x, grad, gl, h0)]
+        x[i:j], grad[i:j] = bad, bad
+        if s is not None:
+            gl[s], h0[s] = bad, bad
+        rows, ends = both()
+        for got, want in zip(rows, clean[0]):
+            assert torch.equal(got[:i], want[:i]) and torch.equal(got[j:T - 50], want[j:T - 50])
+        for got, want in zip(ends, clean[1]):
+            others = [k for k in range(5) if k != s]
+            assert torch.equal(got[others], want[others])
+        if s is not None:
+            assert not bool(torch.isfinite(rows[0][i:j]).all())
+        for t, k in zip((x, grad, gl, h0), kept):
+            t.copy_(k)
