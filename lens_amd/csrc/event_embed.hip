@@ -533,7 +533,9 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     }
     __syncthreads();
     const int64_t t_block = ends[0], r_block = place0 - t_block;
-    const int n_block = (int)(ends[1] - t_block);
+    // no more tokens than places, nor fewer than none: only a list that is not sorted says otherwise
+    const int64_t found = ends[1] - t_block;
+    const int n_block = found < 0 ? 0 : found < here ? (int)found : here;
     for (int i = threadIdx.x; i < n_block; i += 256) {
         const uint64_t e = p.order[t_block + i];
         keys[i] = key_of(p, e);
@@ -594,7 +596,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
         for (int u = 0; u < U; ++u) {
             if (t + u >= t1) break;
             const int key = keys[t + u];
-            while (r < key) end_row();
+            while (r < key && r < r1) end_row();                      // key <= r1 in a sorted list
             if (key >= p.V_rows) {
                 if (WEIGHTS && lane == 0) p.grad_weight[index[t + u]] = 0.0f;
                 continue;

@@ -710,3 +710,48 @@ def test_scan_of_16_bit_rows_keeps_infinities_in_their_sequence(T, D, launches, 
             assert not bool(torch.isfinite(rows[0][i:j]).all())
         for t, k in zip((x, grad, gl, h0), kept):
             t.copy_(k)
+
+
+# ------------------------------------------------------------------------- orders that are not those of the tokens
+def cut_tokens(keys, V, place):
+    """Tokens among the first `place` places of the merged list, as a wavefront of the table gradient searches for them."""
+    lo, hi = 0, min(place, len(keys))
+    while lo < hi:
+        step = (hi - lo + 63) // 64
+        at = lo + (np.arange(64) + 1) * step - 1
+        before = (at < hi) & (at + keys[np.minimum(at, hi - 1)] < place)
+        lo += int(before.sum()) * step
+        hi = min(lo + step - 1, hi)
+    return lo
+
+
+@pytest.mark.parametrize("D,lanes", [(4, 8), (63, 16), (256, 64)])
+def test_table_gradient_of_an_order_that_is_not_sorted(D, lanes):
+    """Wrong sums, but every access inside the buffers and every loop ended; the next call with its own order is right."""
+    from lens_amd import _lib
+    g = gen(D)
+    T, V = 30000, 5000
+    L, per = _lib.lib(), 256 // lanes * 8                                # places a workgroup at this size, 64 a group at most
+    tok = torch.randint(0, V, (T,), generator=g, device="cuda")
+    good = E().sort_events(tok, V)
+    anything = torch.randint(-2**63, 2**63 - 1, (T,), generator=g, device="cuda")
+    orders = [good.flip(0), good[torch.randperm(T, generator=g, device="cuda")], anything, anything.sort().values,
+              torch.full_like(good, 2**63 - 1), torch.where(torch.arange(T, device="cuda") % 2 == 0, V << 32 | 7, good)]
+    grad, table, w = rnd(g, T, D), rnd(g, V, D), rnd(g, T)
+    most = 0
+    for order in orders:
+        keys = (order >> 32).clamp(0, V).cpu().numpy()
+        cuts = [cut_tokens(keys, V, p) for p in range(0, T + V + 1, per)]
+        most = max(most, int(np.diff(cuts).max()))
+        gt, gt_ok = guarded(V, D)
+        gw, gw_ok = guarded(T)
+        need = L.lens_embed_events_grad_scratch_bytes(0, T, V, D)
+        scratch = torch.full((need + 4096,), 7, dtype=torch.uint8, device="cuda")
+        E()._call("lens_embed_events_grad", 0, grad.data_ptr(), 0, D, order.data_ptr(), w.data_ptr(), 0.5, T, V, D, table.data_ptr(), D,
+                  gt.data_ptr(), gw.data_ptr(), scratch.data_ptr(), need)
+        assert gt_ok() and gw_ok() and bool((scratch[need:] == 7).all())
+    assert most > per and (lanes == 8 or most > 8 * per)                # more tokens than places, or than the most that a cut may have
+    gt, gw = E().embed_events_grad(grad, tok, V, weight=w, scale=0.5, table=table, order=good)
+    want, bound, want_w, bound_w = R.embed_grad(grad, tok, V, w, 0.5, table)
+    R.check(gt, want, bound, "table")
+    R.check(gw, want_w, bound_w, "weight")
