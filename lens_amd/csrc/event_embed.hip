@@ -447,8 +447,10 @@ __global__ void __launch_bounds__(FEW_THREADS) k_sort_few(const SortArgs p, uint
 // list: token t stands at place t + key[t], the end of row r behind the last token of r.  A workgroup takes `items` places
 // a group, a group is `G` lanes that hold one row of the table's width, NV vectors each.
 // A row that begins in one group and ends in a later one is joined in LDS, over workgroups by k_grad_join.
+// Rows without events are zeros.  Where events are few, all that lies between two of them is one stretch of the table, which a
+// wavefront or the whole workgroup writes in aligned vectors (grad_gap).
 // Bytes bound a large one: 2000000 x 256 bf16 to 179920 rows 260 us, 4.7 TB/s, and 9 us to join; latency a small one: 30011 x 63
-// f32 to 32768 rows, weights too, 14 and 6 us.
+// f32 to 32768 rows, weights too, 14 and 4 us.
 // ------------------------------------------------------------------------------------------
 constexpr int GRAD_ITEMS = 64, GRAD_U = 4;
 
@@ -463,6 +465,7 @@ struct GradArgs {
     int64_t T, V_rows, ld_grad, ld_table;
     float scale;
     int D, items, blocks;            // blocks: workgroups of k_grad
+    int gap, kept;                   // rows an event from which on zeros are written as stretches; through the caches by how many of 64 workgroups
 };
 
 // A sorted token and its event, kept inside the table and the list whatever order the caller passed.
@@ -513,6 +516,22 @@ __device__ __forceinline__ int channel(int k, int lane, int D, int &skip)
     return c;
 }
 
+// Zeros to n floats from `to` on, by `of` threads: whole vectors of 16 bytes, aligned, and what is left at either end.
+template <bool PAST>
+__device__ __forceinline__ void zeros(float *to, int64_t n, int index, int of)
+{
+    const int most = (int)(-((uintptr_t)to >> 2) & 3), head = n < most ? (int)n : most;
+    const int64_t vectors = (n - head) >> 2;
+    const int tail = (int)(n - head) & 3;
+    if (index < head) to[index] = 0.0f;
+    if (index < tail) to[n - 1 - index] = 0.0f;
+    vec<float, 4> *v = reinterpret_cast<vec<float, 4> *>(to + head);
+    for (int64_t i = index; i < vectors; i += of) {
+        if constexpr (PAST) __builtin_nontemporal_store(vec<float, 4>(0.0f), v + i);
+        else v[i] = vec<float, 4>(0.0f);
+    }
+}
+
 template <int V, int NV, int G, typename X, bool WEIGHTS>
 __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
 {
@@ -542,6 +561,22 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
         index[i] = event_of(p, e);
     }
     __syncthreads();
+    // rows that end here, and whether few of them have events
+    const int64_t rows_end = r_block + (here - n_block) < p.V_rows ? r_block + (here - n_block) : p.V_rows;
+    const bool sparse = n_block * p.gap < here - n_block;
+    if (sparse) {                                    // the rows between two tokens are one stretch of the table
+        const bool share = n_block < 8;              // few stretches: all threads share each; else a wavefront each
+        const int thread = share ? (int)threadIdx.x : (int)threadIdx.x & 63, of = share ? 256 : 64;
+        for (int i = share ? 0 : (int)threadIdx.x >> 6; i <= n_block; i += share ? 1 : 4) {
+            int64_t from = i > 0 ? keys[i - 1] + (int64_t)1 : before_first == r_block ? r_block + 1 : r_block;
+            int64_t to = i < n_block ? keys[i] : rows_end;
+            from = from > r_block ? from : r_block;
+            to = to < rows_end ? to : rows_end;
+            if (from >= to) continue;
+            if ((int)(blockIdx.x & 63) < p.kept) zeros<false>(p.out + from * p.D, (to - from) * p.D, thread, of);
+            else zeros<true>(p.out + from * p.D, (to - from) * p.D, thread, of);
+        }
+    }
     int skip[NV], c[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) c[k] = channel<V, G>(k, lane, p.D, skip[k]);
@@ -559,7 +594,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     const int64_t r0 = r_block + (d0 - t0), r1 = r_block + (d1 - t1);
     int64_t r = r0;
     const bool begun0 = (t0 > 0 ? keys[t0 - 1] : before_first) == r0;     // the row begins before this group
-    bool begun = begun0;
+    bool begun = begun0, any = false;                // any: the row has an event in this group
     Row<V, NV> acc, head;
     acc.zero();
     head.zero();
@@ -567,13 +602,21 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
         if (begun) {
             head = acc;
             begun = false;
-        } else if (r < p.V_rows) {
+        } else if (r < p.V_rows && (any || !sparse)) {
 #pragma unroll
             for (int k = 0; k < NV; ++k)
                 if (skip[k] < V) store_past<V>(p.out + r * p.D + c[k], acc.v[k]);
         }
         acc.zero();
+        any = false;
         ++r;
+    };
+    // the rows in front of row `to`
+    auto end_rows = [&](int64_t to) {
+        while (r < to) {
+            end_row();
+            if (sparse && r < to) r = to;            // these are zeros already
+        }
     };
     for (int t = t0; t < t1; t += U) {
         vec<X, V> g[U][NV], w[WEIGHTS ? U : 1][NV];         // w: of the table
@@ -596,11 +639,12 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
         for (int u = 0; u < U; ++u) {
             if (t + u >= t1) break;
             const int key = keys[t + u];
-            while (r < key && r < r1) end_row();                      // key <= r1 in a sorted list
+            end_rows(key < r1 ? key : r1);                            // key <= r1 in a sorted list
             if (key >= p.V_rows) {
                 if (WEIGHTS && lane == 0) p.grad_weight[index[t + u]] = 0.0f;
                 continue;
             }
+            any = true;
             if constexpr (WEIGHTS) {
                 float dot = 0.0f;
 #pragma unroll
@@ -618,7 +662,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
                 for (int i = 0; i < V; ++i) acc.v[k][i] = __builtin_fmaf(f[u], (float)g[u][k][i], acc.v[k][i]);
         }
     }
-    while (r < r1) end_row();
+    end_rows(r1);
     // rows that groups share
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -802,6 +846,33 @@ int grad_items(int64_t T, int64_t V_rows, int G)
     return items;
 }
 
+// Rows an event from which on a workgroup of k_grad writes the rows without events as stretches, and not one by one with the others.
+// One by one, a store covers 16 bytes of every 32 where a lane holds 8 channels, and lines in parts where rows are not whole vectors;
+// rows of whole vectors lose least by it.  One by one / by this rule, us with the sort, gradients of 179920 rows:
+//            events     1          5000       12000      30000      60000      100000
+//   f32  x 63        25 / 22    31 / 27    33 / 29    41 / 36    59 / 56    60 / 58
+//   f32  x 200       46 / 32    50 / 37    53 / 43    60 / 59    77 / 77    78 / 78
+//   f32  x 293       69 / 40    71 / 45    74 / 50    82 / 58    97 / 84   102 / 97
+//   f32  x 600      116 / 73   118 / 77   118 / 100  123 / 121  137 / 137  145 / 145
+//   bf16 x 200       68 / 32    76 / 37    79 / 41    85 / 49    99 / 70    98 / 90
+//   bf16 x 600      193 / 73   198 / 78   202 / 87   204 / 101  215 / 164  212 / 193
+// Stretches from 8 rows an event on too: f32 x 200, 12000 and 30000 events 40 and 57, 60000 79; x 600 without `kept` 126 and 110 for
+// 90 and 118.  From 4 rows on and not 2: bf16 x 200, 60000 events 92.
+int grad_gap(int type, int D, const float *out)
+{
+    return type == LENS_F32 && D % 4 == 0 && ((uintptr_t)out & 15) == 0 ? 16 : 2;
+}
+
+// Stretches of zeros go through the caches (f32 x 200 and 1 event: 32 us, past them 45), but of a table beyond the 256 MB of the
+// Infinity Cache only 192 MB do.  All through them / 192 MB / 128 MB, us of 179920 rows in f32 and 1 (5000) events:  x 500
+// 80 / 60 / 70 (97 / 65 / 76)   x 600  95 / 73 / 87 (114 / 77 / 91)   x 1500  219 / 238 / 256 (260 / 259 / 271)
+int grad_kept(int64_t V_rows, int D)
+{
+    constexpr int64_t MB = 1 << 20;
+    const int64_t bytes = V_rows * D * 4;
+    return bytes <= 256 * MB ? 64 : (int)(64 * 192 * MB / bytes);
+}
+
 int64_t grad_blocks(int64_t T, int64_t V_rows, int G)
 {
     const int64_t per = (int64_t)(256 / G) * grad_items(T, V_rows, G);
@@ -953,6 +1024,7 @@ int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const 
     p.grad = d_grad; p.table = d_table; p.order = (const uint64_t *)d_order; p.weight = d_weight; p.out = d_grad_table;
     p.grad_weight = d_grad_weight; p.head = (float *)base; p.tail = (float *)(base + up(blocks * D * 4));
     p.first_row = (int64_t *)(base + 2 * up(blocks * D * 4)); p.open = (int32_t *)(base + 2 * up(blocks * D * 4) + up(blocks * 8));
+    p.gap = grad_gap(type, D, d_grad_table); p.kept = grad_kept(n_rows, D);
     p.items = grad_items(T, n_rows, w.G);
     p.blocks = (int)blocks;
     p.T = T; p.V_rows = n_rows; p.ld_grad = ld_grad; p.ld_table = ld_table; p.scale = scale; p.D = D;

@@ -755,3 +755,43 @@ def test_table_gradient_of_an_order_that_is_not_sorted(D, lanes):
     want, bound, want_w, bound_w = R.embed_grad(grad, tok, V, w, 0.5, table)
     R.check(gt, want, bound, "table")
     R.check(gw, want_w, bound_w, "weight")
+
+
+# -------------------------------------------------------------------------------- gradients of tables with few events
+def grad_into(out, grad, tok, V, w, table):
+    """The table's gradient through the C entry point, into a buffer of the caller."""
+    from lens_amd import _lib
+    (T, D), L, size, dev = grad.shape, _lib.lib(), E()._TYPES[grad.dtype], grad.get_device()
+    order, gw = E().sort_events(tok, V), torch.empty(T, device="cuda")
+    need = L.lens_embed_events_grad_scratch_bytes(size, T, V, D)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    E()._call("lens_embed_events_grad", dev, grad.data_ptr(), size, D, order.data_ptr(), w.data_ptr(), 0.5, T, V, D, table.data_ptr(), D,
+              out.data_ptr(), gw.data_ptr(), scratch.data_ptr(), need)
+    return gw
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [1, 3, 4, 7, 8, 63, 64, 200, 293, 600])
+def test_table_gradient_of_few_events(dtype, D):
+    """Every row is written, those between the events too, and nothing around them: rows next to each other, the first and the last,
+    events that stand close in one part of the table and far apart in another, rows that are not aligned to vectors."""
+    for V, tokens in ((1, [0]), (2, [1]), (700, [-1, -1]), (5000, [0]), (5000, [4999]), (5000, [2500, 2499, 2501, -1, 2500]), (5001, [0, 1, 2, 4998, 5000]),
+                      (20011, list(range(3000, 3600)) + [3100] * 300 + list(range(5000, 20011, 777))),
+                      (20011, list(range(0, 20011, 19))), (20011, list(range(5, 20011, 3)) + [11] * 2000)):
+        g = gen(V + D + len(tokens))
+        tok = torch.tensor(tokens, device="cuda")[torch.randperm(len(tokens), generator=g, device="cuda")]
+        grad, table, w = rnd(g, len(tokens), D, dtype=dtype), rnd(g, V, D, dtype=dtype), rnd(g, len(tokens))
+        want, bound, want_w, bound_w = R.embed_grad(grad, tok, V, w, 0.5, table)
+        first = None
+        for shift in (0, 1, 2, 3):
+            buf = torch.full((V * D + 64,), float("nan"), device="cuda")
+            out = buf[32 + shift:32 + shift + V * D].view(V, D)
+            gw = grad_into(out, grad, tok, V, w, table)
+            R.check(out, want, bound, f"table {V} {shift}")
+            R.check(gw, want_w, bound_w, "weight")
+            assert bool(torch.isnan(buf[:32 + shift]).all()) and bool(torch.isnan(buf[32 + shift + V * D:]).all())
+            first = out if first is None else first
+            assert torch.equal(out, first)
+        none = torch.ones(V, dtype=torch.bool, device="cuda")
+        none[tok[tok >= 0]] = False
+        assert not f64_any(first[none])
