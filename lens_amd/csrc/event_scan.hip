@@ -18,7 +18,8 @@
 // A run with the start of a sequence in it does not depend on what enters: it is marked, and the state is selected, not
 // multiplied by zero (an infinity of one sequence must not reach the next).
 //
-// Everything between loads and stores is 32-bit; 16-bit outputs are rounded once, when they are stored.
+// Everything between loads and stores is 32-bit, the sums of grad_rate over runs 64-bit; 16-bit outputs are rounded once, when they
+// are stored.
 // A short decay is evaluated as h + expm1(-dt rate) h: events are microseconds apart and 1 - a would keep only a few
 // bits of a rounded a (a rate of 1 / s and 1 us: 1e-6, against a half step of 3e-8).
 #include <hip/hip_runtime.h>
@@ -126,7 +127,7 @@ struct ScanArgs {
     float *pre;                        // [tiles][ts][2][D] pairs of what is before a run in its tile
     uint64_t *words;                   // one pass: pairs of the tiles and of their groups (Chain)
     unsigned *ticket;
-    float *part;                       // [tiles][D] a tile's share of grad_rate
+    double *part;                      // [tiles][D] a tile's share of grad_rate
     int64_t T;
     int ldx, ldg, ldh, ld_grad, ld_gx, ld_gg;
     int n_seq, D, cg, lanes, ts, run, fill, ny, tiles, levels;
@@ -1128,6 +1129,21 @@ __device__ __forceinline__ void rows_batch(const ScanArgs &p, const Tile &tile, 
     }
 }
 
+// A tile's share of grad_rate from those of its runs: 32 bits over the rows of a run, 64 over runs and tiles (all terms of a long
+// recording may have one sign, and then round the same way).  f: LDS that all threads are done with after a barrier.
+template <int V>
+__device__ __forceinline__ void put_share(const ScanArgs &p, const Own<V> &o, int tile, float *f, int slots, vec<float, V> share)
+{
+    __syncthreads();
+    lds_store<V>(f + o.ts * slots + o.lane * V, share);
+    __syncthreads();
+    if (o.ts != 0 || !o.any) return;
+    vec<double, V> sum(0.0);
+    for (int k = 0; k < p.ts; ++k) sum += __builtin_convertvector(lds_load<V>(f + k * slots + o.lane * V), vec<double, V>);
+    double *to = p.part + (int64_t)tile * p.D + o.c;
+    __builtin_memcpy(to, &sum, sizeof(sum));
+}
+
 template <int V, typename X, typename G>
 __global__ void __launch_bounds__(256) k_scan_back_pairs(const ScanArgs p)
 {
@@ -1191,13 +1207,7 @@ __global__ void __launch_bounds__(256) k_scan_back(const ScanArgs p)
         rows_batch<V, X, G>(p, tile, o, q, ids + b, t, x, d, g, gx, gg, st, r, share);
     }
     if constexpr (__is_same(G, void)) {
-        __syncthreads();
-        lds_store<V>(lds.f + o.ts * lds.slots + o.lane * V, share);
-        __syncthreads();
-        if (o.ts == 0 && o.any) {
-            for (int k = 1; k < p.ts; ++k) share += lds_load<V>(lds.f + k * lds.slots + o.lane * V);
-            store<V>(p.part + (int64_t)index * p.D + o.c, share);
-        }
+        put_share<V>(p, o, index, lds.f, lds.slots, share);
     }
 }
 
@@ -1277,27 +1287,21 @@ __global__ void __launch_bounds__(ONCE, 2) k_scan_back_once(const ScanArgs p)
             }
     }
     if constexpr (__is_same(G, void)) {
-        __syncthreads();
-        lds_store<V>(lds.f + o.ts * lds.slots + o.lane * V, share);
-        __syncthreads();
-        if (o.ts == 0 && o.any) {
-            for (int k = 1; k < p.ts; ++k) share += lds_load<V>(lds.f + k * lds.slots + o.lane * V);
-            store<V>(p.part + (int64_t)index * p.D + o.c, share);
-        }
+        put_share<V>(p, o, index, lds.f, lds.slots, share);
     }
 }
 
 // grad_rate: the tiles' shares, added by 64 runs of tiles side by side and then in their order.
-__global__ void __launch_bounds__(1024) k_scan_rate(const float *__restrict__ part, float *__restrict__ grad_rate, int tiles, int D)
+__global__ void __launch_bounds__(1024) k_scan_rate(const double *__restrict__ part, float *__restrict__ grad_rate, int tiles, int D)
 {
-    __shared__ float sum[64][16];
+    __shared__ double sum[64][16];
     const int lane = threadIdx.x & 15, run = threadIdx.x >> 4;
     const int c = blockIdx.x * 16 + lane;
-    float v = 0.0f;
+    double v = 0.0;
     if (c < D) {
         int i = run;
         for (; i + 7 * 64 < tiles; i += 8 * 64) {
-            float u[8];
+            double u[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) u[k] = part[(int64_t)(i + 64 * k) * D + c];
 #pragma unroll
@@ -1311,7 +1315,7 @@ __global__ void __launch_bounds__(1024) k_scan_rate(const float *__restrict__ pa
         if (run < k) sum[run][lane] += sum[run + k][lane];
         __syncthreads();
     }
-    if (run == 0 && c < D) grad_rate[c] = sum[0][lane];
+    if (run == 0 && c < D) grad_rate[c] = (float)sum[0][lane];
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1425,7 +1429,7 @@ Scratch scratch_of(int64_t T, int D, bool back)
     const size_t end_two = r.pre + whole((size_t)tiles * two.ts * 2 * D * 4);
     const size_t end_one = r.words + whole((size_t)words_of(tiles_one, D, levels) * 8);
     r.part = end_two > end_one ? end_two : end_one;
-    r.bytes = r.part + (back ? whole((size_t)(tiles > tiles_one ? tiles : tiles_one) * D * 4) : 0);
+    r.bytes = r.part + (back ? whole((size_t)(tiles > tiles_one ? tiles : tiles_one) * D * 8) : 0);
     return r;
 }
 
@@ -1457,7 +1461,7 @@ dim3 put_twice(ScanArgs &p, unsigned char *scratch, bool back)
     p.agg = (float2 *)(scratch + r.agg);
     p.entry = (float *)(scratch + r.entry);
     p.pre = (float *)(scratch + r.pre);
-    p.part = (float *)(scratch + r.part);
+    p.part = (double *)(scratch + r.part);
     return dim3((int64_t)p.tiles * 256 > MAX_THREADS ? 0 : p.tiles, s.ny);
 }
 
@@ -1468,7 +1472,7 @@ unsigned put_once(ScanArgs &p, unsigned char *scratch, bool back, int batches)
     put_shape(p, s, batches * B);
     p.ticket = (unsigned *)(scratch + r.ticket);
     p.words = (uint64_t *)(scratch + r.words);
-    p.part = (float *)(scratch + r.part);
+    p.part = (double *)(scratch + r.part);
     words_of(p.tiles, p.D, p.levels);
     const int64_t n = (int64_t)p.tiles * s.ny;
     return n * ONCE > MAX_THREADS ? 0 : (unsigned)n;

@@ -795,3 +795,21 @@ def test_table_gradient_of_few_events(dtype, D):
         none = torch.ones(V, dtype=torch.bool, device="cuda")
         none[tok[tok >= 0]] = False
         assert not f64_any(first[none])
+
+
+# ------------------------------------------------------------------------------------------ gradient of the rates, long sums
+@pytest.mark.parametrize("dtype,launches,run", [(torch.float32, "1", 16), (torch.bfloat16, "1", 16), (torch.bfloat16, "3", 128)])
+@pytest.mark.parametrize("dt", [1.9e-6, 7.3e-6])
+def test_rate_gradient_of_a_long_recording(dtype, launches, run, dt, monkeypatch):
+    """Rates and inputs of zero keep the state and its gradient as they are, so grad_rate is -h0 grad_last sum(dt) and all that may be off
+    is the sum: u for a term's product, u for each of the run's additions in 32 bits, u for the result (64 bits lose nothing here)."""
+    monkeypatch.setenv("LENS_AMD_SCAN_LAUNCHES", launches)
+    T, D = 16 * 1024 * 1024, 4
+    x = torch.zeros(1, D, device="cuda", dtype=dtype).expand(T, D)
+    h0, gl = torch.tensor([[1.0, -1.0, 2.0, 0.5]], device="cuda"), torch.tensor([[1.0, 4.0, 0.25, -1.0]], device="cuda")
+    d = dict(dt=torch.full((T,), dt, device="cuda"), rate=torch.zeros(D, device="cuda"))
+    h, last, marks = E().gated_scan(x, h0=h0, marks=True, **d)
+    gx, gr, g0 = E().gated_scan_grad(None, x, marks, h0=h0, grad_last=gl, **d)
+    assert torch.equal(last, h0) and torch.equal(g0, gl) and bool((h == h0.to(dtype)).all()) and bool((gx == gl.to(dtype)).all())
+    want = -(h0.double() * gl.double())[0] * d["dt"].double().sum()
+    assert bool(((gr.double() - want).abs() <= (run + 3) * R.U * want.abs()).all()), ((gr.double() - want) / want / R.U).tolist()
