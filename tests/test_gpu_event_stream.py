@@ -813,3 +813,22 @@ def test_rate_gradient_of_a_long_recording(dtype, launches, run, dt, monkeypatch
     assert torch.equal(last, h0) and torch.equal(g0, gl) and bool((h == h0.to(dtype)).all()) and bool((gx == gl.to(dtype)).all())
     want = -(h0.double() * gl.double())[0] * d["dt"].double().sum()
     assert bool(((gr.double() - want).abs() <= (run + 3) * R.U * want.abs()).all()), ((gr.double() - want) / want / R.U).tolist()
+
+
+# ------------------------------------------------------------------------------------------ sort, around the longest list of one launch
+@pytest.mark.parametrize("T,V", [(32767, 300), (32768, 300), (32769, 300), (32768, 179920), (32769, 179920), (32768, 2147483000), (32769, 2147483000),
+                                 (20000, 2147482000)])
+def test_sort_at_the_border_of_one_launch(T, V):
+    """Lists that fill every round of the kernel for short lists, and the first that takes the one for long lists: tokens anywhere, all
+    at one row (several chunks in one workgroup), at two, the other way round, and many in a stretch that one workgroup sorts in
+    several digits."""
+    g = gen(T + V)
+    wide = torch.randint(0, V, (T,), generator=g, device="cuda")
+    one = torch.full((T,), V - 1, device="cuda")
+    two = torch.where(torch.rand(T, generator=g, device="cuda") < 0.5, one, one - 1)
+    close = torch.randint(0, min(V, 8000000), (T,), generator=g, device="cuda")
+    outside = torch.where(torch.rand(T, generator=g, device="cuda") < 0.3, torch.full_like(wide, -1), wide)
+    for tok in (wide, one, two, close, outside, torch.arange(T, device="cuda").flip(0) % V, two.int(), wide.int()):
+        key = torch.where(tok >= 0, tok.long(), V)
+        want, at = torch.sort(key, stable=True)
+        assert torch.equal(E().sort_events(tok, V), want << 32 | at)
