@@ -491,20 +491,42 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # LENS_F32,
 
 
 # The checks below are made in one go where nothing is wrong: a call of a few microseconds is mostly its host side.
+_entries = {}
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _call(name, dev, *args):
     """One entry point on the current stream of device `dev` (an index; it need not be the current device)."""
-    fn = getattr(_lib.lib(), name)
-    if dev == torch._C._cuda_getDevice():
-        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.lib(), name)
+    if dev == _current_device():
+        st = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            st = fn(*args, _raw_stream(dev))
     if st:
         _lib.check(st, name)
 
 
 def _addr(t):
     return None if t is None else t.data_ptr()
+
+
+_recording = torch.is_grad_enabled
+
+
+def _unrecorded(call, gradients):
+    """For inputs that require a gradient where autograd records: it would be lost."""
+    raise _lib.LensAmdError(f"{call} is not recorded by autograd, and an input requires a gradient: call it under torch.no_grad() or with "
+                            f"detached tensors; {gradients}")
+
+
+def _needs(*tensors):
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _device(t, name):
@@ -564,7 +586,10 @@ def embed_events(table, tokens, weight=None, scale=1.0, out=None, check=True):
 
     table float32 / bfloat16 / float16 [n_rows, D] (rows may be strided), tokens int32 / int64 [T], weight float32 [T] or None.
     Token -1 is padding and gives a row of zeros.  Any other token outside the table raises IndexError (check=True, which
-    synchronises); with check=False it gives a row of zeros too.  `out` must not overlap the inputs."""
+    synchronises); with check=False it gives a row of zeros too.  `out` must not overlap the inputs.
+    Not recorded by autograd (inputs that require a gradient are refused where it records); gradients: embed_events_grad."""
+    if _recording() and (table.requires_grad or weight is not None and weight.requires_grad or out is not None and out.requires_grad):
+        _unrecorded("embed_events", "embed_events_grad gives the gradients")
     dev = _device(table, "table")
     assert table.dtype in _TYPES and table.dim() == 2, f"table must be [n, D] in float32, bfloat16 or float16, got {list(table.shape)} {table.dtype}"
     V, D = table.shape
@@ -603,7 +628,10 @@ def embed_events_grad(grad, tokens, n_rows, weight=None, scale=1.0, table=None, 
     written, and grad_weight float32 [T] where weight is given -- the table is needed for it -- else None).
 
     Sums are 32-bit and their order is fixed by the tokens: the same call gives the same bits.  order: what
-    sort_events(tokens, n_rows) returned, for a program that passes over the same events again."""
+    sort_events(tokens, n_rows) returned, for a program that passes over the same events again.
+    Not recorded by autograd, like embed_events."""
+    if _recording() and _needs(grad, weight, table):
+        _unrecorded("embed_events_grad", "there are no second derivatives")
     dev = _device(grad, "grad")
     assert grad.dtype in _TYPES and grad.dim() == 2, f"grad must be [T, D] in float32, bfloat16 or float16, got {list(grad.shape)} {grad.dtype}"
     T, D = grad.shape
@@ -666,7 +694,10 @@ def gated_scan(x, gate=None, dt=None, rate=None, seq_off=None, h0=None, out=None
     h0      float32 [S, D], the state before every sequence's first row; None: zeros
     Returns (h [T, D] in x's type, last float32 [S, D]), with marks=True also what gated_scan_grad needs of the states.
     Rows of no sequence are zeros in h; in the caller's `out` (which must not overlap the inputs) they are left as they were.
-    x and gate may be one row expanded to T."""
+    x and gate may be one row expanded to T.
+    Not recorded by autograd (inputs that require a gradient are refused where it records); gradients: gated_scan_grad."""
+    if _recording() and _needs(x, gate, dt, rate, h0, out):
+        _unrecorded("gated_scan", "gated_scan_grad gives the gradients")
     dev = _device(x, "x")
     assert x.dim() == 2 and x.dtype in _TYPES, f"x must be [T, D] in float32, bfloat16 or float16, got {list(x.shape)} {x.dtype}"
     T, D = x.shape
@@ -695,7 +726,10 @@ def gated_scan_grad(grad_h, x, marks, gate=None, dt=None, rate=None, seq_off=Non
     [S, D] of its last states (None: zeros); everything else as it was given there, `marks` as it returned them.
 
     Returns (grad_x [T, D] in x's type, grad_gate [T, D] in the gate's type or grad_rate float32 [D], grad_h0 float32 [S, D] or
-    None where h0 is).  Rows of no sequence get zeros.  There is no gradient for dt, which is recorded."""
+    None where h0 is).  Rows of no sequence get zeros.  There is no gradient for dt, which is measured.
+    Not recorded by autograd, like gated_scan."""
+    if _recording() and _needs(grad_h, x, gate, dt, rate, h0, grad_last):
+        _unrecorded("gated_scan_grad", "there are no second derivatives")
     dev = _device(x, "x")
     assert x.dim() == 2 and x.dtype in _TYPES, f"x must be [T, D] in float32, bfloat16 or float16, got {list(x.shape)} {x.dtype}"
     T, D = x.shape
@@ -718,6 +752,9 @@ def gated_scan_grad(grad_h, x, marks, gate=None, dt=None, rate=None, seq_off=Non
 
 
 def _step(state, x, tokens, weight, scale, gate, dt, rate, out, first_bad):
+    if _recording() and (state.requires_grad or x.requires_grad or rate is not None and rate.requires_grad or
+                         gate is not None and gate.requires_grad or weight is not None and weight.requires_grad):
+        _unrecorded("a single step", "embed_events and gated_scan have gradients")
     dev = _device(state, "state")
     assert state.dim() == 2, f"state must be [n, D], got {list(state.shape)}"
     n, D = state.shape
@@ -742,14 +779,14 @@ def _step(state, x, tokens, weight, scale, gate, dt, rate, out, first_bad):
 
 def gated_step(state, x, gate=None, dt=None, rate=None, out=None):
     """One step of n carried states (float32 [n, D]): a * state + x, gates and x as in gated_scan with one row a state.
-    Written over `state`, or into `out` (float32 [n, D]).  Returns what was written."""
+    Written over `state`, or into `out` (float32 [n, D]).  Returns what was written.  Not recorded by autograd, like gated_scan."""
     return _step(state, x, None, None, 1.0, gate, dt, rate, out, None)
 
 
 def event_step(state, table, tokens, weight=None, scale=1.0, gate=None, dt=None, rate=None, out=None, check=False):
     """One event for each of n carried states, looked up and integrated in one pass: a * state + scale * weight * table[token].
     Arguments as in embed_events and gated_step.  A token -1 only decays its state.  check=True synchronises and raises IndexError
-    for any other token outside the table (its state has then decayed without it)."""
+    for any other token outside the table (its state has then decayed without it).  Not recorded by autograd, like gated_scan."""
     bad = torch.full((1,), INT64_MAX, dtype=torch.int64, device=state.device) if check else None
     out = _step(state, table, tokens, weight, scale, gate, dt, rate, out, bad)
     if check:

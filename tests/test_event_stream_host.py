@@ -204,3 +204,24 @@ def test_shapes_of_many_batches_have_them(L):
         off = R.ragged_offsets(T, D)
         inside = off[(off % 8 == 0) & (off % run != 0)]
         assert inside.numel() > 500 and int(off[0]) > 0 and int(off[-1]) < T and bool((off[1:] == off[:-1]).any())
+
+
+def test_python_callers_refuse_what_autograd_would_lose():
+    """Inputs that require a gradient are refused where autograd records (the check comes before that of the device), and only there."""
+    from lens_amd import engine as E
+    from lens_amd._lib import LensAmdError
+    f, i, v = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32), torch.zeros(4)
+    p, r = torch.zeros(4, 8, requires_grad=True), torch.zeros(8)
+    q, u = torch.zeros(8, requires_grad=True), torch.zeros(4, requires_grad=True)
+    calls = [lambda: E.embed_events(p, i), lambda: E.embed_events(f, i, weight=u), lambda: E.embed_events(f, i, out=p * 1),
+             lambda: E.embed_events_grad(p, i, 4), lambda: E.embed_events_grad(f, i, 4, weight=u, table=f), lambda: E.embed_events_grad(f, i, 4, weight=v, table=p),
+             lambda: E.gated_scan(p, gate=f), lambda: E.gated_scan(f, gate=p), lambda: E.gated_scan(f, dt=v, rate=q), lambda: E.gated_scan(f, dt=u, rate=r),
+             lambda: E.gated_scan(f, gate=f, h0=q[None]), lambda: E.gated_scan_grad(p, f, f, gate=f), lambda: E.gated_scan_grad(f, f, f, gate=p),
+             lambda: E.gated_scan_grad(f, f, f, dt=v, rate=q), lambda: E.gated_scan_grad(f, f, f, gate=f, grad_last=q[None]),
+             lambda: E.gated_step(p, f, gate=f), lambda: E.gated_step(f, p, gate=f), lambda: E.event_step(f, p, i, gate=f),
+             lambda: E.event_step(f, f, i, weight=u, dt=v, rate=r), lambda: E.event_step(f, f, i, dt=v, rate=q, check=True)]
+    for call in calls:
+        with pytest.raises(LensAmdError, match="autograd"):
+            call()
+        with torch.no_grad(), pytest.raises(LensAmdError, match="device"):
+            call()
