@@ -465,7 +465,7 @@ struct GradArgs {
     int64_t T, V_rows, ld_grad, ld_table;
     float scale;
     int D, items, blocks;            // blocks: workgroups of k_grad
-    int gap, kept;                   // rows an event from which on zeros are written as stretches; through the caches by how many of 64 workgroups
+    int gap, filled;                 // rows an event from which on zeros are written as stretches; all zeros are there (k_grad_zeros)
 };
 
 // A sorted token and its event, kept inside the table and the list whatever order the caller passed.
@@ -517,7 +517,6 @@ __device__ __forceinline__ int channel(int k, int lane, int D, int &skip)
 }
 
 // Zeros to n floats from `to` on, by `of` threads: whole vectors of 16 bytes, aligned, and what is left at either end.
-template <bool PAST>
 __device__ __forceinline__ void zeros(float *to, int64_t n, int index, int of)
 {
     const int most = (int)(-((uintptr_t)to >> 2) & 3), head = n < most ? (int)n : most;
@@ -526,10 +525,19 @@ __device__ __forceinline__ void zeros(float *to, int64_t n, int index, int of)
     if (index < head) to[index] = 0.0f;
     if (index < tail) to[n - 1 - index] = 0.0f;
     vec<float, 4> *v = reinterpret_cast<vec<float, 4> *>(to + head);
-    for (int64_t i = index; i < vectors; i += of) {
-        if constexpr (PAST) __builtin_nontemporal_store(vec<float, 4>(0.0f), v + i);
-        else v[i] = vec<float, 4>(0.0f);
-    }
+    for (int64_t i = index; i < vectors; i += of) v[i] = vec<float, 4>(0.0f);
+}
+
+// A thread 16 bytes, the workgroups in the order of the table: 4 KB each reach 6.8 TB/s on tables that memory has to hold, 16 KB
+// 5.9, 64 KB to 1 MB (what a workgroup of k_grad has) 5.4, and 5.0 past the caches (432 MB).
+__global__ void __launch_bounds__(256) k_grad_zeros(float *out, int64_t n)
+{
+    const int most = (int)(-((uintptr_t)out >> 2) & 3), head = n < most ? (int)n : most;      // floats in front of the first aligned vector
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, vectors = (n - head) >> 2;
+    const int tail = (int)(n - head) & 3;
+    if (i < vectors) reinterpret_cast<vec<float, 4> *>(out + head)[i] = vec<float, 4>(0.0f);
+    if (i < head) out[i] = 0.0f;
+    if (i < tail) out[n - 1 - i] = 0.0f;
 }
 
 template <int V, int NV, int G, typename X, bool WEIGHTS>
@@ -563,8 +571,8 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     __syncthreads();
     // rows that end here, and whether few of them have events
     const int64_t rows_end = r_block + (here - n_block) < p.V_rows ? r_block + (here - n_block) : p.V_rows;
-    const bool sparse = n_block * p.gap < here - n_block;
-    if (sparse) {                                    // the rows between two tokens are one stretch of the table
+    const bool sparse = p.filled || n_block * p.gap < here - n_block;
+    if (sparse && !p.filled) {                                    // the rows between two tokens are one stretch of the table
         const bool share = n_block < 8;              // few stretches: all threads share each; else a wavefront each
         const int thread = share ? (int)threadIdx.x : (int)threadIdx.x & 63, of = share ? 256 : 64;
         for (int i = share ? 0 : (int)threadIdx.x >> 6; i <= n_block; i += share ? 1 : 4) {
@@ -572,9 +580,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
             int64_t to = i < n_block ? keys[i] : rows_end;
             from = from > r_block ? from : r_block;
             to = to < rows_end ? to : rows_end;
-            if (from >= to) continue;
-            if ((int)(blockIdx.x & 63) < p.kept) zeros<false>(p.out + from * p.D, (to - from) * p.D, thread, of);
-            else zeros<true>(p.out + from * p.D, (to - from) * p.D, thread, of);
+            if (from < to) zeros(p.out + from * p.D, (to - from) * p.D, thread, of);
         }
     }
     int skip[NV], c[NV];
@@ -846,31 +852,34 @@ int grad_items(int64_t T, int64_t V_rows, int G)
     return items;
 }
 
-// Rows an event from which on a workgroup of k_grad writes the rows without events as stretches, and not one by one with the others.
-// One by one, a store covers 16 bytes of every 32 where a lane holds 8 channels, and lines in parts where rows are not whole vectors;
-// rows of whole vectors lose least by it.  One by one / by this rule, us with the sort, gradients of 179920 rows:
-//            events     1          5000       12000      30000      60000      100000
-//   f32  x 63        25 / 22    31 / 27    33 / 29    41 / 36    59 / 56    60 / 58
-//   f32  x 200       46 / 32    50 / 37    53 / 43    60 / 59    77 / 77    78 / 78
-//   f32  x 293       69 / 40    71 / 45    74 / 50    82 / 58    97 / 84   102 / 97
-//   f32  x 600      116 / 73   118 / 77   118 / 100  123 / 121  137 / 137  145 / 145
-//   bf16 x 200       68 / 32    76 / 37    79 / 41    85 / 49    99 / 70    98 / 90
-//   bf16 x 600      193 / 73   198 / 78   202 / 87   204 / 101  215 / 164  212 / 193
-// Stretches from 8 rows an event on too: f32 x 200, 12000 and 30000 events 40 and 57, 60000 79; x 600 without `kept` 126 and 110 for
-// 90 and 118.  From 4 rows on and not 2: bf16 x 200, 60000 events 92.
-int grad_gap(int type, int D, const float *out)
+// Tables of this size and more do not stay in the 256 MB of the Infinity Cache beside what else a program has.
+bool grad_large(int64_t V_rows, int D) { return V_rows * D * 4 > (int64_t)192 << 20; }
+
+// Whether all zeros are written first, by k_grad_zeros: large tables of at least 8 rows an event (up to what one launch has threads for).
+bool grad_filled(int64_t T, int64_t V_rows, int D)
 {
-    return type == LENS_F32 && D % 4 == 0 && ((uintptr_t)out & 15) == 0 ? 16 : 2;
+    return grad_large(V_rows, D) && T * 8 < V_rows && (V_rows * D + 1023) / 1024 * 256 <= 0xffff0000ll;
 }
 
-// Stretches of zeros go through the caches (f32 x 200 and 1 event: 32 us, past them 45), but of a table beyond the 256 MB of the
-// Infinity Cache only 192 MB do.  All through them / 192 MB / 128 MB, us of 179920 rows in f32 and 1 (5000) events:  x 500
-// 80 / 60 / 70 (97 / 65 / 76)   x 600  95 / 73 / 87 (114 / 77 / 91)   x 1500  219 / 238 / 256 (260 / 259 / 271)
-int grad_kept(int64_t V_rows, int D)
+// Rows an event from which on a workgroup of k_grad writes the rows without events as stretches, and not one by one with the others.
+// One by one, a store covers 16 bytes of every 32 where a lane holds 8 channels, and lines in parts where rows are not whole vectors;
+// f32 rows of whole vectors lose least by it, and past the caches large tables leave these to what is read.
+// One by one / by these rules / plain (zeros and index_add_), us with the sort, 179920 rows, one answer held while the next is made:
+//            events     1               5000               12000              30000              60000
+//   f32  x 63        25 / 22 / 45     31 / 27 / 48       34 / 30 / 45       42 / 36 / 47       59 / 55 / 70
+//   f32  x 200       46 / 33 / 46     50 / 46 / 49       53 / 43 / 59       60 / 58 / 84       77 / 77 / 124
+//   f32  x 293       70 / 50 / 51     72 / 66 / 66       75 / 73 / 82       82 / 82 / 117      97 / 97 / 171
+//   f32  x 600      116 / 84 / 83    119 / 105 / 111    119 / 116 / 138    124 / 125 / 199    167 / 167 / 295
+//   bf16 x 200       72 / 33 / 50     77 / 46 / 52       80 / 53 / 66       84 / 62 / 95       99 / 82 / 138
+//   bf16 x 293      100 / 49 / 53    106 / 64 / 72      109 / 70 / 90      115 / 87 / 129     129 / 111 / 195
+//   bf16 x 600      194 / 83 / 86    199 / 100 / 120    201 / 111 / 151    204 / 143 / 219    215 / 169 / 332
+// Stretches in large f32 tables too: x 293, 30000 and 60000 events 88 and 113; x 600, 30000 events 136.  No zeros first: x 600, 1 and
+// 5000 events 96 and 115; zeros first in all tables: x 200, 1 event 38.
+int grad_gap(int type, int64_t V_rows, int D, const float *out)
 {
-    constexpr int64_t MB = 1 << 20;
-    const int64_t bytes = V_rows * D * 4;
-    return bytes <= 256 * MB ? 64 : (int)(64 * 192 * MB / bytes);
+    if (type != LENS_F32) return 2;
+    if (grad_large(V_rows, D)) return 1 << 16;
+    return D % 4 == 0 && ((uintptr_t)out & 15) == 0 ? 16 : 2;
 }
 
 int64_t grad_blocks(int64_t T, int64_t V_rows, int G)
@@ -883,6 +892,7 @@ template <int V, int NV, int G, typename X>
 int launch_grad(const GradArgs &p, hipStream_t st)
 {
     const dim3 grid((unsigned)grad_blocks(p.T, p.V_rows, G)), block(256);
+    if (p.filled) hipLaunchKernelGGL(k_grad_zeros, dim3((unsigned)((p.V_rows * p.D + 1023) / 1024)), block, 0, st, p.out, p.V_rows * p.D);
     if (p.grad_weight) hipLaunchKernelGGL((k_grad<V, NV, G, X, true>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((k_grad<V, NV, G, X, false>), grid, block, 0, st, p);
     hipLaunchKernelGGL((k_grad_join<V, NV, G>), dim3((p.blocks + 256 / G - 1) / (256 / G)), block, 0, st, p);
@@ -1024,7 +1034,7 @@ int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const 
     p.grad = d_grad; p.table = d_table; p.order = (const uint64_t *)d_order; p.weight = d_weight; p.out = d_grad_table;
     p.grad_weight = d_grad_weight; p.head = (float *)base; p.tail = (float *)(base + up(blocks * D * 4));
     p.first_row = (int64_t *)(base + 2 * up(blocks * D * 4)); p.open = (int32_t *)(base + 2 * up(blocks * D * 4) + up(blocks * 8));
-    p.gap = grad_gap(type, D, d_grad_table); p.kept = grad_kept(n_rows, D);
+    p.gap = grad_gap(type, n_rows, D, d_grad_table); p.filled = grad_filled(T, n_rows, D);
     p.items = grad_items(T, n_rows, w.G);
     p.blocks = (int)blocks;
     p.T = T; p.V_rows = n_rows; p.ld_grad = ld_grad; p.ld_table = ld_table; p.scale = scale; p.D = D;

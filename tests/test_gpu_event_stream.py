@@ -797,6 +797,60 @@ def test_table_gradient_of_few_events(dtype, D):
         assert not f64_any(first[none])
 
 
+def check_rows(out, grad, tok, w, table=None):
+    """Rows with events against sums in 64 bits, all others zero."""
+    V = out.shape[0]
+    rows, at = torch.unique(tok[tok >= 0], return_inverse=True)
+    terms = 0.5 * w[tok >= 0].double()[:, None] * grad[tok >= 0].double()
+    want, mag = (torch.zeros(len(rows), out.shape[1], device="cuda", dtype=torch.float64).index_add_(0, at, v) for v in (terms, terms.abs()))
+    R.check_all(out[rows], want, (len(tok) + 3) * R.U * mag, "rows with events")
+    bounds = [-1, *rows.tolist(), V]
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        for part in out[a + 1:b].split(1 << 17) if b > a + 1 else ():
+            assert int(torch.count_nonzero(part)) == 0, (a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,D", [(170003, 300), (200011, 293), (100003, 601), (30011, 2047), (170003, 296)])
+def test_gradient_of_a_large_table_with_few_events(dtype, V, D):
+    """Tables beyond 192 MB, with few enough events that all zeros are written first, and with a few more."""
+    for tokens in ([0], [V - 1, 7, V - 1, -1, 8], [-1], list(range(1000, 1400)) + [1200] * 100, list(range(0, V, 23)), list(range(3, V, 6))):
+        g = gen(V + len(tokens))
+        tok = torch.tensor(tokens, device="cuda")[torch.randperm(len(tokens), generator=g, device="cuda")]
+        grad, table, w = rnd(g, len(tokens), D, dtype=dtype), rnd(g, V, D, dtype=dtype), rnd(g, len(tokens))
+        for shift in (0, 3):
+            buf = torch.full((V * D + 64,), float("nan"), device="cuda")
+            out = buf[32 + shift:32 + shift + V * D].view(V, D)
+            grad_into(out, grad, tok, V, w, table)
+            assert bool(torch.isnan(buf[:32 + shift]).all()) and bool(torch.isnan(buf[32 + shift + V * D:]).all())
+            if len(tokens) < 600:
+                check_rows(out, grad, tok, w)
+            else:
+                order = torch.argsort(tok)                                 # every row has one event
+                want = 0.5 * w[order].double()[:, None] * grad[order].double()
+                R.check_all(out[tok[order]], want, 4 * R.U * want.abs(), "rows with events")
+                out[tok[order]] = 0
+                assert not f64_any(out)
+
+
+def test_gradient_of_a_table_of_more_threads_than_a_launch_has():
+    """69 GB: more 16-byte zeros than one launch writes."""
+    V, D = 8389000, 2048
+    g = gen(80)
+    tok = torch.tensor([V - 1, 0, 5000000, 0, -1], device="cuda")
+    grad, w = rnd(g, 5, D, dtype=torch.bfloat16), rnd(g, 5)
+    out = torch.empty(V, D, device="cuda")
+    for part in out.split(1 << 20):
+        part.fill_(float("nan"))
+    order = E().sort_events(tok, V)
+    from lens_amd import _lib
+    need = _lib.lib().lens_embed_events_grad_scratch_bytes(1, 5, V, D)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    E()._call("lens_embed_events_grad", 0, grad.data_ptr(), 1, D, order.data_ptr(), w.data_ptr(), 0.5, 5, V, D, None, 0, out.data_ptr(), None,
+              scratch.data_ptr(), need)
+    check_rows(out, grad, tok, w)
+
+
 # ------------------------------------------------------------------------------------------ gradient of the rates, long sums
 @pytest.mark.parametrize("dtype,launches,run", [(torch.float32, "1", 16), (torch.bfloat16, "1", 16), (torch.bfloat16, "3", 128)])
 @pytest.mark.parametrize("dt", [1.9e-6, 7.3e-6])
