@@ -113,17 +113,21 @@ __global__ void __launch_bounds__(256) k_embed(const EmbedArgs p)
 // and more a digit at once instead of 8).
 // Tokens that name no row get the key V_rows and end behind all others.
 // ------------------------------------------------------------------------------------------
-// Latency and the issue of a digit's ballots bound it.  2000000 tokens of 179920 rows (16000000), us, by threads x elements of a
+// Latency and the issue of a digit's ballots bound it.  Long lists, 2000000 tokens of 179920 rows (16000000), us, by threads x elements of a
 // thread:  512 x 8  49 (273)   512 x 4  61 (355)   512 x 6  62 (313)   256 x 16  58 (311)   1024 x 8  51 (279)
 constexpr int SORT_BITS = 9, SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64;
-constexpr int SORT_EACH = 8;         // elements a thread
+constexpr int SORT_EACH = 8;         // elements a thread at most
+// Up to 64 blocks each adds up the counts of those before it by itself, and as long as they are no more they are smaller.  Always three
+// launches a pass, of 4096 elements a block / this / up to 128 blocks, tokens of 179920 rows:  33000  31 / 20 / 20    80000  32 / 23 / 26
+// 160000  33 / 29 / 30    260000  33 / 32 / 36    400000  35 / 35 / 37.   Half of them at one row: 35 / 21, 36 / 25, 37 / 33, 37 / 36.
+constexpr int SORT_DIRECT = 64;
 
 struct SortArgs {
     const void *tokens;              // first pass: the caller's; else NULL
     const uint64_t *from;
     uint64_t *to;
-    int32_t *count;                  // [digits][blocks] counts, then what lies before (k_sort_add)
-    int32_t *total;                  // [digits]
+    int32_t *count;                  // many blocks: [digits][blocks] counts, then what lies before (k_sort_add); few: [blocks][digits] counts
+    int32_t *total;                  // many blocks: [digits]; few: NULL
     int64_t T, V_rows;
     int wide_tokens, shift, bits, blocks;
 };
@@ -144,20 +148,22 @@ __device__ __forceinline__ void sort_elements(const SortArgs &p, int64_t i, int6
     }
 }
 
+template <int EACH>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_count(const SortArgs p)
 {
     __shared__ int n[1 << SORT_BITS];
     const int digits = 1 << p.bits;
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) n[d] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * SORT_THREADS * SORT_EACH + threadIdx.x;
-    uint64_t e[SORT_EACH];
+    const int64_t base = (int64_t)blockIdx.x * SORT_THREADS * EACH + threadIdx.x;
+    uint64_t e[EACH];
     sort_elements(p, base, SORT_THREADS, e);
 #pragma unroll
-    for (int r = 0; r < SORT_EACH; ++r)
+    for (int r = 0; r < EACH; ++r)
         if (base + r * SORT_THREADS < p.T) atomicAdd(&n[(int)(e[r] >> (32 + p.shift)) & (digits - 1)], 1);
     __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) p.count[(int64_t)d * p.blocks + blockIdx.x] = n[d];
+    for (int d = threadIdx.x; d < digits; d += SORT_THREADS)
+        p.count[p.total ? (int64_t)d * p.blocks + blockIdx.x : (int64_t)blockIdx.x * digits + d] = n[d];
 }
 
 // v of every thread -> the sum of those before it; all: the sum of all.
@@ -211,9 +217,10 @@ __device__ __forceinline__ uint64_t lanes_of(int d, int bits, bool in)
     return (uint64_t)hi << 32 | lo;
 }
 
+template <int EACH>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
 {
-    constexpr int EACH = SORT_EACH, BLOCK = SORT_THREADS * EACH;
+    constexpr int BLOCK = SORT_THREADS * EACH;
     __shared__ volatile int n[SORT_WAVES][1 << SORT_BITS];   // a wavefront's elements of a digit so far; then where they start
     __shared__ int start[1 << SORT_BITS], goes[1 << SORT_BITS];   // a digit's elements: where they start in the block, in the list
     __shared__ uint64_t sorted[BLOCK];
@@ -247,13 +254,25 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
     int before = 0, before_here = 0;
     for (int d0 = 0; d0 < digits; d0 += SORT_THREADS) {
         const int d = d0 + threadIdx.x;
-        int mine = 0, all, all_here;
-        if (d < digits)
+        int mine = 0, total = 0, earlier = 0, all, all_here;
+        if (d < digits) {
             for (int k = 0; k < SORT_WAVES; ++k) mine += n[k][d];
-        const int list = sum_before(d < digits ? p.total[d] : 0, part, all);
+            if (p.total) {
+                total = p.total[d];
+                earlier = p.count[(int64_t)d * p.blocks + blockIdx.x];
+            } else {
+#pragma unroll 8
+                for (int b = 0; b < p.blocks; ++b) {
+                    const int c = p.count[(int64_t)b * digits + d];
+                    total += c;
+                    earlier += b < (int)blockIdx.x ? c : 0;
+                }
+            }
+        }
+        const int list = sum_before(total, part, all);
         const int block = sum_before(mine, part, all_here);
         if (d < digits) {
-            goes[d] = before + list + p.count[(int64_t)d * p.blocks + blockIdx.x];
+            goes[d] = before + list + earlier;
             start[d] = before_here + block;
             int at = before_here + block;
             for (int k = 0; k < SORT_WAVES; ++k) {
@@ -822,7 +841,7 @@ size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 struct SortPlan {
     bool few;                        // in one launch
     uint32_t span;                   // then: rows of a workgroup
-    int bits, passes, blocks;
+    int bits, passes, each, blocks;  // each: elements a thread
     size_t other, count, total, bytes;
 };
 
@@ -835,12 +854,25 @@ SortPlan sort_plan(int64_t T, int64_t V_rows)
     while (bits < 31 && ((s.few ? (int64_t)s.span - 1 : V_rows) >> bits) != 0) ++bits;
     s.passes = s.few ? (bits + FEW_BITS - 1) / FEW_BITS : (bits + SORT_BITS - 1) / SORT_BITS;
     s.bits = (bits + s.passes - 1) / s.passes;
-    s.blocks = (int)((T + SORT_THREADS * SORT_EACH - 1) / (SORT_THREADS * SORT_EACH));
+    auto blocks = [&](int each) { return (int)((T + SORT_THREADS * each - 1) / (SORT_THREADS * each)); };
+    s.each = 2;
+    while (s.each < SORT_EACH && blocks(s.each) > SORT_DIRECT) s.each *= 2;
+    s.blocks = blocks(s.each);
     s.other = 0;
     s.count = up((size_t)T * 8);
     s.total = s.count + (s.few ? 0 : up((size_t)s.blocks * 4 << s.bits));
     s.bytes = s.total + (s.few ? 0 : up((size_t)4 << s.bits));
     return s;
+}
+
+// One pass over a digit.
+template <int EACH>
+void launch_sort(const SortArgs &p, dim3 grid, hipStream_t st)
+{
+    const dim3 block(SORT_THREADS);
+    hipLaunchKernelGGL(k_sort_count<EACH>, grid, block, 0, st, p);
+    if (p.total) hipLaunchKernelGGL(k_sort_add, dim3(1 << p.bits), block, 0, st, p.count, p.total, p.blocks);
+    hipLaunchKernelGGL(k_sort_move<EACH>, grid, block, 0, st, p);
 }
 
 // Places a group of k_grad: as many as leave 1024 workgroups, 8 at least.  By this rule / 64 always / 8 always, us with the
@@ -981,22 +1013,23 @@ int lens_sort_tokens(const void *d_tokens, int token_bytes, int64_t T, int64_t n
     p.count = (int32_t *)(base + s.count); p.total = (int32_t *)(base + s.total);
     p.T = T; p.V_rows = n_rows; p.wide_tokens = token_bytes == 8; p.bits = s.bits; p.blocks = s.blocks;
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid(s.blocks), block(SORT_THREADS);
+    const dim3 grid(s.blocks);
     if (s.few) {
         p.tokens = d_tokens;
         p.to = list[1];
         hipLaunchKernelGGL(k_sort_few, dim3((unsigned)((n_rows + s.span) / s.span)), dim3(FEW_THREADS), 0, st, p, list[0], s.span, s.passes);
         return (int)hipGetLastError();
     }
+    if (s.blocks <= SORT_DIRECT) p.total = nullptr;
     for (int i = 0; i < s.passes; ++i) {
         const int to = (s.passes - 1 - i) & 1 ? 0 : 1;                 // the last pass writes the caller's list
         p.tokens = i == 0 ? d_tokens : nullptr;
         p.from = list[to ^ 1];
         p.to = list[to];
         p.shift = i * s.bits;
-        hipLaunchKernelGGL(k_sort_count, grid, block, 0, st, p);
-        hipLaunchKernelGGL(k_sort_add, dim3(1 << s.bits), block, 0, st, p.count, p.total, s.blocks);
-        hipLaunchKernelGGL(k_sort_move, grid, block, 0, st, p);
+        if (s.each == 2) launch_sort<2>(p, grid, st);
+        else if (s.each == 4) launch_sort<4>(p, grid, st);
+        else launch_sort<SORT_EACH>(p, grid, st);
     }
     return (int)hipGetLastError();
 }

@@ -851,6 +851,21 @@ def test_gradient_of_a_table_of_more_threads_than_a_launch_has():
     check_rows(out, grad, tok, w)
 
 
+
+@pytest.mark.parametrize("T", [32769, 33793, 65536, 65537, 131072, 131073, 262143, 262144, 262145, 524289])
+@pytest.mark.parametrize("V", [1, 300, 511, 512, 179920, 40000000])
+def test_sort_at_the_borders_of_blocks(T, V):
+    """Blocks of 1024, 2048 and 4096 tokens, 64 of them and one more, with digits of one bit to nine."""
+    g = gen(T + V)
+    wide = torch.randint(0, V, (T,), generator=g, device="cuda")
+    u = torch.rand(T, generator=g, device="cuda")
+    hot = torch.where(u < 0.5, torch.full_like(wide, V // 2), wide)
+    outside = torch.where(u < 0.3, torch.full_like(wide, -1), wide)
+    for tok in (wide.int(), hot, outside, torch.full_like(wide, V - 1), torch.arange(T, device="cuda").flip(0) % V):
+        want, at = torch.sort(torch.where(tok >= 0, tok.long(), V), stable=True)
+        assert torch.equal(E().sort_events(tok, V), want << 32 | at)
+
+
 # ------------------------------------------------------------------------------------------ gradient of the rates, long sums
 @pytest.mark.parametrize("dtype,launches,run", [(torch.float32, "1", 16), (torch.bfloat16, "1", 16), (torch.bfloat16, "3", 128)])
 @pytest.mark.parametrize("dt", [1.9e-6, 7.3e-6])
