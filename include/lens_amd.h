@@ -371,7 +371,8 @@ int lens_output_counts_dense(const float *d_featspk, int Q, int T, int F, int ld
  * Types: LENS_F32, LENS_BF16 or LENS_F16 where a `type` is passed, float elsewhere.  All arithmetic is 32-bit; a 16-bit
  * output is rounded once.  Leading dimensions count elements; rows are contiguous in their last index and aligned to their
  * elements.  Results do not depend on timing: the same inputs give the same bits.
- * Scratch is the caller's, 16-byte aligned, contents irrelevant; two calls that may overlap need scratch of their own.
+ * Scratch is the caller's, 16-byte aligned, contents irrelevant; two calls that may overlap need scratch of their own (a scan
+ * whose scratch another call writes ends, about a second later at most, with NaN and no error status).
  * ------------------------------------------------------------------------------------------- */
 
 /*
@@ -399,7 +400,8 @@ int lens_sort_tokens(const void *d_tokens, int token_bytes, int64_t T, int64_t n
  *   grad_table[v] = scale * sum_{i : tokens[i] = v} weight[i] * grad[i]          float [n_rows][D], every row written
  *   grad_weight[i] = scale * <grad[i], table[tokens[i]]>                         float [T], optional; 0 for tokens without a row
  * d_grad type [T][ld_grad] (ld_grad 0: one row for all events); d_table is read for grad_weight only.
- * Sums are 32-bit, in an order that the tokens alone fix.  Scratch: lens_embed_events_grad_scratch_bytes(type, T, n_rows, D).
+ * Sums are 32-bit, in an order that the tokens alone fix.  An order that is not that of the tokens gives wrong sums, never an
+ * access outside of the buffers.  Scratch: lens_embed_events_grad_scratch_bytes(type, T, n_rows, D).
  */
 size_t lens_embed_events_grad_scratch_bytes(int type, int64_t T, int64_t n_rows, int D);
 int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const int64_t *d_order,
@@ -419,7 +421,8 @@ int lens_embed_events_grad(const void *d_grad, int type, int64_t ld_grad, const 
  * d_last    float [n_seq][D], the last state of every sequence (h0 for one without rows), in 32 bits
  * d_marks   float [ceil(T / lens_scan_mark_rows(D))][D], optional: what lens_gated_scan_grad needs of the states
  * d_h must not overlap the inputs.  |a| <= 1 is assumed to the extent that the product of the gates over the rows of a
- * sequence must not overflow: products over runs of rows are formed.  Scratch: lens_gated_scan_scratch_bytes(T, D, 0).
+ * sequence must not overflow: products over runs of rows are formed.  An infinite state becomes NaN where such a product is
+ * zero, as 0 * inf does.  Scratch: lens_gated_scan_scratch_bytes(T, D, 0).
  */
 int lens_scan_mark_rows(int D);
 size_t lens_gated_scan_scratch_bytes(int64_t T, int D, int backward);
@@ -432,7 +435,7 @@ int lens_gated_scan(const void *d_x, int x_type, int64_t ldx, const void *d_gate
  * Gradients of lens_gated_scan for the gradients of its states and last states (inputs and d_marks as there):
  *   g_t = grad_h_t + a_{t+1} g_{t+1} (behind a sequence's last row: grad_last);  grad_x = g,  grad_gate = g_t h_{t-1},
  *   grad_rate_d = -sum_t dt_t a_t g_t h_{t-1},  grad_h0 = a g at a sequence's first row (grad_last for one without rows)
- * The states are computed again from the marks, in 32 bits.
+ * The states are computed again from the marks, in 32 bits; grad_rate adds 128 rows at most in 32 bits and these sums in 64.
  * d_grad_h x_type [T][ld_grad] or NULL (zeros; ld_grad 0: one row for all), d_grad_last float [n_seq][D] or NULL (zeros)
  * d_grad_x x_type [T][ld_gx], d_grad_gate gate_type [T][ld_gg] (gates), d_grad_rate float [D] (decays), d_grad_h0 float
  * [n_seq][D] or NULL.  Rows of no sequence get zeros.  Outputs must not overlap the inputs.

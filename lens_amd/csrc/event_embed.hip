@@ -299,9 +299,10 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs p)
 // A list of at most SORT_FEW tokens, in one launch: a workgroup for every `span` rows reads all tokens (240 KB for 30 K events:
 // from L2), counts the smaller ones, picks its own and sorts them by counting their digits -- one pass, unless it has more than
 // 1024 rows.  Against the launches above, us a list of int32 tokens of 32768 rows (of 179920):
-//   500 events  8 / 25 (10 / 26)     5000  9 / 27 (10 / 30)     30011  16 / 30 (17 / 31)     65536  25 / 30 (27 / 31)
-// What a workgroup picks it sorts alone: half of the events at one row cost 41 / 33 (45 / 35) at 30011, 83 / 34 (93 / 35) at
-// 65536, and two rows with all 57 / 34 (64 / 35) and 117 / 34 (132 / 35).  So up to 32 K, where that costs little.
+//   500 events  8 / 16 (10 / 16)     5000  9 / 17 (11 / 17)     16000  11 / 17 (13 / 17)     30011  16 / 20 (18 / 21)
+// What a workgroup picks it sorts alone.  A tenth of the events at one row cost 18 / 21 (21 / 21) at 30011, half of them 41 / 21
+// (45 / 22), and 16 / 18 (19 / 18) at 16000; all at two rows 57 / 21 (65 / 22) and 32 / 18 (36 / 18).  So up to 32 K, where a camera's
+// lists take less by it: a hot pixel has some hundredths of the events.
 constexpr int FEW_THREADS = 1024, FEW_WAVES = FEW_THREADS / 64, FEW_GROUPS = 256, FEW_U = 8, FEW_EACH = 8;
 constexpr int FEW_BITS = 10;                                 // of a digit at most: a thread a digit
 constexpr int64_t SORT_FEW = 32 * FEW_THREADS;
@@ -876,7 +877,7 @@ void launch_sort(const SortArgs &p, dim3 grid, hipStream_t st)
 }
 
 // Places a group of k_grad: as many as leave 1024 workgroups, 8 at least.  By this rule / 64 always / 8 always, us with the
-// sort:  30011 x 63 to 32768 rows  34 / 74 / 35    2000 x 128 to 32768  22 / 27 / 21    2000000 x 256 bf16 to 179920  330 / 329 / 421
+// sort:  30011 x 63 to 32768 rows  30 / 52 / 30    2000 x 128 to 32768  21 / 26 / 21    2000000 x 256 bf16 to 179920  320 / 321 / 360
 int grad_items(int64_t T, int64_t V_rows, int G)
 {
     int items = GRAD_ITEMS;

@@ -551,7 +551,7 @@ __device__ __forceinline__ void join_runs(const ScanArgs &p, const Lds<V> &lds, 
 }
 
 // Tiles' pairs -> what enters every tile.  A workgroup holds 4 channels x 256 runs of up to JOIN tiles at once: every thread joins
-// its run, the 16 runs of a wavefront are joined by shuffles, the 16 wavefronts through LDS.  Latency: 7 us for 1042 tiles of 200
+// its run, the 16 runs of a wavefront are joined by shuffles, the 16 wavefronts through LDS.  Latency: 7 us for 1251 tiles of 200
 // channels.
 constexpr int JOIN = 8;
 
@@ -803,10 +803,12 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
 //   gates                 1048573 x 128 bf16, bf16 gates 184 / 253     30000 x 128 f32, f32 gates 18 / 23
 //   gates, backward        524287 x 256 bf16, bf16 gates 317 / 357 (the backward launches)
 //   f32 rows, decays      262144 x 128  75 / 77    1501 x 200  16 / 18       with gradients  186 / 197  and  40 / 47
-//   16-bit rows, decays   of 128 channels, 4 sequences:  16384  19 / 19    32768  21 / 22    65536  25 / 31    131072  35 / 34
-//                         262144  59 / 56    524288  101 / 87     400009 x 200, 37 sequences  134 / 115
-//       with gradients    16384  42 / 46    32768  48 / 48    65536  59 / 68    131072  86 / 85    262144  155 / 141    524288  277 / 233
-//                         400009 x 200  355 / 292
+//   16-bit rows, decays   of 128 channels, 4 sequences:  16384  18 / 19    32768  21 / 21    65536  23 / 29    131072  32 / 34
+//                         262144  54 / 56    524288  91 / 82     of 200:  40960  24 / 28    81920  33 / 36    163840  58 / 51
+//                         400009 in 37 sequences, of 200  115 / 105, of 63  58 / 57
+//       with gradients    of 128:  16384  42 / 43    32768  47 / 48    65536  55 / 66    131072  82 / 84    262144  144 / 140
+//                         524288  266 / 227    of 200:  40960  58 / 66    81920  85 / 87    163840  152 / 127
+//                         400009 in 37 sequences, of 200  349 / 285, of 63  158 / 132
 // So 16-bit rows with decays -- the fewest bytes for the arithmetic of a row -- are read twice from 16 M elements on, by
 // workgroups that wait for nothing; all others go in one pass.
 //
@@ -970,8 +972,8 @@ __global__ void __launch_bounds__(256) k_scan_clear(uint4 *words, int64_t n, uns
         words[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
 }
 
-// Workgroups of 512 threads; forward at most 128 registers each (two workgroups a CU), backward 256: with three operands and the
-// states it would spill.
+// Workgroups of 512 threads; forward at most 128 registers each (two workgroups a CU), backward 256 (one): with three operands and the
+// states it would spill, and f32 rows with f32 gates in two batches still spill 14 (262144 x 128: 88 us forward, 231 with gradients).
 constexpr int ONCE = 512;
 
 template <int V, int NB, typename X, typename G>
