@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs p)
     // rows that end here, and whether few of them have events
     const int64_t rows_end = r_block + (here - n_block) < p.V_rows ? r_block + (here - n_block) : p.V_rows;
     const bool sparse = p.filled || n_block * p.gap < here - n_block;
-    if (sparse && !p.filled) {                                    // the rows between two tokens are one stretch of the table
+    if (sparse && !p.filled) {                      // the rows between two tokens are one stretch of the table
         const bool share = n_block < 8;              // few stretches: all threads share each; else a wavefront each
         const int thread = share ? (int)threadIdx.x : (int)threadIdx.x & 63, of = share ? 256 : 64;
         for (int i = share ? 0 : (int)threadIdx.x >> 6; i <= n_block; i += share ? 1 : 4) {

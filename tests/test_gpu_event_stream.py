@@ -901,3 +901,47 @@ def test_sort_at_the_border_of_one_launch(T, V):
         key = torch.where(tok >= 0, tok.long(), V)
         want, at = torch.sort(key, stable=True)
         assert torch.equal(E().sort_events(tok, V), want << 32 | at)
+
+
+# ------------------------------------------------------------------------------------- gradients of few events, streams and graphs
+def few_events(seed):
+    """Gradients of 500 events on a table beyond 192 MB, of 40 000 events sorted by small blocks, and of few events among stretches."""
+    g = gen(seed)
+    sets = []
+    for T, V, D, dtype in ((500, 170003, 300, torch.float32), (40000, 5003, 63, torch.bfloat16), (300, 20011, 100, torch.bfloat16)):
+        sets.append((rnd(g, T, D, dtype=dtype), skewed(T, V, g).clamp(max=V - 1), V, rnd(g, T), rnd(g, V, D, dtype=dtype)))
+    return sets
+
+
+def few_gradients(sets):
+    return [t for grad, tok, V, w, table in sets for t in E().embed_events_grad(grad, tok, V, weight=w, table=table)]
+
+
+def test_gradients_of_few_events_in_graphs_and_on_streams():
+    args = few_events(90)
+    few_gradients(args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        out = few_gradients(args)
+    for k in range(4):
+        for mine, theirs in zip(args, few_events(91 + k)):
+            for i in (0, 1, 3, 4):
+                mine[i].copy_(theirs[i])                                   # other events, other tokens
+        want = few_gradients(args)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    other = few_events(99)
+    wants = few_gradients(args), few_gradients(other)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(a):
+            got = few_gradients(args)
+        with torch.cuda.stream(b):
+            got_other = few_gradients(other)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got + got_other, wants[0] + wants[1]))
