@@ -815,6 +815,8 @@ __global__ void __launch_bounds__(256) k_scan_states(const ScanArgs p)
 // What it reaches: 1048573 x 128 bf16 with gates 184 us, 4.4 TB/s of the 805 MB that have to move (torch's copy of 1 GB:
 // 5.0); 262144 x 128 f32 with decays 75 us, 3.6 TB/s: two rounds of workgroups, each of which loads, waits and stores in step.
 // Outputs past the caches: 184 / 192 us with / without, forward and backward of 262144 x 128 f32 186 / 216.
+// Rows that are not whole lines leave little to choose, with / without:  1000003 x 63 with decays f32 147 / 139, bf16 118 / 109, with
+// gradients 378 / 371 and 278 / 278;  215003 x 293  146 / 148, 129 / 123, 377 / 376, 304 / 308;  gates  1000003 x 63  172 / 179, 118 / 114.
 constexpr uint64_t EMPTY = ~0ull;
 constexpr int MOST_TRIES = 1 << 20;
 
