@@ -492,7 +492,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # LENS_F32,
 
 # The checks below are made in one go where nothing is wrong: a call of a few microseconds is mostly its host side.
 _entries = {}
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_current_device, _raw_stream = (getattr(torch._C, n, None) for n in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 
 
 def _call(name, dev, *args):
